@@ -1,0 +1,446 @@
+// client.cu -- the client's token step on the GPU: the head product with a 4-bit table, the choice of
+// the next token, and the look-up of the next embedding row in the same (tied) table.
+//
+// The server returns encrypted normed rows; the client decrypts them, applies the tied head in plaintext
+// (the --dec-out side of gpu_real_model.cu:2444-2533), picks a token (spec_decode/decode_policy.py:37) and
+// embeds it with a row of the same table (ml-eval/fhe_client.py:123-135).
+//
+// All three run on a stream of the caller's choice, allocate nothing and read nothing of the context's
+// chain or keys.
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace fhe {
+
+// one value of a tensor whose type is known at run time (FHE_F32, FHE_F16, FHE_BF16)
+__device__ __forceinline__ float ld_any(const void* p, int type, long long i) {
+    if (type == FHE_F32) return static_cast<const float*>(p)[i];
+    if (type == FHE_F16) return __half2float(static_cast<const __half*>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void st_any(void* p, int type, long long i, float v) {
+    if (type == FHE_F32) static_cast<float*>(p)[i] = v;
+    else if (type == FHE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// ---- products with a 4-bit table -----------------------------------------------------------
+// W[i][c] = s[i][c / group] (q[i][c] - 8); out[r][i] = sum_c x[r][c] W[i][c].  One warp per table row and 8 rows of
+// x: a lane takes 32 columns (one 16-byte load, one scale) at a time, sums them with whole q and applies the scale once.
+constexpr int kQ4Rows = 8;
+
+__global__ void __launch_bounds__(256) k_q4_matvec(const fhe_q4 w, const void* __restrict__ x, int xt, long long ldx,
+                                                   int m, void* __restrict__ out, int ot, long long ldo) {
+    const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int r0 = blockIdx.y * kQ4Rows, mr = min(kQ4Rows, m - r0);
+    if (i >= w.rows) return;
+    float acc[kQ4Rows];
+#pragma unroll
+    for (int r = 0; r < kQ4Rows; r++) acc[r] = 0.f;
+    const uint8_t* qrow = w.q + (long long)i * w.ldq;
+    for (int c0 = lane * 32; c0 < w.cols; c0 += 1024) {
+        const uint4 v = *reinterpret_cast<const uint4*>(qrow + c0 / 2);
+        const float s = ld_any(w.scale, w.scale_type, (long long)i * w.lds + c0 / w.group);
+        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+        const int nc = min(32, w.cols - c0);
+#pragma unroll
+        for (int r = 0; r < kQ4Rows; r++) {
+            if (r >= mr) break;
+            float sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 32; c++)
+                if (c < nc)
+                    sum += (float)((int)(word[c >> 3] >> (4 * (c & 7)) & 15) - 8) *
+                           ld_any(x, xt, (long long)(r0 + r) * ldx + c0 + c);
+            acc[r] += s * sum;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kQ4Rows; r++) {
+        for (int o = 16; o; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
+        if (lane == 0 && r < mr) st_any(out, ot, (long long)(r0 + r) * ldo + i, acc[r]);
+    }
+}
+
+// ---- rows of a 4-bit table by token id --------------------------------------------------------
+// One warp per row; a token outside the table gives zeros.
+__global__ void __launch_bounds__(256) k_q4_rows(const fhe_q4 w, const int64_t* __restrict__ tokens, int m,
+                                                 void* __restrict__ out, int ot, long long ldo) {
+    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= m) return;
+    const int64_t t = tokens[r];
+    const bool in = t >= 0 && t < w.rows;
+    for (int c = lane; c < w.cols; c += 32) {
+        float v = 0.f;
+        if (in) {
+            const int q = w.q[t * w.ldq + c / 2] >> (4 * (c & 1)) & 15;
+            v = (float)(q - 8) * ld_any(w.scale, w.scale_type, t * w.lds + c / w.group);
+        }
+        st_any(out, ot, (long long)r * ldo + c, v);
+    }
+}
+
+// ---- the choice of a token -----------------------------------------------------------------
+// Per row of logits l (NaN counts as -inf), M = max l:
+//   z = (l - M) / T (0 where l = M), e = exp(z), weight w = round(2^40 e), a whole number, so that sums of weights do
+//   not depend on their order; tokens are ranked by l, equal ones by index;
+//   kept: rank < top_k, sum of the weights ranked before < ceil(top_p * the top_k's sum), e >= min_p;
+//   S = sum of the kept weights, the token is the first in index order whose running sum passes floor(u S).
+constexpr int kSampleThreads = 1024, kSampleWarps = kSampleThreads / 32;
+constexpr int kSampleBins = 2048;
+constexpr int kSampleList = 2048;      // tokens of one bin that are ranked against each other directly
+constexpr float kSampleOne = 1099511627776.f;   // 2^40
+// e < 2^-41 rounds to no weight: exp(-29) 2^40 = 0.28, so everything further than 29 T below M is out
+constexpr float kSampleReach = 29.f;
+
+struct SampleArgs {
+    const void* logits;
+    long long ld;
+    int type, rows, vocab;
+    const float* u;
+    const float *temperature, *top_p, *min_p;   // per row, or null: the one value
+    const int32_t* top_k;
+    float temperature1, top_p1, min_p1;
+    int32_t top_k1;
+    int64_t* token;
+    float* logprob;
+};
+
+// larger for what is ranked first: the logit's bits in order, then the lower index
+__device__ __forceinline__ uint64_t sample_rank_key(float x, uint32_t i) {
+    const uint32_t b = __float_as_uint(x + 0.f);   // -0 and 0 are equal
+    const uint32_t k = b & 0x80000000u ? ~b : b | 0x80000000u;
+    return (uint64_t)k << 32 | (0xffffffffu - i);
+}
+
+struct SampleRow {
+    const void* p;
+    int type, v;
+    float top, t, bins_per_unit, reach;
+    __device__ float x(int i) const {
+        const float a = ld_any(p, type, i);
+        return a != a ? -INFINITY : a;
+    }
+    __device__ float z(float a) const { return a == top ? 0.f : __fdiv_rn(a - top, t); }
+    __device__ static uint64_t weight(float e) { return __float2ull_rn(e * kSampleOne); }
+    __device__ float d(float a) const { return a == top ? 0.f : top - a; }
+    __device__ bool counts(float a) const { return a > -INFINITY && d(a) <= reach; }
+    __device__ int bin(float a) const { return min(kSampleBins - 1, (int)(d(a) * bins_per_unit)); }
+};
+
+template <class T, class F>
+__device__ T sample_reduce(T v, F f, T* sh) {
+    for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = sh[threadIdx.x & 31];
+    for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+struct SampleShared {
+    uint64_t sum[kSampleBins];
+    uint32_t count[kSampleBins];
+    uint64_t key[kSampleList], wt[kSampleList];
+    uint64_t red[32];
+    float redf[32];
+    uint32_t n;
+    uint64_t got, got_before;
+    int at;
+};
+
+// The lowest rank key that is still in, among the tokens with keys in [lo, hi], where `want` is a count of tokens (BY_COUNT) or
+// a sum of weights: the first token, in rank order, at which the running count or sum reaches `want` (>= 1).  The running
+// sum of weights before it goes to *before.  0 if it is never reached.
+template <bool BY_COUNT>
+__device__ uint64_t sample_select(const SampleRow& row, SampleShared& sh, uint64_t want, uint64_t* before) {
+    const int tid = threadIdx.x;
+    uint64_t lo = 0, hi = ~0ull, sum_before = 0;
+    bool first = true;
+    while (true) {
+        // histogram of the tokens in [lo, hi]: by distance below the top at first, by rank key after that
+        int shift = 0;
+        if (!first) {
+            const uint64_t range = hi - lo;
+            shift = max(0, 64 - __clzll((long long)range) - 11);
+        }
+        for (int b = tid; b < kSampleBins; b += kSampleThreads) sh.sum[b] = 0, sh.count[b] = 0;
+        if (tid == 0) sh.at = -1, sh.n = 0;
+        __syncthreads();
+        for (int i = tid; i < row.v; i += kSampleThreads) {
+            const float a = row.x(i);
+            if (!row.counts(a)) continue;
+            const uint64_t k = sample_rank_key(a, i);
+            if (k < lo || k > hi) continue;
+            const int b = first ? row.bin(a) : (int)((hi - k) >> shift);
+            atomicAdd(&sh.count[b], 1u);
+            atomicAdd((unsigned long long*)&sh.sum[b], (unsigned long long)row.weight(expf(row.z(a))));
+        }
+        __syncthreads();
+        if (tid == 0) {
+            uint64_t run = 0, s = sum_before;
+            for (int b = 0; b < kSampleBins; b++) {
+                const uint64_t now = BY_COUNT ? sh.count[b] : sh.sum[b];
+                if (run + now >= want) { sh.at = b; sh.got = run; sh.got_before = s; break; }
+                run += now;
+                s += sh.sum[b];
+            }
+            if (sh.at < 0) sh.got_before = s;
+        }
+        __syncthreads();
+        const int at = sh.at;
+        sum_before = sh.got_before;
+        if (at < 0) { *before = sum_before; return 0; }
+        want -= sh.got;
+        const uint32_t n = sh.count[at];
+        if (n <= kSampleList) {
+            for (int i = tid; i < row.v; i += kSampleThreads) {
+                const float a = row.x(i);
+                if (!row.counts(a)) continue;
+                const uint64_t k = sample_rank_key(a, i);
+                if (k < lo || k > hi) continue;
+                const int b = first ? row.bin(a) : (int)((hi - k) >> shift);
+                if (b != at) continue;
+                const uint32_t j = atomicAdd(&sh.n, 1u);
+                sh.key[j] = k;
+                sh.wt[j] = row.weight(expf(row.z(a)));
+            }
+            __syncthreads();
+            // the list's own order: each token sums what is ranked before it
+            for (uint32_t j = tid; j < n; j += kSampleThreads) {
+                const uint64_t k = sh.key[j];
+                uint64_t c = 0, s = 0;
+                for (uint32_t l = 0; l < n; l++)
+                    if (sh.key[l] > k) { c++; s += sh.wt[l]; }
+                const uint64_t run = BY_COUNT ? c : s, own = BY_COUNT ? 1 : sh.wt[j];
+                if (run < want && run + own >= want) { sh.got = k; sh.got_before = sum_before + s; }
+            }
+            __syncthreads();
+            *before = sh.got_before;
+            const uint64_t r = sh.got;
+            __syncthreads();
+            return r;
+        }
+        // too many: their own range of rank keys, in finer bins
+        uint64_t a0 = ~0ull, a1 = 0;
+        for (int i = tid; i < row.v; i += kSampleThreads) {
+            const float a = row.x(i);
+            if (!row.counts(a)) continue;
+            const uint64_t k = sample_rank_key(a, i);
+            if (k < lo || k > hi) continue;
+            const int b = first ? row.bin(a) : (int)((hi - k) >> shift);
+            if (b == at) a0 = min(a0, k), a1 = max(a1, k);
+        }
+        lo = sample_reduce(a0, [](uint64_t p, uint64_t q) { return min(p, q); }, sh.red);
+        hi = sample_reduce(a1, [](uint64_t p, uint64_t q) { return max(p, q); }, sh.red);
+        first = false;
+    }
+}
+
+__global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
+    extern __shared__ __align__(16) uint8_t ssm[];
+    SampleShared& sh = *reinterpret_cast<SampleShared*>(ssm);
+    const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    SampleRow row;
+    row.p = static_cast<const uint8_t*>(a.logits) + (long long)r * a.ld * (a.type == FHE_F32 ? 4 : 2);
+    row.type = a.type;
+    row.v = a.vocab;
+    float t = a.temperature ? a.temperature[r] : a.temperature1;
+    float p = a.top_p ? a.top_p[r] : a.top_p1;
+    float mp = a.min_p ? a.min_p[r] : a.min_p1;
+    int64_t k = a.top_k ? a.top_k[r] : a.top_k1;
+    mp = mp > 0.f ? fminf(mp, 1.f) : 0.f;   // a NaN in the array: off
+    if (!(t > 0.f)) t = 1.f, k = 1;
+    float top = -INFINITY, low = INFINITY;
+    for (int i = tid; i < row.v; i += kSampleThreads) {
+        const float x = row.x(i);
+        top = fmaxf(top, x);
+        if (x > -INFINITY) low = fminf(low, x);
+    }
+    row.top = top = sample_reduce(top, [](float x, float y) { return fmaxf(x, y); }, sh.redf);
+    low = sample_reduce(low, [](float x, float y) { return fminf(x, y); }, sh.redf);
+    if (top == -INFINITY) {
+        if (tid == 0) a.token[r] = -1, a.logprob[r] = -INFINITY;
+        return;
+    }
+    row.t = t;
+    row.reach = kSampleReach * t;
+    const float span = fminf(row.reach, top - low);
+    row.bins_per_unit = span > 0.f ? fminf(kSampleBins / span, 1e30f) : 0.f;
+
+    uint64_t bound = 0, before;
+    const bool by_p = p < 1.f;
+    if (k > 0 && k < row.v) bound = sample_select<true>(row, sh, k, &before);
+    if (by_p) {
+        uint64_t s = 0;
+        for (int i = tid; i < row.v; i += kSampleThreads) {
+            const float x = row.x(i);
+            if (row.counts(x) && sample_rank_key(x, i) >= bound) s += row.weight(expf(row.z(x)));
+        }
+        s = sample_reduce(s, [](uint64_t x, uint64_t y) { return x + y; }, sh.red);
+        const double want = ceil((double)p * (double)s);
+        const uint64_t b = sample_select<false>(row, sh, want > 1.0 ? (uint64_t)want : 1, &before);
+        bound = max(bound, b);
+    }
+    // the kept weights of each warp's stretch of tokens
+    const int per = (row.v + kSampleWarps - 1) / kSampleWarps, i0 = min(row.v, warp * per), i1 = min(row.v, i0 + per);
+    auto kept = [&](int i) -> uint64_t {
+        const float x = row.x(i);
+        if (!row.counts(x) || sample_rank_key(x, i) < bound) return 0;
+        const float e = expf(row.z(x));
+        return e >= mp ? row.weight(e) : 0;
+    };
+    uint64_t mine = 0;
+    for (int i = i0 + lane; i < i1; i += 32) mine += kept(i);
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    __syncthreads();
+    if (lane == 0) sh.red[warp] = mine;
+    __syncthreads();
+    uint64_t total = 0, start = 0;
+    for (int w = 0; w < kSampleWarps; w++) {
+        if (w == warp) start = total;
+        total += sh.red[w];
+    }
+    const float u = fminf(fmaxf(a.u[r], 0.f), 1.f);
+    uint64_t target = (uint64_t)((double)u * (double)total);
+    if (target >= total) target = total - 1;
+    if (target < start || target >= start + mine) return;
+    for (int i = i0; i < i1; i += 32) {
+        const uint64_t w = i + lane < i1 ? kept(i + lane) : 0;
+        uint64_t run = w;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t v = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += v;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, start + run > target);
+        if (past) {
+            if (lane == __ffs(past) - 1) {
+                a.token[r] = i + lane;
+                a.logprob[r] = row.z(row.x(i + lane)) - (float)log((double)total / (double)kSampleOne);
+            }
+            return;
+        }
+        start += __shfl_sync(0xffffffffu, run, 31);
+    }
+}
+
+}  // namespace fhe
+
+// ---- the C ABI --------------------------------------------------------------------------------
+namespace {
+
+int client_type_bytes(int type, const char* what) {
+    if (type != FHE_F32 && type != FHE_F16 && type != FHE_BF16)
+        throw fhe::Error(std::string(what) + ": unknown type", FHE_ERR_ARG);
+    return type == FHE_F32 ? 4 : 2;
+}
+
+// device memory of the context's GPU, aligned to `align` bytes
+void client_ptr(const fhe::Context& c, const void* p, size_t align, const char* what) {
+    cudaPointerAttributes at{};
+    if (!p) throw fhe::Error(std::string(what) + " is null", FHE_ERR_ARG);
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        throw fhe::Error(std::string("cannot query ") + what, FHE_ERR_ARG);
+    }
+    const bool dev = at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged;
+    if (!dev || at.device != c.device)
+        throw fhe::Error(std::string(what) + " is not device memory of the context's GPU", FHE_ERR_ARG);
+    if (reinterpret_cast<uintptr_t>(p) % align)
+        throw fhe::Error(std::string(what) + " is not " + std::to_string(align) + "-byte aligned", FHE_ERR_ARG);
+}
+
+void client_table(const fhe::Context& c, const fhe_q4* w) {
+    REQUIRE(w, "null argument");
+    REQUIRE(w->rows >= 0 && w->cols >= 1, "q4 table: rows >= 0 and cols >= 1");
+    REQUIRE(w->group >= 32 && w->group % 32 == 0, "q4 table: the group is a multiple of 32 columns");
+    REQUIRE(w->ldq % 16 == 0 && w->ldq >= ((long long)w->cols + 31) / 32 * 16,
+            "q4 table: rows are padded to a multiple of 16 bytes (32 columns)");
+    REQUIRE(w->lds >= ((long long)w->cols + w->group - 1) / w->group, "q4 table: a scale for each group of a row");
+    const int sb = client_type_bytes(w->scale_type, "q4 scales");
+    if (!w->rows) return;
+    client_ptr(c, w->q, 16, "q4 table");
+    client_ptr(c, w->scale, sb, "q4 scales");
+}
+
+cudaStream_t client_stream(fhe_ctx* cx, void* stream) {
+    CUDA_CHECK(cudaSetDevice(cx->cx.device));
+    return stream ? static_cast<cudaStream_t>(stream) : cx->cx.stream;
+}
+
+}  // namespace
+
+extern "C" int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_type, long long ldx, int m, void* out,
+                             int out_type, long long ldo, void* stream) {
+    return guard([&] {
+        REQUIRE(cx, "null argument");
+        client_table(cx->cx, w);
+        const int xb = client_type_bytes(x_type, "x"), ob = client_type_bytes(out_type, "out");
+        REQUIRE(m >= 0, "m is negative");
+        REQUIRE(ldx >= w->cols || m <= 1, "x: rows are shorter than the table's columns");
+        REQUIRE(ldo >= w->rows || m <= 1, "out: rows are shorter than the table's rows");
+        if (m == 0 || w->rows == 0) return;
+        client_ptr(cx->cx, x, xb, "x");
+        client_ptr(cx->cx, out, ob, "out");
+        cudaStream_t st = client_stream(cx, stream);
+        REQUIRE((m + fhe::kQ4Rows - 1) / fhe::kQ4Rows <= 65535, "m is too large");
+        fhe::k_q4_matvec<<<dim3((w->rows + 7) / 8, (m + fhe::kQ4Rows - 1) / fhe::kQ4Rows), 256, 0, st>>>(
+            *w, x, x_type, ldx, m, out, out_type, ldo);
+        CUDA_CHECK(cudaGetLastError());
+        cx->cx.launches++;
+    });
+}
+
+extern "C" int fhe_q4_rows(fhe_ctx* cx, const fhe_q4* w, const int64_t* tokens, int m, void* out, int out_type,
+                           long long ldo, void* stream) {
+    return guard([&] {
+        REQUIRE(cx, "null argument");
+        client_table(cx->cx, w);
+        const int ob = client_type_bytes(out_type, "out");
+        REQUIRE(m >= 0, "m is negative");
+        REQUIRE(ldo >= w->cols || m <= 1, "out: rows are shorter than the table's columns");
+        if (m == 0) return;
+        client_ptr(cx->cx, tokens, 8, "tokens");
+        client_ptr(cx->cx, out, ob, "out");
+        cudaStream_t st = client_stream(cx, stream);
+        fhe::k_q4_rows<<<(m + 7) / 8, 256, 0, st>>>(*w, tokens, m, out, out_type, ldo);
+        CUDA_CHECK(cudaGetLastError());
+        cx->cx.launches++;
+    });
+}
+
+extern "C" int fhe_sample(fhe_ctx* cx, const fhe_sample_cfg* cfg, const void* logits, int type, long long ld, int rows,
+                          int vocab, const float* u, int64_t* token, float* logprob, void* stream) {
+    return guard([&] {
+        REQUIRE(cx && cfg, "null argument");
+        const int b = client_type_bytes(type, "logits");
+        REQUIRE(rows >= 0 && vocab >= 1, "sample: rows >= 0 and vocab >= 1");
+        REQUIRE(vocab <= FHE_SAMPLE_MAX_VOCAB, "sample: the vocabulary is above FHE_SAMPLE_MAX_VOCAB");
+        REQUIRE(ld >= vocab || rows <= 1, "logits: rows are shorter than the vocabulary");
+        if (!cfg->temperature) REQUIRE(cfg->temperature_all >= 0.f && cfg->temperature_all <= 1e30f,
+                                       "sample: temperature is a finite number >= 0");
+        if (!cfg->top_k) REQUIRE(cfg->top_k_all >= 0, "sample: top_k >= 0 (0: off)");
+        if (!cfg->top_p) REQUIRE(cfg->top_p_all > 0.f && cfg->top_p_all <= 1.f, "sample: top_p in (0, 1]");
+        if (!cfg->min_p) REQUIRE(cfg->min_p_all >= 0.f && cfg->min_p_all <= 1.f, "sample: min_p in [0, 1]");
+        if (rows == 0) return;
+        client_ptr(cx->cx, logits, b, "logits");
+        client_ptr(cx->cx, u, 4, "u");
+        client_ptr(cx->cx, token, 8, "token");
+        client_ptr(cx->cx, logprob, 4, "logprob");
+        if (cfg->temperature) client_ptr(cx->cx, cfg->temperature, 4, "temperature");
+        if (cfg->top_k) client_ptr(cx->cx, cfg->top_k, 4, "top_k");
+        if (cfg->top_p) client_ptr(cx->cx, cfg->top_p, 4, "top_p");
+        if (cfg->min_p) client_ptr(cx->cx, cfg->min_p, 4, "min_p");
+        cudaStream_t st = client_stream(cx, stream);
+        fhe::SampleArgs a{logits, ld, type, rows, vocab, u, cfg->temperature, cfg->top_p, cfg->min_p, cfg->top_k,
+                          cfg->temperature_all, cfg->top_p_all, cfg->min_p_all, cfg->top_k_all, token, logprob};
+        const size_t smem = sizeof(fhe::SampleShared);
+        CUDA_CHECK(cudaFuncSetAttribute(fhe::k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        fhe::k_sample<<<rows, fhe::kSampleThreads, smem, st>>>(a);
+        CUDA_CHECK(cudaGetLastError());
+        cx->cx.launches++;
+    });
+}

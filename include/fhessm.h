@@ -383,6 +383,56 @@ int fhe_keyswitch_dist(fhe_ctx* cx, uint64_t which, const uint64_t* d_own, int l
 int fhe_keyswitch_noalloc(fhe_ctx* cx, uint64_t which, const uint64_t* d, int level, uint64_t* out0,
                           uint64_t* out1);
 
+/* ---- the client's token step --------------------------------------------------------------
+ * The plaintext end of a tick on the client's GPU: the tied head on the decrypted rows (--dec-out,
+ * gpu_real_model.cu:2444-2533), the choice of the next token (spec_decode/decode_policy.py:37)
+ * and the embedding row that is encrypted next (ml-eval/fhe_client.py:123-135).  Operands are device
+ * memory of the context's GPU; rows are contiguous, ld* is the distance between rows in elements.
+ * Calls are enqueued on `stream` (a cudaStream_t; NULL = the context's own stream,
+ * cudaStreamLegacy / cudaStreamPerThread name those) and allocate nothing.  Operands that are
+ * written must not overlap the others.  m = 0 rows is a valid call that does nothing. */
+#define FHE_F32 0
+#define FHE_F16 1
+#define FHE_BF16 2
+/* a table of rows x cols values in 4 bits: value (i, c) = scale[i * lds + c / group] * (q - 8), q the
+ * low (even c) or high (odd c) half of byte q[i * ldq + c / 2].  Rows start on 16-byte boundaries and
+ * are padded to a multiple of 16 bytes (32 columns; the padding's content does not matter); ldq is
+ * in bytes; group is a multiple of 32 (group >= cols: one scale a row); the last group may be short. */
+typedef struct {
+    const uint8_t* q;
+    const void* scale;
+    int scale_type;      /* FHE_F32, FHE_F16 or FHE_BF16 */
+    int rows, cols, group;
+    long long ldq, lds;
+} fhe_q4;
+/* out[r][i] = sum_c x[r][c] W[i][c] for m rows of x (the head: W is vocabulary x d).  Sums are held in
+ * 32 bits and rounded once to the output's type. */
+int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_type, long long ldx, int m, void* out,
+                  int out_type, long long ldo, void* stream);
+/* out[r] = row tokens[r] of the table; a token outside [0, rows) gives a row of zeros */
+int fhe_q4_rows(fhe_ctx* cx, const fhe_q4* w, const int64_t* tokens, int m, void* out, int out_type, long long ldo,
+                void* stream);
+/* settings of fhe_sample: a device array with a value for each row, or (array NULL) one value for all */
+typedef struct {
+    const float* temperature;   /* 0 (or an array's value that is not above 0): the largest logit, lowest index */
+    const int32_t* top_k;       /* 0: off (an array's negative values too) */
+    const float* top_p;         /* (0, 1]; 1: off; an array's values <= 0 keep one token */
+    const float* min_p;         /* [0, 1] of the largest probability; 0: off */
+    float temperature_all;
+    int32_t top_k_all;
+    float top_p_all, min_p_all;
+} fhe_sample_cfg;
+#define FHE_SAMPLE_MAX_VOCAB (1 << 20)
+/* One token for each row of logits, from the given random number u[r] in [0, 1).  With M the row's largest logit,
+ * z = (l - M) / T and e = exp(z), a token's weight is the whole number round(2^40 e).  Tokens are ranked by
+ * logit, equal ones by index; kept are the first top_k, of these the shortest run whose weights reach top_p of their
+ * sum, and of these the ones with e >= min_p.  token[r] is the first in index order at which the kept weights' running
+ * sum passes u times their sum; logprob[r] its logarithm of probability among the kept.  NaN counts as
+ * -inf (never drawn); a row of nothing else gives token -1 and logprob -inf.  Weights being whole numbers, the token is
+ * the same in every run. */
+int fhe_sample(fhe_ctx* cx, const fhe_sample_cfg* cfg, const void* logits, int type, long long ld, int rows, int vocab,
+               const float* u, int64_t* token, float* logprob, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
