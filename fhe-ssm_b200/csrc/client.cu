@@ -26,41 +26,207 @@ __device__ __forceinline__ void st_any(void* p, int type, long long i, float v) 
 }
 
 // ---- products with a 4-bit table -----------------------------------------------------------
-// W[i][c] = s[i][c / group] (q[i][c] - 8); out[r][i] = sum_c x[r][c] W[i][c].  One warp per table row and 8 rows of
-// x: a lane takes 32 columns (one 16-byte load, one scale) at a time, sums them with whole q and applies the scale once.
-constexpr int kQ4Rows = 8;
+// W[i][c] = s[i][c / group] (q[i][c] - 8); out[r][i] = sum_c x[r][c] W[i][c].
+//
+// Within a group the sum is a product of whole numbers -8..7, which every 16-bit float holds exactly, with x; the
+// scale is applied to the group's sum in float32.  x is cut into bf16 pieces that add up to it exactly (float32: 3 of 8
+// bits, float16: 2, bf16: itself), each piece a column of the matrix product, so nothing is rounded before the
+// float32 sums.
+//
+// k_q4_mma: few columns (one row of x, or some).  What it must read is the table, so a warp streams 16 table rows through a
+// shared-memory ring of its own (cp.async, no block barrier) and multiplies them on the tensor cores (m16n8k16: 16 table
+// rows x 8 columns of pieces); with a CUDA-core product the unpacking and the float32 multiply-adds, 4 instructions
+// a value, would cost more than the table's bytes.  Columns are permuted so that a 32-bit word of
+// 8 values is a lane's share of two steps: the pairs (0,4), (1,5), (2,6), (3,7) come out of the word by one
+// mask each.  KS warps share 16 rows where the table is short, each a part of the columns.
+constexpr int kQ4Warps = 8, kQ4Threads = 32 * kQ4Warps;
+constexpr int kQ4Stage = 8;             // 32-column chunks of a stage
+constexpr int kQ4Stages = 3;
+constexpr int kQ4Pitch = kQ4Stage * 16 + 16;   // bytes of a row in a stage: rows 4 banks apart
+constexpr int kQ4StageBytes = 16 * kQ4Pitch;
+constexpr int kQ4MaxXBytes = 98304;     // shared memory for x's pieces
 
-__global__ void __launch_bounds__(256) k_q4_matvec(const fhe_q4 w, const void* __restrict__ x, int xt, long long ldx,
-                                                   int m, void* __restrict__ out, int ot, long long ldo) {
-    const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int r0 = blockIdx.y * kQ4Rows, mr = min(kQ4Rows, m - r0);
-    if (i >= w.rows) return;
-    float acc[kQ4Rows];
+struct Q4Args {
+    fhe_q4 w;
+    const void* x;
+    int xt, terms, m;
+    long long ldx;
+    void* out;
+    int ot;
+    long long ldo;
+    int kb_chunks;   // chunks of x held at a time
+};
+
+// piece `term` of v (a bf16's bits): the pieces are cut, not rounded, so none overflows; an infinity or NaN is all in the first
+__device__ __forceinline__ uint32_t q4_piece(float v, int term) {
+    uint32_t b = __float_as_uint(v);
+    if ((b & 0x7f800000u) == 0x7f800000u) return term ? 0u : (b & 0x007fffffu ? 0x7fffu : b >> 16);
+    for (int i = 0; i < term; i++) b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
+    return b >> 16;
+}
+
+// 8 values of 4 bits -> bf16 pairs (0,4), (1,5), (2,6), (3,7) of q - 8: 0x4300 is 128, its last bits count in ones
+__device__ __forceinline__ void q4_unpack(uint32_t w, uint32_t* p) {
+    const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
 #pragma unroll
-    for (int r = 0; r < kQ4Rows; r++) acc[r] = 0.f;
-    const uint8_t* qrow = w.q + (long long)i * w.ldq;
-    for (int c0 = lane * 32; c0 < w.cols; c0 += 1024) {
-        const uint4 v = *reinterpret_cast<const uint4*>(qrow + c0 / 2);
-        const float s = ld_any(w.scale, w.scale_type, (long long)i * w.lds + c0 / w.group);
-        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
-        const int nc = min(32, w.cols - c0);
+    for (int i = 0; i < 4; i++) {
+        const uint32_t v = (w >> (4 * i) & 0x000f000fu) | 0x43004300u;
+        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
+        p[i] = *reinterpret_cast<const uint32_t*>(&d);
+    }
+}
+
+__device__ __forceinline__ void q4_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int NT, int KS>
+__global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
+    extern __shared__ __align__(16) uint8_t qsm[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    uint8_t* ring = qsm + warp * (kQ4Stages * kQ4StageBytes);
+    uint4* xs = reinterpret_cast<uint4*>(qsm + kQ4Warps * kQ4Stages * kQ4StageBytes);
+    const int cols = a.w.cols, chunks = (cols + 31) / 32, gpc = a.w.group / 32;
+    const int row0 = (blockIdx.x * (kQ4Warps / KS) + warp / KS) * 16, kq = warp % KS;
+    const int r0 = blockIdx.y * (NT * 8 / a.terms), mr = min(NT * 8 / a.terms, a.m - r0);
+    float acc[NT][4], c[NT][4];
 #pragma unroll
-        for (int r = 0; r < kQ4Rows; r++) {
-            if (r >= mr) break;
-            float sum = 0.f;
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int c = 0; c < 32; c++)
-                if (c < nc)
-                    sum += (float)((int)(word[c >> 3] >> (4 * (c & 7)) & 15) - 8) *
-                           ld_any(x, xt, (long long)(r0 + r) * ldx + c0 + c);
-            acc[r] += s * sum;
+        for (int j = 0; j < 4; j++) acc[n][j] = c[n][j] = 0.f;
+    // rows past the end read the last one and are not stored
+    const long long rg = min(row0 + g, a.w.rows - 1), rh = min(row0 + g + 8, a.w.rows - 1);
+
+    for (int kb0 = 0; kb0 < chunks; kb0 += a.kb_chunks) {
+        const int kb1 = min(chunks, kb0 + a.kb_chunks);
+        // this warp's chunks: its share of the block's, in whole stages
+        const int each = ((kb1 - kb0 + KS - 1) / KS + kQ4Stage - 1) / kQ4Stage * kQ4Stage;
+        const int c0 = min(kb1, kb0 + kq * each), c1 = min(kb1, c0 + each);
+        auto fetch = [&](int s) {
+            // stage s: 16 rows x up to 8 chunks of 16 bytes, 4 copies a lane
+            const int at = c0 + s * kQ4Stage;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = i * 4 + g / 2, ch = (g & 1) * 4 + t;
+                if (at + ch < c1) {
+                    const uint8_t* src = a.w.q + (long long)min(row0 + r, a.w.rows - 1) * a.w.ldq + (at + ch) * 16;
+                    const uint32_t dst =
+                        (uint32_t)__cvta_generic_to_shared(ring + (s % kQ4Stages) * kQ4StageBytes + r * kQ4Pitch + ch * 16);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        const int stages = (c1 - c0 + kQ4Stage - 1) / kQ4Stage;
+        for (int s = 0; s < kQ4Stages - 1; s++) fetch(s);
+        __syncthreads();   // the previous block's pieces are read
+        for (int i = tid; i < (kb1 - kb0) * NT * 32; i += kQ4Threads) {
+            const int l = i & 31, n = (i >> 5) % NT, ch = (i >> 5) / NT;
+            const int col = n * 8 + (l >> 2), r = col / a.terms, term = col - r * a.terms;
+            const int k = (kb0 + ch) * 32 + (l & 3) * 8;
+            uint32_t p[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                p[j] = r < mr && k + j < cols ? q4_piece(ld_any(a.x, a.xt, (r0 + r) * a.ldx + k + j), term) : 0u;
+            xs[i] = make_uint4(p[0] | p[4] << 16, p[1] | p[5] << 16, p[2] | p[6] << 16, p[3] | p[7] << 16);
         }
-    }
+        __syncthreads();
+        for (int s = 0; s < stages; s++) {
+            fetch(s + kQ4Stages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kQ4Stages - 1) : "memory");
+            __syncwarp();
+            const uint8_t* st = ring + (s % kQ4Stages) * kQ4StageBytes;
+            const int at = c0 + s * kQ4Stage, n_ch = min(kQ4Stage, c1 - at);
+            int gi = at / gpc, left = gpc - at % gpc;   // the group and its chunks from here on
+            for (int ch = 0; ch < n_ch; ch++) {
+                uint32_t p[4], q[4];
+                q4_unpack(*reinterpret_cast<const uint32_t*>(st + g * kQ4Pitch + ch * 16 + t * 4), p);
+                q4_unpack(*reinterpret_cast<const uint32_t*>(st + (g + 8) * kQ4Pitch + ch * 16 + t * 4), q);
+                const uint4* xc = xs + (size_t)(at - kb0 + ch) * NT * 32 + lane;
 #pragma unroll
-    for (int r = 0; r < kQ4Rows; r++) {
-        for (int o = 16; o; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
-        if (lane == 0 && r < mr) st_any(out, ot, (long long)(r0 + r) * ldo + i, acc[r]);
+                for (int n = 0; n < NT; n++) {
+                    const uint4 b = xc[n * 32];
+                    q4_mma(c[n], p[0], q[0], p[1], q[1], b.x, b.y);
+                    q4_mma(c[n], p[2], q[2], p[3], q[3], b.z, b.w);
+                }
+                if (--left == 0 || ch == n_ch - 1) {
+                    const float sg = ld_any(a.w.scale, a.w.scale_type, rg * a.w.lds + gi);
+                    const float sh = ld_any(a.w.scale, a.w.scale_type, rh * a.w.lds + gi);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        acc[n][0] += sg * c[n][0];
+                        acc[n][1] += sg * c[n][1];
+                        acc[n][2] += sh * c[n][2];
+                        acc[n][3] += sh * c[n][3];
+                        c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+                    }
+                    gi++;
+                    left = gpc;
+                }
+            }
+            __syncwarp();
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
+    // [KS warps][column][16 rows] of the tile, then the pieces and the warps' parts are added up
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(qsm) + warp * (NT * 8 * 16);
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        so[(n * 8 + 2 * t) * 16 + g] = acc[n][0];
+        so[(n * 8 + 2 * t + 1) * 16 + g] = acc[n][1];
+        so[(n * 8 + 2 * t) * 16 + g + 8] = acc[n][2];
+        so[(n * 8 + 2 * t + 1) * 16 + g + 8] = acc[n][3];
+    }
+    __syncthreads();
+    constexpr int kRows = 16 * (kQ4Warps / KS);
+    for (int i = tid; i < mr * kRows; i += kQ4Threads) {
+        const int r = i / kRows, row = i % kRows, i0 = blockIdx.x * kRows + row;
+        if (i0 >= a.w.rows) continue;
+        const float* sp = reinterpret_cast<const float*>(qsm) + (row >> 4) * KS * (NT * 8 * 16) + (row & 15);
+        float v = 0.f;
+        for (int k = 0; k < KS; k++)
+            for (int j = a.terms - 1; j >= 0; j--) v += sp[k * (NT * 8 * 16) + (r * a.terms + j) * 16];
+        st_any(a.out, a.ot, (long long)(r0 + r) * a.ldo + i0, v);
+    }
+}
+
+template <int NT, int KS>
+static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
+    const int per = NT * 8 / a.terms, tiles = (a.w.rows + 15) / 16, chunks = (a.w.cols + 31) / 32;
+    a.kb_chunks = std::min(chunks, kQ4MaxXBytes / (512 * NT));
+    const size_t smem = (size_t)kQ4Warps * kQ4Stages * kQ4StageBytes + (size_t)a.kb_chunks * NT * 512;
+    CUDA_CHECK(cudaFuncSetAttribute(k_q4_mma<NT, KS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    constexpr int kTiles = kQ4Warps / KS;
+    k_q4_mma<NT, KS><<<dim3((tiles + kTiles - 1) / kTiles, (a.m + per - 1) / per), kQ4Threads, smem, st>>>(a);
+    CUDA_CHECK(cudaGetLastError());
+    cx.launches++;
+}
+
+template <int NT>
+static void q4_mma_split(Context& cx, const Q4Args& a, cudaStream_t st) {
+    // warps enough to keep the loads in flight (16 an SM), but at least a stage of columns for each
+    const int tiles = (a.w.rows + 15) / 16, chunks = (a.w.cols + 31) / 32;
+    int ks = 1;
+    while (ks < 8 && tiles * ks < 148 * 8 && chunks >= 2 * ks * kQ4Stage) ks *= 2;
+    if (ks == 1) q4_mma_launch<NT, 1>(cx, a, st);
+    else if (ks == 2) q4_mma_launch<NT, 2>(cx, a, st);
+    else if (ks == 4) q4_mma_launch<NT, 4>(cx, a, st);
+    else q4_mma_launch<NT, 8>(cx, a, st);
+}
+
+static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
+    a.terms = a.xt == FHE_F32 ? 3 : a.xt == FHE_F16 ? 2 : 1;
+    const int cols = a.m * a.terms;
+    if (cols <= 8) q4_mma_split<1>(cx, a, st);
+    else if (cols <= 16) q4_mma_split<2>(cx, a, st);
+    else if (cols <= 24) q4_mma_split<3>(cx, a, st);
+    else q4_mma_split<6>(cx, a, st);
 }
 
 // ---- rows of a 4-bit table by token id --------------------------------------------------------
@@ -386,11 +552,7 @@ extern "C" int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_
         client_ptr(cx->cx, x, xb, "x");
         client_ptr(cx->cx, out, ob, "out");
         cudaStream_t st = client_stream(cx, stream);
-        REQUIRE((m + fhe::kQ4Rows - 1) / fhe::kQ4Rows <= 65535, "m is too large");
-        fhe::k_q4_matvec<<<dim3((w->rows + 7) / 8, (m + fhe::kQ4Rows - 1) / fhe::kQ4Rows), 256, 0, st>>>(
-            *w, x, x_type, ldx, m, out, out_type, ldo);
-        CUDA_CHECK(cudaGetLastError());
-        cx->cx.launches++;
+        fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0}, st);
     });
 }
 
