@@ -11,6 +11,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace fhe {
 
 // one value of a tensor whose type is known at run time (FHE_F32, FHE_F16, FHE_BF16)
@@ -23,6 +25,16 @@ __device__ __forceinline__ void st_any(void* p, int type, long long i, float v) 
     if (type == FHE_F32) static_cast<float*>(p)[i] = v;
     else if (type == FHE_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Lets kernel K have all the shared memory a block can; asked of the driver once per GPU.
+template <auto K>
+static void client_smem(const Context& cx) {
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = 1ull << cx.device;
+    if (done.load(std::memory_order_relaxed) & bit) return;
+    CUDA_CHECK(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+    done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 // ---- products with a 4-bit table -----------------------------------------------------------
@@ -40,11 +52,12 @@ __device__ __forceinline__ void st_any(void* p, int type, long long i, float v) 
 // 8 values is a lane's share of two steps: the pairs (0,4), (1,5), (2,6), (3,7) come out of the word by one
 // mask each.  KS warps share 16 rows where the table is short, each a part of the columns.
 constexpr int kQ4Warps = 8, kQ4Threads = 32 * kQ4Warps;
-constexpr int kQ4Stage = 8;             // 32-column chunks of a stage
-constexpr int kQ4Stages = 3;
-constexpr int kQ4Pitch = kQ4Stage * 16 + 16;   // bytes of a row in a stage: rows 4 banks apart
+constexpr int kQ4Stage = 4;             // 32-column chunks of a stage
+constexpr int kQ4Stages = 4;
+constexpr int kQ4Pitch = kQ4Stage * 16 + 16;   // bytes of a row in a stage: 20 banks apart, 8 rows x 4 words meet all 32
 constexpr int kQ4StageBytes = 16 * kQ4Pitch;
-constexpr int kQ4MaxXBytes = 98304;     // shared memory for x's pieces
+constexpr int kQ4RingBytes = kQ4Warps * kQ4Stages * kQ4StageBytes;
+constexpr int kQ4MaxBytes = 163840;     // shared memory for x's pieces and the scales
 
 struct Q4Args {
     fhe_q4 w;
@@ -54,15 +67,61 @@ struct Q4Args {
     void* out;
     int ot;
     long long ldo;
-    int kb_chunks;   // chunks of x held at a time
+    int kb_chunks;   // chunks of columns held at a time, a multiple of a stage's unless they are all
+    int kb_groups;   // most groups that one warp's share of them meets
+    int wide;        // rows of x start on 16-byte boundaries
 };
 
-// piece `term` of v (a bf16's bits): the pieces are cut, not rounded, so none overflows; an infinity or NaN is all in the first
-__device__ __forceinline__ uint32_t q4_piece(float v, int term) {
-    uint32_t b = __float_as_uint(v);
-    if ((b & 0x7f800000u) == 0x7f800000u) return term ? 0u : (b & 0x007fffffu ? 0x7fffu : b >> 16);
-    for (int i = 0; i < term; i++) b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
+// The first bf16 piece of v (its bits), and what is left of v: pieces are cut, not rounded, so none overflows; an infinity or
+// NaN is all in the first.
+__device__ __forceinline__ uint32_t q4_piece(float& v) {
+    const uint32_t b = __float_as_uint(v);
+    if ((b & 0x7f800000u) == 0x7f800000u) {
+        v = 0.f;
+        return b & 0x007fffffu ? 0x7fffu : b >> 16;
+    }
+    v -= __uint_as_float(b & 0xffff0000u);
     return b >> 16;
+}
+
+template <class T>
+__device__ __forceinline__ float q4_float(T v);
+template <>
+__device__ __forceinline__ float q4_float(float v) { return v; }
+template <>
+__device__ __forceinline__ float q4_float(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float q4_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Pieces of rows r0..r0+mr of x, chunks kb0..kb1 -> the product's operand [chunk][tile of 8 columns][lane], 16 bytes each:
+// the lane's column (r TERMS + piece) and its 8 values, paired as q4_unpack pairs the table's.
+template <class T, int TERMS>
+__device__ __forceinline__ void q4_cut(const Q4Args& a, uint4* xs, int nt, int r0, int mr, int kb0, int kb1) {
+    for (int i = threadIdx.x; i < (kb1 - kb0) * mr * 4; i += blockDim.x) {
+        const int t = i & 3, r = (i >> 2) % mr, ch = (i >> 2) / mr, k = (kb0 + ch) * 32 + t * 8;
+        const T* src = static_cast<const T*>(a.x) + (r0 + r) * a.ldx + k;
+        float v[8];
+        if (a.wide && k + 8 <= a.w.cols) {
+            T u[8];
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) * 8 / 16; j++)
+                reinterpret_cast<uint4*>(u)[j] = reinterpret_cast<const uint4*>(src)[j];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = q4_float(u[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = k + j < a.w.cols ? q4_float(src[j]) : 0.f;
+        }
+#pragma unroll
+        for (int term = 0; term < TERMS; term++) {
+            uint32_t p[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) p[j] = q4_piece(v[j]);
+            const int col = r * TERMS + term;
+            xs[(ch * nt + (col >> 3)) * 32 + (col & 7) * 4 + t] =
+                make_uint4(p[0] | p[4] << 16, p[1] | p[5] << 16, p[2] | p[6] << 16, p[3] | p[7] << 16);
+        }
+    }
 }
 
 // 8 values of 4 bits -> bf16 pairs (0,4), (1,5), (2,6), (3,7) of q - 8: 0x4300 is 128, its last bits count in ones
@@ -90,7 +149,8 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
     extern __shared__ __align__(16) uint8_t qsm[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t* ring = qsm + warp * (kQ4Stages * kQ4StageBytes);
-    uint4* xs = reinterpret_cast<uint4*>(qsm + kQ4Warps * kQ4Stages * kQ4StageBytes);
+    uint4* xs = reinterpret_cast<uint4*>(qsm + kQ4RingBytes);
+    float* sc = reinterpret_cast<float*>(xs + a.kb_chunks * NT * 32) + warp * 16 * a.kb_groups;   // [group][16 rows]
     const int cols = a.w.cols, chunks = (cols + 31) / 32, gpc = a.w.group / 32;
     const int row0 = (blockIdx.x * (kQ4Warps / KS) + warp / KS) * 16, kq = warp % KS;
     const int r0 = blockIdx.y * (NT * 8 / a.terms), mr = min(NT * 8 / a.terms, a.m - r0);
@@ -100,7 +160,6 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
 #pragma unroll
         for (int j = 0; j < 4; j++) acc[n][j] = c[n][j] = 0.f;
     // rows past the end read the last one and are not stored
-    const long long rg = min(row0 + g, a.w.rows - 1), rh = min(row0 + g + 8, a.w.rows - 1);
 
     for (int kb0 = 0; kb0 < chunks; kb0 += a.kb_chunks) {
         const int kb1 = min(chunks, kb0 + a.kb_chunks);
@@ -108,11 +167,11 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
         const int each = ((kb1 - kb0 + KS - 1) / KS + kQ4Stage - 1) / kQ4Stage * kQ4Stage;
         const int c0 = min(kb1, kb0 + kq * each), c1 = min(kb1, c0 + each);
         auto fetch = [&](int s) {
-            // stage s: 16 rows x up to 8 chunks of 16 bytes, 4 copies a lane
+            // stage s: 16 rows x up to 4 chunks of 16 bytes, 2 copies a lane
             const int at = c0 + s * kQ4Stage;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int r = i * 4 + g / 2, ch = (g & 1) * 4 + t;
+            for (int i = 0; i < 2; i++) {
+                const int r = i * 8 + g, ch = t;
                 if (at + ch < c1) {
                     const uint8_t* src = a.w.q + (long long)min(row0 + r, a.w.rows - 1) * a.w.ldq + (at + ch) * 16;
                     const uint32_t dst =
@@ -124,26 +183,24 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
         };
         const int stages = (c1 - c0 + kQ4Stage - 1) / kQ4Stage;
         for (int s = 0; s < kQ4Stages - 1; s++) fetch(s);
+        const int g0 = c0 / gpc, ng = c1 > c0 ? (c1 - 1) / gpc - g0 + 1 : 0;
+        for (int i = lane; i < ng * 16; i += 32)
+            sc[i] = ld_any(a.w.scale, a.w.scale_type, (long long)min(row0 + (i & 15), a.w.rows - 1) * a.w.lds + g0 + (i >> 4));
         __syncthreads();   // the previous block's pieces are read
-        for (int i = tid; i < (kb1 - kb0) * NT * 32; i += kQ4Threads) {
-            const int l = i & 31, n = (i >> 5) % NT, ch = (i >> 5) / NT;
-            const int col = n * 8 + (l >> 2), r = col / a.terms, term = col - r * a.terms;
-            const int k = (kb0 + ch) * 32 + (l & 3) * 8;
-            uint32_t p[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                p[j] = r < mr && k + j < cols ? q4_piece(ld_any(a.x, a.xt, (r0 + r) * a.ldx + k + j), term) : 0u;
-            xs[i] = make_uint4(p[0] | p[4] << 16, p[1] | p[5] << 16, p[2] | p[6] << 16, p[3] | p[7] << 16);
-        }
+        if (a.xt == FHE_F32) q4_cut<float, 3>(a, xs, NT, r0, mr, kb0, kb1);
+        else if (a.xt == FHE_F16) q4_cut<__half, 2>(a, xs, NT, r0, mr, kb0, kb1);
+        else q4_cut<__nv_bfloat16, 1>(a, xs, NT, r0, mr, kb0, kb1);
         __syncthreads();
+        int gi = 0, left = gpc - c0 % gpc;   // the group and its chunks from here on
         for (int s = 0; s < stages; s++) {
             fetch(s + kQ4Stages - 1);
             asm volatile("cp.async.wait_group %0;" ::"n"(kQ4Stages - 1) : "memory");
             __syncwarp();
             const uint8_t* st = ring + (s % kQ4Stages) * kQ4StageBytes;
             const int at = c0 + s * kQ4Stage, n_ch = min(kQ4Stage, c1 - at);
-            int gi = at / gpc, left = gpc - at % gpc;   // the group and its chunks from here on
-            for (int ch = 0; ch < n_ch; ch++) {
+#pragma unroll
+            for (int ch = 0; ch < kQ4Stage; ch++) {
+                if (ch >= n_ch) break;
                 uint32_t p[4], q[4];
                 q4_unpack(*reinterpret_cast<const uint32_t*>(st + g * kQ4Pitch + ch * 16 + t * 4), p);
                 q4_unpack(*reinterpret_cast<const uint32_t*>(st + (g + 8) * kQ4Pitch + ch * 16 + t * 4), q);
@@ -154,9 +211,8 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
                     q4_mma(c[n], p[0], q[0], p[1], q[1], b.x, b.y);
                     q4_mma(c[n], p[2], q[2], p[3], q[3], b.z, b.w);
                 }
-                if (--left == 0 || ch == n_ch - 1) {
-                    const float sg = ld_any(a.w.scale, a.w.scale_type, rg * a.w.lds + gi);
-                    const float sh = ld_any(a.w.scale, a.w.scale_type, rh * a.w.lds + gi);
+                if (--left == 0 || at + ch == c1 - 1) {
+                    const float sg = sc[gi * 16 + g], sh = sc[gi * 16 + g + 8];
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
                         acc[n][0] += sg * c[n][0];
@@ -198,10 +254,14 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
 
 template <int NT, int KS>
 static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
-    const int per = NT * 8 / a.terms, tiles = (a.w.rows + 15) / 16, chunks = (a.w.cols + 31) / 32;
-    a.kb_chunks = std::min(chunks, kQ4MaxXBytes / (512 * NT));
-    const size_t smem = (size_t)kQ4Warps * kQ4Stages * kQ4StageBytes + (size_t)a.kb_chunks * NT * 512;
-    CUDA_CHECK(cudaFuncSetAttribute(k_q4_mma<NT, KS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int per = NT * 8 / a.terms, tiles = (a.w.rows + 15) / 16, chunks = (a.w.cols + 31) / 32, gpc = a.w.group / 32;
+    // as many columns at a time as fit: 512 bytes a chunk and tile of pieces, 512 a group and chunk of 8 warps' scales
+    const int fit = kQ4MaxBytes / (512 * (NT + 2)) / (KS * kQ4Stage) * (KS * kQ4Stage);
+    a.kb_chunks = std::min(chunks, fit);
+    const int share = ((a.kb_chunks + KS - 1) / KS + kQ4Stage - 1) / kQ4Stage * kQ4Stage;
+    a.kb_groups = std::min((share + gpc - 2) / gpc + 1, (chunks + gpc - 1) / gpc);
+    const size_t smem = kQ4RingBytes + (size_t)a.kb_chunks * NT * 512 + (size_t)a.kb_groups * kQ4Warps * 64;
+    if (smem > 48 * 1024) client_smem<k_q4_mma<NT, KS>>(cx);
     constexpr int kTiles = kQ4Warps / KS;
     k_q4_mma<NT, KS><<<dim3((tiles + kTiles - 1) / kTiles, (a.m + per - 1) / per), kQ4Threads, smem, st>>>(a);
     CUDA_CHECK(cudaGetLastError());
@@ -222,6 +282,8 @@ static void q4_mma_split(Context& cx, const Q4Args& a, cudaStream_t st) {
 
 static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
     a.terms = a.xt == FHE_F32 ? 3 : a.xt == FHE_F16 ? 2 : 1;
+    const long long row = a.ldx * (a.xt == FHE_F32 ? 4 : 2);
+    a.wide = (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(a.m > 1 ? row : 0)) % 16 == 0;
     const int cols = a.m * a.terms;
     if (cols <= 8) q4_mma_split<1>(cx, a, st);
     else if (cols <= 16) q4_mma_split<2>(cx, a, st);
@@ -552,7 +614,7 @@ extern "C" int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_
         client_ptr(cx->cx, x, xb, "x");
         client_ptr(cx->cx, out, ob, "out");
         cudaStream_t st = client_stream(cx, stream);
-        fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0}, st);
+        fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0, 0, 0}, st);
     });
 }
 
@@ -600,7 +662,7 @@ extern "C" int fhe_sample(fhe_ctx* cx, const fhe_sample_cfg* cfg, const void* lo
         fhe::SampleArgs a{logits, ld, type, rows, vocab, u, cfg->temperature, cfg->top_p, cfg->min_p, cfg->top_k,
                           cfg->temperature_all, cfg->top_p_all, cfg->min_p_all, cfg->top_k_all, token, logprob};
         const size_t smem = sizeof(fhe::SampleShared);
-        CUDA_CHECK(cudaFuncSetAttribute(fhe::k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        fhe::client_smem<fhe::k_sample>(cx->cx);
         fhe::k_sample<<<rows, fhe::kSampleThreads, smem, st>>>(a);
         CUDA_CHECK(cudaGetLastError());
         cx->cx.launches++;

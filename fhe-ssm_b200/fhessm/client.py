@@ -62,12 +62,13 @@ def _bad(msg):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream or _LEGACY_STREAM
+    # torch.cuda.current_stream(device).cuda_stream without the Stream object, 2 us of a call's 8
+    return torch._C._cuda_getCurrentRawStream(device) or _LEGACY_STREAM
 
 
-def _on_gpu(cx, t, what):
-    if t.device.type != "cuda" or t.device.index != cx.p.device:
-        raise _bad(f"{what} is not on the context's GPU (cuda:{cx.p.device})")
+def _on_gpu(device, t, what):
+    if t.get_device() != device or t.device.type != "cuda":
+        raise _bad(f"{what} is not on the context's GPU (cuda:{device})")
 
 
 def _rows_of(t, what):
@@ -91,7 +92,7 @@ class Q4Table:
     weight[i, c // 2].  weight: uint8 (rows, bytes), a row padded to a multiple of 16 bytes;
     scale: float32, float16 or bfloat16 (rows, ceil(cols / group)); group: a multiple of 32."""
 
-    __slots__ = ("weight", "scale", "rows", "cols", "group", "c")
+    __slots__ = ("weight", "scale", "rows", "cols", "group", "c", "ref")
 
     def __init__(self, weight, scale, *, cols, group):
         if weight.dtype != torch.uint8 or weight.dim() != 2:
@@ -113,6 +114,7 @@ class Q4Table:
             raise _bad("q4 table: rows overlap")
         self.weight, self.scale, self.rows, self.cols, self.group = weight, scale, rows, cols, group
         self.c = Q4C(weight.data_ptr(), scale.data_ptr(), st, rows, cols, group, ldq, lds)
+        self.ref = C.byref(self.c)
 
     @classmethod
     def quantise(cls, w, *, group=64, scale_dtype=torch.float16, device="cpu"):
@@ -141,12 +143,17 @@ class Q4Table:
         return q * self.scale.float().repeat_interleave(self.group, dim=1)[:, :self.cols]
 
 
-def _out(out, shape, dtype, device, what):
+def _out(out, like, shape, dtype, device):
+    """(output, its type, its row stride): a new one, or the caller's."""
+    if dtype not in _TYPES:
+        raise _bad(f"out: float32, float16 or bfloat16, got {dtype}")
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype), _TYPES[dtype], shape[1]
     if tuple(out.shape) != shape or out.dtype != dtype:
-        raise _bad(f"{what}: expected {dtype} {shape}, got {out.dtype} {tuple(out.shape)}")
-    return out
+        raise _bad(f"out: expected {dtype} {shape}, got {out.dtype} {tuple(out.shape)}")
+    _on_gpu(device, out, "out")
+    ot, _, _, ldo = _rows_of(out, "out")
+    return out, ot, ldo
 
 
 def q4_matvec(cx, x, table, *, dtype=torch.float32, out=None):
@@ -155,13 +162,12 @@ def q4_matvec(cx, x, table, *, dtype=torch.float32, out=None):
     xt, m, k, ldx = _rows_of(x, "x")
     if k != table.cols:
         raise _bad(f"x has {k} columns, the table {table.cols}")
-    _on_gpu(cx, x, "x")
-    _on_gpu(cx, table.weight, "q4 table")
-    out = _out(out, (m, table.rows), dtype, x.device, "out")
-    _on_gpu(cx, out, "out")
-    ot, _, _, ldo = _rows_of(out, "out")
-    _check(_sigs().fhe_q4_matvec(cx.h, C.byref(table.c), x.data_ptr(), xt, ldx, m, out.data_ptr(), ot, ldo,
-                                 _stream(x.device)))
+    device = cx.p.device
+    _on_gpu(device, x, "x")
+    _on_gpu(device, table.weight, "q4 table")
+    out, ot, ldo = _out(out, x, (m, table.rows), dtype, device)
+    _check((_fns or _sigs()).fhe_q4_matvec(cx.h, table.ref, x.data_ptr(), xt, ldx, m, out.data_ptr(), ot, ldo,
+                                           _stream(device)))
     return out
 
 
@@ -170,23 +176,23 @@ def q4_rows(cx, tokens, table, *, dtype=torch.float32, out=None):
     outside the table (the -1 of an empty row) gives zeros."""
     if tokens.dim() != 1 or tokens.dtype != torch.int64 or (tokens.numel() > 1 and tokens.stride(0) != 1):
         raise _bad("tokens: a contiguous int64 vector")
-    _on_gpu(cx, tokens, "tokens")
-    _on_gpu(cx, table.weight, "q4 table")
-    out = _out(out, (tokens.shape[0], table.cols), dtype, tokens.device, "out")
-    _on_gpu(cx, out, "out")
-    ot, m, _, ldo = _rows_of(out, "out")
-    _check(_sigs().fhe_q4_rows(cx.h, C.byref(table.c), tokens.data_ptr(), m, out.data_ptr(), ot, ldo,
-                               _stream(tokens.device)))
+    device = cx.p.device
+    _on_gpu(device, tokens, "tokens")
+    _on_gpu(device, table.weight, "q4 table")
+    m = tokens.shape[0]
+    out, ot, ldo = _out(out, tokens, (m, table.cols), dtype, device)
+    _check((_fns or _sigs()).fhe_q4_rows(cx.h, table.ref, tokens.data_ptr(), m, out.data_ptr(), ot, ldo,
+                                         _stream(device)))
     return out
 
 
-def _setting(cx, v, rows, dtype, what):
+def _setting(device, v, rows, dtype, what):
     """(device pointer or None, plain value) of a setting given as one number or as a value per row."""
     if not torch.is_tensor(v):
         return None, v
     if v.dim() != 1 or v.shape[0] != rows or v.dtype != dtype or (rows > 1 and v.stride(0) != 1):
         raise _bad(f"{what}: one number, or a contiguous {dtype} vector with a value for each row")
-    _on_gpu(cx, v, what)
+    _on_gpu(device, v, what)
     return v.data_ptr(), 0
 
 
@@ -196,21 +202,21 @@ def sample(cx, logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     one number or a vector with a value for each row (float32; top_k int32).  temperature 0: the
     largest logit.  top_k 0, top_p 1 and min_p 0 are off.  The token of a row that allows none is -1."""
     lt, rows, vocab, ld = _rows_of(logits, "logits")
-    _on_gpu(cx, logits, "logits")
+    device = cx.p.device
+    _on_gpu(device, logits, "logits")
     if not 1 <= vocab <= MAX_VOCAB:
         raise _bad(f"logits: a vocabulary of 1 to {MAX_VOCAB}")
-    up, _ = _setting(cx, u, rows, torch.float32, "u")
+    up, _ = _setting(device, u, rows, torch.float32, "u")
     if up is None:
         raise _bad("u: a float32 vector with a random number for each row")
-    t, t1 = _setting(cx, temperature, rows, torch.float32, "temperature")
-    k, k1 = _setting(cx, top_k, rows, torch.int32, "top_k")
-    p, p1 = _setting(cx, top_p, rows, torch.float32, "top_p")
-    mp, mp1 = _setting(cx, min_p, rows, torch.float32, "min_p")
-    token = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    t, t1 = _setting(device, temperature, rows, torch.float32, "temperature")
+    k, k1 = _setting(device, top_k, rows, torch.int32, "top_k")
+    p, p1 = _setting(device, top_p, rows, torch.float32, "top_p")
+    mp, mp1 = _setting(device, min_p, rows, torch.float32, "min_p")
+    token, logprob = u.new_empty(rows, dtype=torch.int64), u.new_empty(rows)
     cfg = SampleC(t, k, p, mp, t1, min(k1, vocab), p1, mp1)
-    _check(_sigs().fhe_sample(cx.h, C.byref(cfg), logits.data_ptr(), lt, ld, rows, vocab, up, token.data_ptr(),
-                              logprob.data_ptr(), _stream(logits.device)))
+    _check((_fns or _sigs()).fhe_sample(cx.h, C.byref(cfg), logits.data_ptr(), lt, ld, rows, vocab, up,
+                                        token.data_ptr(), logprob.data_ptr(), _stream(device)))
     return token, logprob
 
 
