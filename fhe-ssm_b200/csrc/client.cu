@@ -50,7 +50,7 @@ static void client_smem(const Context& cx) {
 // rows x 8 columns of pieces); with a CUDA-core product the unpacking and the float32 multiply-adds, 4 instructions
 // a value, would cost more than the table's bytes.  Columns are permuted so that a 32-bit word of
 // 8 values is a lane's share of two steps: the pairs (0,4), (1,5), (2,6), (3,7) come out of the word by one
-// mask each.  KS warps share 16 rows where the table is short, each a part of the columns.
+// mask each.  Several warps share 16 rows where the table is short, each a part of the columns.
 constexpr int kQ4Warps = 8, kQ4Threads = 32 * kQ4Warps;
 constexpr int kQ4Stage = 4;             // 32-column chunks of a stage
 constexpr int kQ4Stages = 4;
@@ -67,8 +67,11 @@ struct Q4Args {
     void* out;
     int ot;
     long long ldo;
-    int kb_chunks;   // chunks of columns held at a time, a multiple of a stage's unless they are all
-    int kb_groups;   // most groups that one warp's share of them meets
+    int per;         // rows of x that a block takes
+    int ks_log2;     // 2^ks_log2 warps share a row tile's columns
+    int kb_chunks;   // chunks of columns held at a time, in whole stages for each of these warps
+    int units;       // scales that a warp holds for each row
+    uint32_t group_magic;   // chunk / (chunks of a group) = chunk * magic >> 32 (both at most 2^15); 0: a group is a chunk
     int wide;        // rows of x start on 16-byte boundaries
 };
 
@@ -97,8 +100,14 @@ __device__ __forceinline__ float q4_float(__nv_bfloat16 v) { return __bfloat162f
 // the lane's column (r TERMS + piece) and its 8 values, paired as q4_unpack pairs the table's.
 template <class T, int TERMS>
 __device__ __forceinline__ void q4_cut(const Q4Args& a, uint4* xs, int nt, int r0, int mr, int kb0, int kb1) {
-    for (int i = threadIdx.x; i < (kb1 - kb0) * mr * 4; i += blockDim.x) {
-        const int t = i & 3, r = (i >> 2) % mr, ch = (i >> 2) / mr, k = (kb0 + ch) * 32 + t * 8;
+    // a warp takes 8 chunks of a row at a time
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    int r = threadIdx.x >> 5, ch = lane >> 2;
+    for (;; r += kQ4Warps) {
+        while (r >= mr) r -= mr, ch += 8;
+        if (ch - (lane >> 2) >= kb1 - kb0) break;
+        if (ch >= kb1 - kb0) continue;
+        const int k = (kb0 + ch) * 32 + t * 8;
         const T* src = static_cast<const T*>(a.x) + (r0 + r) * a.ldx + k;
         float v[8];
         if (a.wide && k + 8 <= a.w.cols) {
@@ -135,101 +144,113 @@ __device__ __forceinline__ void q4_unpack(uint32_t w, uint32_t* p) {
     }
 }
 
-__device__ __forceinline__ void q4_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
+__device__ __forceinline__ void q4_mma(float* d, const float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                       uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};\n"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "{%10, %11, %12, %13};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-template <int NT, int KS>
+// Scales of 16 rows (from row0) for `units` units of P chunks from chunk c0 -> sc[unit][row]; 0 past the last column
+template <class S, int P>
+__device__ __forceinline__ void q4_scales(const fhe_q4& w, uint32_t magic, float* sc, int row0, int c0, int units,
+                                          int chunks) {
+    const int lane = threadIdx.x & 31;
+    const S* src = static_cast<const S*>(w.scale) + (long long)min(row0 + (lane & 15), w.rows - 1) * w.lds;
+#pragma unroll 4
+    for (int u = lane >> 4; u < units; u += 2) {
+        const int ch = c0 + u * P;
+        sc[u * 16 + (lane & 15)] = ch < chunks ? q4_float(src[magic ? __umulhi(ch, magic) : ch]) : 0.f;
+    }
+}
+
+// NT: tiles of 8 columns.  P: chunks after which the scale is applied, the largest of 1, 2, 4 that divides a group's.
+template <int NT, int P>
 __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
     extern __shared__ __align__(16) uint8_t qsm[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t* ring = qsm + warp * (kQ4Stages * kQ4StageBytes);
     uint4* xs = reinterpret_cast<uint4*>(qsm + kQ4RingBytes);
-    float* sc = reinterpret_cast<float*>(xs + a.kb_chunks * NT * 32) + warp * 16 * a.kb_groups;   // [group][16 rows]
-    const int cols = a.w.cols, chunks = (cols + 31) / 32, gpc = a.w.group / 32;
-    const int row0 = (blockIdx.x * (kQ4Warps / KS) + warp / KS) * 16, kq = warp % KS;
-    const int r0 = blockIdx.y * (NT * 8 / a.terms), mr = min(NT * 8 / a.terms, a.m - r0);
-    float acc[NT][4], c[NT][4];
+    const int chunks = (a.w.cols + 31) / 32;
+    const int ks = 1 << a.ks_log2, rows = 16 * kQ4Warps >> a.ks_log2;   // warps on a tile, table rows of a block
+    const int row0 = blockIdx.x * rows + (warp >> a.ks_log2) * 16, kq = warp & (ks - 1);
+    const int r0 = blockIdx.y * a.per, mr = min(a.per, a.m - r0);
+    float* sc = reinterpret_cast<float*>(xs + a.kb_chunks * NT * 32) + warp * 16 * a.units;   // [unit][16 rows]
+    float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[n][j] = c[n][j] = 0.f;
-    // rows past the end read the last one and are not stored
+        for (int j = 0; j < 4; j++) acc[n][j] = 0.f;
+    // a lane copies 16 bytes of rows g and g + 8 a stage; rows past the end read the last one and are not stored
+    const uint8_t* src0 = a.w.q + (long long)min(row0 + g, a.w.rows - 1) * a.w.ldq;
+    const uint8_t* src1 = a.w.q + (long long)min(row0 + g + 8, a.w.rows - 1) * a.w.ldq;
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring) + g * kQ4Pitch + t * 16;
+    const uint8_t* words = ring + g * kQ4Pitch + t * 4;
 
     for (int kb0 = 0; kb0 < chunks; kb0 += a.kb_chunks) {
-        const int kb1 = min(chunks, kb0 + a.kb_chunks);
-        // this warp's chunks: its share of the block's, in whole stages
-        const int each = ((kb1 - kb0 + KS - 1) / KS + kQ4Stage - 1) / kQ4Stage * kQ4Stage;
-        const int c0 = min(kb1, kb0 + kq * each), c1 = min(kb1, c0 + each);
+        // the last block may pass the end: values and scales are 0 there
+        const int kb1 = kb0 + a.kb_chunks, each = a.kb_chunks >> a.ks_log2, stages = each / kQ4Stage;
+        const int c0 = kb0 + kq * each, c1 = c0 + each;
         auto fetch = [&](int s) {
-            // stage s: 16 rows x up to 4 chunks of 16 bytes, 2 copies a lane
-            const int at = c0 + s * kQ4Stage;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int r = i * 8 + g, ch = t;
-                if (at + ch < c1) {
-                    const uint8_t* src = a.w.q + (long long)min(row0 + r, a.w.rows - 1) * a.w.ldq + (at + ch) * 16;
-                    const uint32_t dst =
-                        (uint32_t)__cvta_generic_to_shared(ring + (s % kQ4Stages) * kQ4StageBytes + r * kQ4Pitch + ch * 16);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-                }
+            const int at = c0 + s * kQ4Stage + t;
+            if (at < min(c1, chunks)) {
+                const uint32_t d = dst + (s % kQ4Stages) * kQ4StageBytes;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src0 + at * 16) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + 8 * kQ4Pitch), "l"(src1 + at * 16)
+                             : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        const int stages = (c1 - c0 + kQ4Stage - 1) / kQ4Stage;
+#pragma unroll
         for (int s = 0; s < kQ4Stages - 1; s++) fetch(s);
-        const int g0 = c0 / gpc, ng = c1 > c0 ? (c1 - 1) / gpc - g0 + 1 : 0;
-        for (int i = lane; i < ng * 16; i += 32)
-            sc[i] = ld_any(a.w.scale, a.w.scale_type, (long long)min(row0 + (i & 15), a.w.rows - 1) * a.w.lds + g0 + (i >> 4));
+        if (a.w.scale_type == FHE_F16) q4_scales<__half, P>(a.w, a.group_magic, sc, row0, c0, (c1 - c0) / P, chunks);
+        else if (a.w.scale_type == FHE_BF16) q4_scales<__nv_bfloat16, P>(a.w, a.group_magic, sc, row0, c0, (c1 - c0) / P, chunks);
+        else q4_scales<float, P>(a.w, a.group_magic, sc, row0, c0, (c1 - c0) / P, chunks);
         __syncthreads();   // the previous block's pieces are read
         if (a.xt == FHE_F32) q4_cut<float, 3>(a, xs, NT, r0, mr, kb0, kb1);
         else if (a.xt == FHE_F16) q4_cut<__half, 2>(a, xs, NT, r0, mr, kb0, kb1);
         else q4_cut<__nv_bfloat16, 1>(a, xs, NT, r0, mr, kb0, kb1);
         __syncthreads();
-        int gi = 0, left = gpc - c0 % gpc;   // the group and its chunks from here on
+        const uint4* xc = xs + (size_t)(c0 - kb0) * NT * 32 + lane;
+        const float* su = sc + g;
         for (int s = 0; s < stages; s++) {
             fetch(s + kQ4Stages - 1);
             asm volatile("cp.async.wait_group %0;" ::"n"(kQ4Stages - 1) : "memory");
             __syncwarp();
-            const uint8_t* st = ring + (s % kQ4Stages) * kQ4StageBytes;
-            const int at = c0 + s * kQ4Stage, n_ch = min(kQ4Stage, c1 - at);
+            const uint8_t* st = words + (s % kQ4Stages) * kQ4StageBytes;
+            constexpr float zero[4] = {0.f, 0.f, 0.f, 0.f};
+            float c[NT][4];
 #pragma unroll
             for (int ch = 0; ch < kQ4Stage; ch++) {
-                if (ch >= n_ch) break;
                 uint32_t p[4], q[4];
-                q4_unpack(*reinterpret_cast<const uint32_t*>(st + g * kQ4Pitch + ch * 16 + t * 4), p);
-                q4_unpack(*reinterpret_cast<const uint32_t*>(st + (g + 8) * kQ4Pitch + ch * 16 + t * 4), q);
-                const uint4* xc = xs + (size_t)(at - kb0 + ch) * NT * 32 + lane;
+                q4_unpack(*reinterpret_cast<const uint32_t*>(st + ch * 16), p);
+                q4_unpack(*reinterpret_cast<const uint32_t*>(st + 8 * kQ4Pitch + ch * 16), q);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    const uint4 b = xc[n * 32];
-                    q4_mma(c[n], p[0], q[0], p[1], q[1], b.x, b.y);
-                    q4_mma(c[n], p[2], q[2], p[3], q[3], b.z, b.w);
+                    const uint4 b = xc[(ch * NT + n) * 32];
+                    q4_mma(c[n], ch % P == 0 ? zero : c[n], p[0], q[0], p[1], q[1], b.x, b.y);
+                    q4_mma(c[n], c[n], p[2], q[2], p[3], q[3], b.z, b.w);
                 }
-                if (--left == 0 || at + ch == c1 - 1) {
-                    const float sg = sc[gi * 16 + g], sh = sc[gi * 16 + g + 8];
+                if (ch % P == P - 1) {
+                    const float sg = su[ch / P * 16], sh = su[ch / P * 16 + 8];
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
                         acc[n][0] += sg * c[n][0];
                         acc[n][1] += sg * c[n][1];
                         acc[n][2] += sh * c[n][2];
                         acc[n][3] += sh * c[n][3];
-                        c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
                     }
-                    gi++;
-                    left = gpc;
                 }
             }
+            xc += kQ4Stage * NT * 32;
+            su += kQ4Stage / P * 16;
             __syncwarp();
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    // [KS warps][column][16 rows] of the tile, then the pieces and the warps' parts are added up
+    // [warp][column][16 rows], then the pieces and the ks warps' parts are added up
     __syncthreads();
     float* so = reinterpret_cast<float*>(qsm) + warp * (NT * 8 * 16);
 #pragma unroll
@@ -240,44 +261,45 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
         so[(n * 8 + 2 * t + 1) * 16 + g + 8] = acc[n][3];
     }
     __syncthreads();
-    constexpr int kRows = 16 * (kQ4Warps / KS);
-    for (int i = tid; i < mr * kRows; i += kQ4Threads) {
-        const int r = i / kRows, row = i % kRows, i0 = blockIdx.x * kRows + row;
-        if (i0 >= a.w.rows) continue;
-        const float* sp = reinterpret_cast<const float*>(qsm) + (row >> 4) * KS * (NT * 8 * 16) + (row & 15);
+    const int rows_log2 = 7 - a.ks_log2;
+    for (int i = tid; i < mr << rows_log2; i += kQ4Threads) {
+        const int r = i >> rows_log2, row = i & (rows - 1), at = blockIdx.x * rows + row;
+        if (at >= a.w.rows) continue;
+        const float* sp = reinterpret_cast<const float*>(qsm) + ((row >> 4) << a.ks_log2) * (NT * 8 * 16) + (row & 15);
         float v = 0.f;
-        for (int k = 0; k < KS; k++)
+        for (int k = 0; k < ks; k++)
             for (int j = a.terms - 1; j >= 0; j--) v += sp[k * (NT * 8 * 16) + (r * a.terms + j) * 16];
-        st_any(a.out, a.ot, (long long)(r0 + r) * a.ldo + i0, v);
+        st_any(a.out, a.ot, (long long)(r0 + r) * a.ldo + at, v);
     }
 }
 
-template <int NT, int KS>
+template <int NT, int P>
 static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
-    const int per = NT * 8 / a.terms, tiles = (a.w.rows + 15) / 16, chunks = (a.w.cols + 31) / 32, gpc = a.w.group / 32;
-    // as many columns at a time as fit: 512 bytes a chunk and tile of pieces, 512 a group and chunk of 8 warps' scales
-    const int fit = kQ4MaxBytes / (512 * (NT + 2)) / (KS * kQ4Stage) * (KS * kQ4Stage);
-    a.kb_chunks = std::min(chunks, fit);
-    const int share = ((a.kb_chunks + KS - 1) / KS + kQ4Stage - 1) / kQ4Stage * kQ4Stage;
-    a.kb_groups = std::min((share + gpc - 2) / gpc + 1, (chunks + gpc - 1) / gpc);
-    const size_t smem = kQ4RingBytes + (size_t)a.kb_chunks * NT * 512 + (size_t)a.kb_groups * kQ4Warps * 64;
-    if (smem > 48 * 1024) client_smem<k_q4_mma<NT, KS>>(cx);
-    constexpr int kTiles = kQ4Warps / KS;
-    k_q4_mma<NT, KS><<<dim3((tiles + kTiles - 1) / kTiles, (a.m + per - 1) / per), kQ4Threads, smem, st>>>(a);
+    const int tiles = (a.w.rows + 15) / 16, gpc = std::min(a.w.group, FHE_Q4_MAX_COLS) / 32;
+    // warps enough to keep the loads in flight (8 an SM), but two stages of columns at least for each
+    const int chunks = (a.w.cols + 31) / 32;
+    a.per = NT * 8 / a.terms;
+    a.ks_log2 = 0;
+    while (a.ks_log2 < 3 && (tiles << a.ks_log2) < 148 * 8 && chunks >= (4 << a.ks_log2) * kQ4Stage) a.ks_log2++;
+    const int step = kQ4Stage << a.ks_log2;
+    // as many columns at a time as fit: 512 bytes a chunk and tile of pieces, 512 a chunk for the scales of 8 warps' rows
+    a.kb_chunks = std::min((chunks + step - 1) / step * step, kQ4MaxBytes / (512 * (NT + 1)) / step * step);
+    a.units = (a.kb_chunks >> a.ks_log2) / P;
+    a.group_magic = gpc == 1 ? 0u : (uint32_t)(((1ull << 32) + gpc - 1) / gpc);
+    const size_t smem = kQ4RingBytes + (size_t)a.kb_chunks * NT * 512 + (size_t)a.units * kQ4Warps * 64;
+    if (smem > 48 * 1024) client_smem<k_q4_mma<NT, P>>(cx);
+    const int each = kQ4Warps >> a.ks_log2;
+    k_q4_mma<NT, P><<<dim3((tiles + each - 1) / each, (a.m + a.per - 1) / a.per), kQ4Threads, smem, st>>>(a);
     CUDA_CHECK(cudaGetLastError());
     cx.launches++;
 }
 
 template <int NT>
 static void q4_mma_split(Context& cx, const Q4Args& a, cudaStream_t st) {
-    // warps enough to keep the loads in flight (16 an SM), but at least a stage of columns for each
-    const int tiles = (a.w.rows + 15) / 16, chunks = (a.w.cols + 31) / 32;
-    int ks = 1;
-    while (ks < 8 && tiles * ks < 148 * 8 && chunks >= 2 * ks * kQ4Stage) ks *= 2;
-    if (ks == 1) q4_mma_launch<NT, 1>(cx, a, st);
-    else if (ks == 2) q4_mma_launch<NT, 2>(cx, a, st);
-    else if (ks == 4) q4_mma_launch<NT, 4>(cx, a, st);
-    else q4_mma_launch<NT, 8>(cx, a, st);
+    const int gpc = a.w.group / 32;
+    if (gpc % 2) q4_mma_launch<NT, 1>(cx, a, st);
+    else if (gpc % 4) q4_mma_launch<NT, 2>(cx, a, st);
+    else q4_mma_launch<NT, 4>(cx, a, st);
 }
 
 static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
@@ -583,7 +605,8 @@ void client_ptr(const fhe::Context& c, const void* p, size_t align, const char* 
 
 void client_table(const fhe::Context& c, const fhe_q4* w) {
     REQUIRE(w, "null argument");
-    REQUIRE(w->rows >= 0 && w->cols >= 1, "q4 table: rows >= 0 and cols >= 1");
+    REQUIRE(w->rows >= 0 && w->cols >= 1 && w->cols <= FHE_Q4_MAX_COLS,
+            "q4 table: rows >= 0 and cols in 1..FHE_Q4_MAX_COLS");
     REQUIRE(w->group >= 32 && w->group % 32 == 0, "q4 table: the group is a multiple of 32 columns");
     REQUIRE(w->ldq % 16 == 0 && w->ldq >= ((long long)w->cols + 31) / 32 * 16,
             "q4 table: rows are padded to a multiple of 16 bytes (32 columns)");
@@ -614,7 +637,7 @@ extern "C" int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_
         client_ptr(cx->cx, x, xb, "x");
         client_ptr(cx->cx, out, ob, "out");
         cudaStream_t st = client_stream(cx, stream);
-        fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0, 0, 0}, st);
+        fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0, 0, 0, 0, 0, 0}, st);
     });
 }
 
