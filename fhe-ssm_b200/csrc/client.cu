@@ -8,6 +8,7 @@
 // All three run on a stream of the caller's choice, allocate nothing and read nothing of the context's
 // chain or keys.
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -337,11 +338,20 @@ __global__ void __launch_bounds__(256) k_q4_rows(const fhe_q4 w, const int64_t* 
 //   not depend on their order; tokens are ranked by l, equal ones by index;
 //   kept: rank < top_k, sum of the weights ranked before < ceil(top_p * the top_k's sum), e >= min_p;
 //   S = sum of the kept weights, the token is the first in index order whose running sum passes floor(u S).
+//
+// k_sample: a cluster of blocks per row, each with its part of the row's e in shared memory, so that the logits are read
+// once.  Nothing is sorted.  A histogram of e in 128 bins an octave (a count for top_k, 16 bits of each e for top_p) tells
+// the bins around the last kept token; only their tokens, some hundreds, go to a list that one block selects from
+// exactly, while the bins above them are summed exactly.  If the list overflows (thousands of equal logits) or the
+// histogram's guess was off by more than a bin, the block selects on the row itself, by the same radix search.
 constexpr int kSampleThreads = 1024, kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleBins = 2048;
-constexpr int kSampleList = 2048;      // tokens of one bin that are ranked against each other directly
+constexpr int kSampleRadix = 1024;              // bins of one step of the radix search
+constexpr int kSamplePart = 32768;              // logits of a row that one block holds
+constexpr int kSampleBins = 41 * 128 + 1;       // e from 1 down to 2^-41, below which a token has no weight
+constexpr int kSampleList = 3072;
+constexpr int kSampleClusterMax = 8;
 constexpr float kSampleOne = 1099511627776.f;   // 2^40
-// e < 2^-41 rounds to no weight: exp(-29) 2^40 = 0.28, so everything further than 29 T below M is out
+// exp(-29) 2^40 = 0.28 rounds to no weight: what is further than 29 T below M is out
 constexpr float kSampleReach = 29.f;
 
 struct SampleArgs {
@@ -363,20 +373,59 @@ __device__ __forceinline__ uint64_t sample_rank_key(float x, uint32_t i) {
     const uint32_t k = b & 0x80000000u ? ~b : b | 0x80000000u;
     return (uint64_t)k << 32 | (0xffffffffu - i);
 }
+__device__ __forceinline__ uint64_t sample_weight(float e) { return __float2ull_rn(e * kSampleOne); }
+// bin 0: e = 1; bins 128 (i - 1) + 1 .. 128 i: e from 2^(1 - i) down to 2^-i, which is in the last
+__device__ __forceinline__ int sample_bin(float e) { return (int)((0x3fffffffu - __float_as_uint(e)) >> 16) - 127; }
+// e's bits are above this for the bins below b, and for no others
+__device__ __forceinline__ uint32_t sample_bin_bits(int b) { return 0x3fffffffu - ((uint32_t)(b + 127) << 16); }
+
+// sample_weight in two halves of 20 bits by float32 additions, for sums over many: the conversion to 64 bits is slow
+__device__ __forceinline__ void sample_weight_add(float e, uint32_t& hi, uint32_t& lo) {
+    const float b = e * 1048576.f, h = __fadd_rz(b, 8388608.f);           // its last bits: floor(b)
+    const float l = __fmaf_rn(b - (h - 8388608.f), 1048576.f, 8388608.f);   // the rest, rounded to nearest even
+    hi += __float_as_uint(h) - 0x4B000000u;
+    lo += __float_as_uint(l) - 0x4B000000u;
+}
 
 struct SampleRow {
     const void* p;
     int type, v;
-    float top, t, bins_per_unit, reach;
+    float top, t, rt, reach;
+    bool mul;   // t's reciprocal is far from the ends of float32
+    __device__ void set(const SampleArgs& a, int r) {
+        p = static_cast<const uint8_t*>(a.logits) + (long long)r * a.ld * (a.type == FHE_F32 ? 4 : 2);
+        type = a.type;
+        v = a.vocab;
+    }
+    __device__ void scale(float top_, float t_) {
+        top = top_;
+        t = t_;
+        rt = __frcp_rn(t_);
+        reach = kSampleReach * t_;
+        mul = t_ > 1e-30f && t_ < 1e30f;
+    }
     __device__ float x(int i) const {
         const float a = ld_any(p, type, i);
         return a != a ? -INFINITY : a;
     }
     __device__ float z(float a) const { return a == top ? 0.f : __fdiv_rn(a - top, t); }
-    __device__ static uint64_t weight(float e) { return __float2ull_rn(e * kSampleOne); }
-    __device__ float d(float a) const { return a == top ? 0.f : top - a; }
-    __device__ bool counts(float a) const { return a > -INFINITY && d(a) <= reach; }
-    __device__ int bin(float a) const { return min(kSampleBins - 1, (int)(d(a) * bins_per_unit)); }
+    __device__ bool counts(float a) const { return a == top || top - a <= reach; }
+    // exp((a - M) / T), or 0 for a token without weight.  The quotient by the reciprocal and one correction of its exact
+    // remainder (Markstein 1990) is the rounded one.
+    __device__ float e(float a) const {
+        const float d = a - top;
+        if (a == top) return 1.f;
+        if (!(-d <= reach)) return 0.f;
+        float z;
+        if (mul) {
+            const float q = d * rt;
+            z = __fmaf_rn(__fmaf_rn(-q, t, d), rt, q);
+        } else {
+            z = __fdiv_rn(d, t);
+        }
+        const float v = expf(z);
+        return v >= 4.547473508864641e-13f ? v : 0.f;   // 2^-41: one half, which rounds to the even 0, has no weight either
+    }
 };
 
 template <class T, class F>
@@ -389,158 +438,179 @@ __device__ T sample_reduce(T v, F f, T* sh) {
     for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+template <class T>
+__device__ T sample_scan(T v) {   // inclusive, over a warp
+    for (int o = 1; o < 32; o <<= 1) {
+        const T n = __shfl_up_sync(0xffffffffu, v, o);
+        if ((threadIdx.x & 31) >= o) v += n;
+    }
+    return v;
+}
+// inclusive over the block; sh: 32 values
+template <class T>
+__device__ T sample_block_scan(T v, T* sh) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    v = sample_scan(v);
+    __syncthreads();
+    if (lane == 31) sh[warp] = v;
+    __syncthreads();
+    const T w = sample_scan(sh[lane]);
+    return v + (warp ? __shfl_sync(0xffffffffu, w, warp - 1) : T(0));
+}
 
-struct SampleShared {
-    uint64_t sum[kSampleBins];
-    uint32_t count[kSampleBins];
-    uint64_t key[kSampleList], wt[kSampleList];
-    uint64_t red[32];
-    float redf[32];
+struct SampleRadix {
+    uint64_t sum[kSampleRadix];
+    uint32_t count[kSampleRadix];
+    uint64_t key[32], wt[32];
+    uint64_t red[32], red2[32];
+    uint64_t got, before, before2;
     uint32_t n;
-    uint64_t got, got_before;
     int at;
 };
+struct SampleFound {
+    uint64_t key, sum;   // the last kept token's rank key, and the sum of the weights down to it
+};
 
-// The lowest rank key that is still in, among the tokens with keys in [lo, hi], where `want` is a count of tokens (BY_COUNT) or
-// a sum of weights: the first token, in rank order, at which the running count or sum reaches `want` (>= 1).  The running
-// sum of weights before it goes to *before.  0 if it is never reached.
-template <bool BY_COUNT>
-__device__ uint64_t sample_select(const SampleRow& row, SampleShared& sh, uint64_t want, uint64_t* before) {
+// The token, in rank order, at which the running count (BY_COUNT) or sum of weights reaches `want` (>= 1); key 0 and the whole
+// sum if none does.  each(f) calls f(rank key, e) for the calling thread's share of the tokens.
+template <bool BY_COUNT, class Each>
+__device__ SampleFound sample_select(SampleRadix& sh, uint64_t want, Each each) {
     const int tid = threadIdx.x;
-    uint64_t lo = 0, hi = ~0ull, sum_before = 0;
-    bool first = true;
+    uint64_t lo = ~0ull, hi = 0, before = 0;
+    each([&](uint64_t k, float) { lo = min(lo, k), hi = max(hi, k); });
+    lo = sample_reduce(lo, [](uint64_t p, uint64_t q) { return min(p, q); }, sh.red);
+    hi = sample_reduce(hi, [](uint64_t p, uint64_t q) { return max(p, q); }, sh.red);
+    if (hi == 0) return {0, 0};
     while (true) {
-        // histogram of the tokens in [lo, hi]: by distance below the top at first, by rank key after that
-        int shift = 0;
-        if (!first) {
-            const uint64_t range = hi - lo;
-            shift = max(0, 64 - __clzll((long long)range) - 11);
-        }
-        for (int b = tid; b < kSampleBins; b += kSampleThreads) sh.sum[b] = 0, sh.count[b] = 0;
+        // the tokens with keys in [lo, hi], in 1024 bins of equal width
+        const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
+        sh.sum[tid] = 0;
+        sh.count[tid] = 0;
         if (tid == 0) sh.at = -1, sh.n = 0;
         __syncthreads();
-        for (int i = tid; i < row.v; i += kSampleThreads) {
-            const float a = row.x(i);
-            if (!row.counts(a)) continue;
-            const uint64_t k = sample_rank_key(a, i);
-            if (k < lo || k > hi) continue;
-            const int b = first ? row.bin(a) : (int)((hi - k) >> shift);
+        each([&](uint64_t k, float e) {
+            if (k < lo || k > hi) return;
+            const int b = (int)((hi - k) >> shift);
             atomicAdd(&sh.count[b], 1u);
-            atomicAdd((unsigned long long*)&sh.sum[b], (unsigned long long)row.weight(expf(row.z(a))));
-        }
+            atomicAdd((unsigned long long*)&sh.sum[b], (unsigned long long)sample_weight(e));
+        });
         __syncthreads();
-        if (tid == 0) {
-            uint64_t run = 0, s = sum_before;
-            for (int b = 0; b < kSampleBins; b++) {
-                const uint64_t now = BY_COUNT ? sh.count[b] : sh.sum[b];
-                if (run + now >= want) { sh.at = b; sh.got = run; sh.got_before = s; break; }
-                run += now;
-                s += sh.sum[b];
-            }
-            if (sh.at < 0) sh.got_before = s;
-        }
+        const uint64_t c = sh.count[tid], s = sh.sum[tid];
+        const uint64_t sums = sample_block_scan(s, sh.red2);
+        const uint64_t run = BY_COUNT ? sample_block_scan(c, sh.red) : sums, own = BY_COUNT ? c : s;
+        if (run >= want && run - own < want) sh.at = tid, sh.got = run - own, sh.before = before + sums - s;
+        if (tid == kSampleRadix - 1) sh.before2 = before + sums;
         __syncthreads();
         const int at = sh.at;
-        sum_before = sh.got_before;
-        if (at < 0) { *before = sum_before; return 0; }
+        if (at < 0) return {0, sh.before2};
         want -= sh.got;
+        before = sh.before;
         const uint32_t n = sh.count[at];
-        if (n <= kSampleList) {
-            for (int i = tid; i < row.v; i += kSampleThreads) {
-                const float a = row.x(i);
-                if (!row.counts(a)) continue;
-                const uint64_t k = sample_rank_key(a, i);
-                if (k < lo || k > hi) continue;
-                const int b = first ? row.bin(a) : (int)((hi - k) >> shift);
-                if (b != at) continue;
+        // the bin's own range of keys
+        const uint64_t top = hi - ((uint64_t)at << shift), bottom = top - ((1ull << shift) - 1);
+        lo = bottom > top ? lo : max(lo, bottom);
+        hi = top;
+        if (n <= 32) {
+            each([&](uint64_t k, float e) {
+                if (k < lo || k > hi) return;
                 const uint32_t j = atomicAdd(&sh.n, 1u);
                 sh.key[j] = k;
-                sh.wt[j] = row.weight(expf(row.z(a)));
-            }
+                sh.wt[j] = sample_weight(e);
+            });
             __syncthreads();
-            // the list's own order: each token sums what is ranked before it
-            for (uint32_t j = tid; j < n; j += kSampleThreads) {
-                const uint64_t k = sh.key[j];
+            if (tid < n) {
                 uint64_t c = 0, s = 0;
                 for (uint32_t l = 0; l < n; l++)
-                    if (sh.key[l] > k) { c++; s += sh.wt[l]; }
-                const uint64_t run = BY_COUNT ? c : s, own = BY_COUNT ? 1 : sh.wt[j];
-                if (run < want && run + own >= want) { sh.got = k; sh.got_before = sum_before + s; }
+                    if (sh.key[l] > sh.key[tid]) c++, s += sh.wt[l];
+                const uint64_t run = BY_COUNT ? c : s, own = BY_COUNT ? 1 : sh.wt[tid];
+                if (run < want && run + own >= want) sh.got = sh.key[tid], sh.before2 = before + s + sh.wt[tid];
             }
             __syncthreads();
-            *before = sh.got_before;
-            const uint64_t r = sh.got;
+            const SampleFound f{sh.got, sh.before2};
             __syncthreads();
-            return r;
+            return f;
         }
-        // too many: their own range of rank keys, in finer bins
-        uint64_t a0 = ~0ull, a1 = 0;
-        for (int i = tid; i < row.v; i += kSampleThreads) {
-            const float a = row.x(i);
-            if (!row.counts(a)) continue;
-            const uint64_t k = sample_rank_key(a, i);
-            if (k < lo || k > hi) continue;
-            const int b = first ? row.bin(a) : (int)((hi - k) >> shift);
-            if (b == at) a0 = min(a0, k), a1 = max(a1, k);
-        }
-        lo = sample_reduce(a0, [](uint64_t p, uint64_t q) { return min(p, q); }, sh.red);
-        hi = sample_reduce(a1, [](uint64_t p, uint64_t q) { return max(p, q); }, sh.red);
-        first = false;
+        __syncthreads();
     }
 }
 
-__global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
-    extern __shared__ __align__(16) uint8_t ssm[];
-    SampleShared& sh = *reinterpret_cast<SampleShared*>(ssm);
-    const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    SampleRow row;
-    row.p = static_cast<const uint8_t*>(a.logits) + (long long)r * a.ld * (a.type == FHE_F32 ? 4 : 2);
-    row.type = a.type;
-    row.v = a.vocab;
-    float t = a.temperature ? a.temperature[r] : a.temperature1;
-    float p = a.top_p ? a.top_p[r] : a.top_p1;
-    float mp = a.min_p ? a.min_p[r] : a.min_p1;
-    int64_t k = a.top_k ? a.top_k[r] : a.top_k1;
-    mp = mp > 0.f ? fminf(mp, 1.f) : 0.f;   // a NaN in the array: off
-    if (!(t > 0.f)) t = 1.f, k = 1;
-    float top = -INFINITY, low = INFINITY;
-    for (int i = tid; i < row.v; i += kSampleThreads) {
-        const float x = row.x(i);
-        top = fmaxf(top, x);
-        if (x > -INFINITY) low = fminf(low, x);
+struct SampleSettings {
+    float t, p, mp, u;
+    int64_t k;
+    __device__ SampleSettings(const SampleArgs& a, int r) {
+        t = a.temperature ? a.temperature[r] : a.temperature1;
+        p = a.top_p ? a.top_p[r] : a.top_p1;
+        mp = a.min_p ? a.min_p[r] : a.min_p1;
+        k = a.top_k ? a.top_k[r] : a.top_k1;
+        u = fminf(fmaxf(a.u[r], 0.f), 1.f);     // a NaN: 0
+        mp = mp > 0.f ? fminf(mp, 1.f) : 0.f;   // a NaN in the array: off
+        if (!(t > 0.f)) t = 1.f, k = 1;
+        t = fminf(t, 1e30f);
+        if (k <= 0 || k >= a.vocab) k = 0;
     }
-    row.top = top = sample_reduce(top, [](float x, float y) { return fmaxf(x, y); }, sh.redf);
-    low = sample_reduce(low, [](float x, float y) { return fminf(x, y); }, sh.redf);
+    // the running sum of weights that top_p asks for, of the top_k's sum s
+    __device__ uint64_t limit(uint64_t s) const {
+        const double w = ceil((double)p * (double)s);
+        return w > 1.0 ? (uint64_t)w : 1;
+    }
+    __device__ uint64_t target(uint64_t s) const {
+        const uint64_t v = (uint64_t)((double)u * (double)s);
+        return v < s ? v : s - 1;
+    }
+};
+
+// The first of a stretch [i0, i1) of tokens at which start + the running sum of kept(i) passes target, by one warp
+template <class Kept>
+__device__ int sample_walk(int i0, int i1, uint64_t start, uint64_t target, Kept kept) {
+    const int lane = threadIdx.x & 31;
+    for (int i = i0; i < i1; i += 32) {
+        const uint64_t run = start + sample_scan(i + lane < i1 ? kept(i + lane) : 0ull);
+        const uint32_t past = __ballot_sync(0xffffffffu, run > target);
+        if (past) return i + __ffs(past) - 1;
+        start = __shfl_sync(0xffffffffu, run, 31);
+    }
+    return -1;
+}
+__device__ __forceinline__ float sample_logprob(const SampleRow& row, int i, uint64_t total) {
+    return row.z(row.x(i)) - (float)log((double)total / (double)kSampleOne);
+}
+
+// Rows longer than a cluster's shared memory: one block per row, which reads the logits again for every step.
+__global__ void __launch_bounds__(kSampleThreads) k_sample_long(const SampleArgs a) {
+    __shared__ SampleRadix sh;
+    __shared__ float redf[32];
+    const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const SampleSettings set(a, r);
+    SampleRow row;
+    row.set(a, r);
+    float top = -INFINITY;
+    for (int i = tid; i < row.v; i += kSampleThreads) top = fmaxf(top, row.x(i));
+    top = sample_reduce(top, [](float x, float y) { return fmaxf(x, y); }, redf);
     if (top == -INFINITY) {
         if (tid == 0) a.token[r] = -1, a.logprob[r] = -INFINITY;
         return;
     }
-    row.t = t;
-    row.reach = kSampleReach * t;
-    const float span = fminf(row.reach, top - low);
-    row.bins_per_unit = span > 0.f ? fminf(kSampleBins / span, 1e30f) : 0.f;
-
-    uint64_t bound = 0, before;
-    const bool by_p = p < 1.f;
-    if (k > 0 && k < row.v) bound = sample_select<true>(row, sh, k, &before);
-    if (by_p) {
-        uint64_t s = 0;
+    row.scale(top, set.t);
+    auto each = [&](auto f) {
         for (int i = tid; i < row.v; i += kSampleThreads) {
             const float x = row.x(i);
-            if (row.counts(x) && sample_rank_key(x, i) >= bound) s += row.weight(expf(row.z(x)));
+            if (row.counts(x)) f(sample_rank_key(x, i), row.e(x));
         }
+    };
+    uint64_t bound = 0;
+    if (set.k) bound = sample_select<true>(sh, set.k, each).key;
+    if (set.p < 1.f) {
+        uint64_t s = 0;
+        each([&](uint64_t k, float e) { s += k >= bound ? sample_weight(e) : 0; });
         s = sample_reduce(s, [](uint64_t x, uint64_t y) { return x + y; }, sh.red);
-        const double want = ceil((double)p * (double)s);
-        const uint64_t b = sample_select<false>(row, sh, want > 1.0 ? (uint64_t)want : 1, &before);
-        bound = max(bound, b);
+        bound = max(bound, sample_select<false>(sh, set.limit(s), each).key);
     }
-    // the kept weights of each warp's stretch of tokens
     const int per = (row.v + kSampleWarps - 1) / kSampleWarps, i0 = min(row.v, warp * per), i1 = min(row.v, i0 + per);
     auto kept = [&](int i) -> uint64_t {
         const float x = row.x(i);
         if (!row.counts(x) || sample_rank_key(x, i) < bound) return 0;
-        const float e = expf(row.z(x));
-        return e >= mp ? row.weight(e) : 0;
+        const float e = row.e(x);
+        return e >= set.mp ? sample_weight(e) : 0;
     };
     uint64_t mine = 0;
     for (int i = i0 + lane; i < i1; i += 32) mine += kept(i);
@@ -553,27 +623,348 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
         if (w == warp) start = total;
         total += sh.red[w];
     }
-    const float u = fminf(fmaxf(a.u[r], 0.f), 1.f);
-    uint64_t target = (uint64_t)((double)u * (double)total);
-    if (target >= total) target = total - 1;
+    const uint64_t target = set.target(total);
     if (target < start || target >= start + mine) return;
-    for (int i = i0; i < i1; i += 32) {
-        const uint64_t w = i + lane < i1 ? kept(i + lane) : 0;
-        uint64_t run = w;
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t v = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += v;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, start + run > target);
-        if (past) {
-            if (lane == __ffs(past) - 1) {
-                a.token[r] = i + lane;
-                a.logprob[r] = row.z(row.x(i + lane)) - (float)log((double)total / (double)kSampleOne);
+    const int i = sample_walk(i0, i1, start, target, kept);
+    if (lane == 0) a.token[r] = i, a.logprob[r] = sample_logprob(row, i, total);
+}
+
+struct alignas(16) SampleShared {
+    SampleRadix radix;
+    uint64_t sum[kSampleClusterMax], above[kSampleClusterMax], part[kSampleClusterMax];   // each block writes its own to all
+    float top[kSampleClusterMax];
+    uint32_t n[kSampleClusterMax];
+    uint64_t bound, found;                  // block 0's answer
+    int slow, done;
+    uint64_t red[32];
+    float redf[32];
+    uint64_t run_lo, run_all;
+    int at;
+    uint32_t listed;
+    // tokens of the bins around the last kept one: their index, then their rank key; their e
+    uint64_t list_k[kSampleList];
+    float list_e[kSampleList];
+    uint32_t counts[kSampleBins + 7], sums[kSampleBins + 7];
+};
+
+static_assert(sizeof(SampleShared) + kSamplePart * sizeof(float) <= 232448, "a block's shared memory");
+
+// n logits from row.p + first -> buf, as float32 without NaN; the calling thread's largest
+template <class T>
+__device__ __forceinline__ float sample_load(const SampleRow& row, int first, int n, float* buf) {
+    const T* src = static_cast<const T*>(row.p) + first;
+    constexpr int kVec = 16 / sizeof(T), kDeep = 4;
+    float top = -INFINITY;
+    int done = 0;
+    if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+        const int nv = n / kVec;
+        for (int i = threadIdx.x; i < nv; i += kSampleThreads * kDeep) {
+            uint4 v[kDeep];
+#pragma unroll
+            for (int d = 0; d < kDeep; d++)
+                if (i + d * kSampleThreads < nv) v[d] = reinterpret_cast<const uint4*>(src)[i + d * kSampleThreads];
+#pragma unroll
+            for (int d = 0; d < kDeep; d++) {
+                if (i + d * kSampleThreads >= nv) break;
+                const T* u = reinterpret_cast<const T*>(&v[d]);
+                float x[kVec];
+#pragma unroll
+                for (int j = 0; j < kVec; j++) {
+                    x[j] = q4_float(u[j]);
+                    if (x[j] != x[j]) x[j] = -INFINITY;
+                    top = fmaxf(top, x[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < kVec; j += 4)
+                    *reinterpret_cast<float4*>(buf + (size_t)(i + d * kSampleThreads) * kVec + j) =
+                        make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
             }
+        }
+        done = nv * kVec;
+    }
+    for (int i = done + threadIdx.x; i < n; i += kSampleThreads * 8) {
+        T v[8];
+#pragma unroll
+        for (int d = 0; d < 8; d++)
+            if (i + d * kSampleThreads < n) v[d] = src[i + d * kSampleThreads];
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+            if (i + d * kSampleThreads >= n) break;
+            float x = q4_float(v[d]);
+            if (x != x) x = -INFINITY;
+            top = fmaxf(top, x);
+            buf[i + d * kSampleThreads] = x;
+        }
+    }
+    return top;
+}
+
+__global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
+    namespace cg = cooperative_groups;
+    extern __shared__ __align__(16) uint8_t ssm[];
+    SampleShared& sh = *reinterpret_cast<SampleShared*>(ssm);
+    float* buf = reinterpret_cast<float*>(ssm + sizeof(SampleShared));
+    cg::cluster_group cluster = cg::this_cluster();
+    const int nb = cluster.num_blocks(), rank = cluster.block_rank(), r = blockIdx.x / nb;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    cluster.barrier_arrive();
+    const SampleSettings set(a, r);
+    const bool by_k = set.k != 0, by_p = set.p < 1.f;
+    const auto add = [](uint64_t x, uint64_t y) { return x + y; };
+    SampleRow row;
+    row.set(a, r);
+    const int part = ((row.v + nb - 1) / nb + 7) / 8 * 8, first = min(row.v, rank * part), n = min(row.v, first + part) - first;
+
+    float top = a.type == FHE_F32   ? sample_load<float>(row, first, n, buf)
+                : a.type == FHE_F16 ? sample_load<__half>(row, first, n, buf)
+                                    : sample_load<__nv_bfloat16>(row, first, n, buf);
+    if (by_k || by_p)
+        for (int b = tid; b < kSampleBins; b += kSampleThreads) sh.counts[b] = 0, sh.sums[b] = 0;
+    top = sample_reduce(top, [](float x, float y) { return fmaxf(x, y); }, sh.redf);
+    cluster.barrier_wait();   // every block runs
+    if (tid < nb) *cluster.map_shared_rank(&sh.top[rank], tid) = top;
+    cluster.sync();
+    for (int b = 0; b < nb; b++) top = fmaxf(top, sh.top[b]);
+    if (top == -INFINITY) {   // in every block of the cluster
+        if (rank == 0 && tid == 0) a.token[r] = -1, a.logprob[r] = -INFINITY;
+        return;
+    }
+    row.scale(top, set.t);
+
+    // e in the logits' place, each warp its stretch; the histograms
+    const int per = (n + kSampleThreads - 1) / kSampleThreads * 32, i0 = min(n, warp * per), i1 = min(n, i0 + per);
+    uint64_t all = 0;   // the whole sum
+    {
+        uint32_t hi = 0, lo = 0;
+        for (int i = i0 + lane; i < i1; i += 32) {
+            const float e = row.e(buf[i]);
+            buf[i] = e;
+            if (e > 0.f && (by_k || by_p)) {
+                const int b = sample_bin(e);
+                if (by_k) atomicAdd(&sh.counts[b], 1u);
+                if (by_p) {
+                    // 16 bits of e: a block's 2^15 tokens add up to less than 2^31
+                    atomicAdd(&sh.sums[b], (__float_as_uint(e) >> 8 & 0x7fffu) | 0x8000u);
+                    sample_weight_add(e, hi, lo);
+                }
+            }
+        }
+        if (by_p) {
+            const uint64_t s = sample_reduce(((uint64_t)hi << 20) + lo, add, sh.red);
+            if (tid < nb) *cluster.map_shared_rank(&sh.sum[rank], tid) = s;
+        }
+        if (by_k || by_p) cluster.sync();
+        if (by_p)
+            for (int b = 0; b < nb; b++) all += sh.sum[b];
+    }
+
+    uint32_t cut = 0;   // kept are e with bits above this, and whatever the lists have not struck off
+    // One selection.  The histogram tells a guess of the last kept token's bin; the tokens of that bin and its neighbours go to
+    // the list (by count, and where they are few, all the tokens above as well), the weights above are summed, and block 0 selects.
+    auto locate = [&](bool by_count, uint64_t want) {
+        constexpr int kPer = (kSampleBins + kSampleThreads - 1) / kSampleThreads;
+        uint64_t own[kPer], mine = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int b = tid * kPer + j;
+            uint64_t v = 0;
+            if (b < kSampleBins)
+                for (int q = 0; q < nb; q++) {
+                    const SampleShared* o = cluster.map_shared_rank(&sh, q);
+                    v += by_count ? o->counts[b] : o->sums[b];
+                }
+            // a sum is in units of 2^-15 of its octave's top
+            const int up = 40 - 15 - (b + 127) / 128;
+            own[j] = by_count ? v : up >= 0 ? v << up : v >> -up;
+            mine += own[j];
+        }
+        uint64_t run = sample_block_scan(mine, sh.red);
+        if (tid == kSampleThreads - 1) sh.run_all = run;
+        if (tid == 0) sh.at = kSampleBins, sh.listed = 0, sh.run_lo = 0;
+        run -= mine;
+        __syncthreads();
+        // the sums' 16 bits are cut off, all alike
+        uint64_t guess = want;
+        if (!by_count) {
+            guess = (uint64_t)((double)want * ((double)sh.run_all / (double)all));
+            guess = guess < 1 ? 1 : guess > sh.run_all ? sh.run_all : guess;
+        }
+        uint64_t v = run;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            if (v < guess && v + own[j] >= guess) sh.at = tid * kPer + j;
+            v += own[j];
+        }
+        __syncthreads();
+        const int at = sh.at;
+        if (by_count && at == kSampleBins) {   // no more than top_k have a weight: nothing is struck off
+            if (tid == 0) sh.done = 0, sh.found = all;
+            __syncthreads();
             return;
         }
-        start += __shfl_sync(0xffffffffu, run, 31);
+        const int lo = by_count && want <= kSampleRadix ? 0 : max(0, at - 1), hi = min(kSampleBins - 1, at + 1);
+        if (by_count) {
+            v = run;
+#pragma unroll
+            for (int j = 0; j < kPer; j++) {
+                if (tid * kPer + j == lo) sh.run_lo = v;
+                v += own[j];
+            }
+        }
+        const uint32_t above = sample_bin_bits(lo), in = max(cut, sample_bin_bits(hi + 1));
+        uint32_t wh = 0, wl = 0;
+        for (int i = i0; i < i1; i += 32) {
+            const float e = i + lane < i1 ? buf[i + lane] : 0.f;
+            const uint32_t bits = __float_as_uint(e);
+            if (bits > above) sample_weight_add(e, wh, wl);
+            const bool hit = bits > in && bits <= above;
+            const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+            if (hits) {
+                uint32_t j = 0;
+                if (lane == 0) j = atomicAdd(&sh.listed, __popc(hits));
+                j = __shfl_sync(0xffffffffu, j, 0) + __popc(hits & ((1u << lane) - 1));
+                if (hit && j < kSampleList) sh.list_k[j] = first + i + lane, sh.list_e[j] = e;
+            }
+        }
+        const uint64_t s = sample_reduce(((uint64_t)wh << 20) + wl, add, sh.red);
+        const uint32_t listed = min(sh.listed, (uint32_t)kSampleList);   // sample_reduce has waited for all
+        for (uint32_t j = tid; j < listed; j += kSampleThreads) {
+            const uint32_t i = (uint32_t)sh.list_k[j];
+            sh.list_k[j] = sample_rank_key(row.x(i), i);
+        }
+        if (tid < nb) {
+            *cluster.map_shared_rank(&sh.above[rank], tid) = s;
+            *cluster.map_shared_rank(&sh.n[rank], tid) = sh.listed;
+        }
+        cluster.sync();
+        if (rank == 0) {
+            uint64_t over = 0;
+            uint32_t m = 0;
+            bool slow = false;
+            for (int q = 0; q < nb; q++) {
+                over += sh.above[q];
+                m += sh.n[q];
+                slow |= m > kSampleList;   // also if one block's list is cut off
+            }
+            uint64_t bound = 0, found = 0;
+            int done = 0;
+            if (!slow) {
+                uint32_t off = sh.n[0];
+                for (int q = 1; q < nb; q++) {
+                    const SampleShared* o = cluster.map_shared_rank(&sh, q);
+                    for (uint32_t j = tid; j < sh.n[q]; j += kSampleThreads)
+                        sh.list_k[off + j] = o->list_k[j], sh.list_e[off + j] = o->list_e[j];
+                    off += sh.n[q];
+                }
+                __syncthreads();
+                auto each = [&](auto f) {
+                    for (uint32_t j = tid; j < m; j += kSampleThreads) f(sh.list_k[j], sh.list_e[j]);
+                };
+                if (by_count) {
+                    const SampleFound f = sample_select<true>(sh.radix, want - sh.run_lo, each);
+                    bound = f.key;
+                    found = over + f.sum;
+                    slow = bound == 0;
+                    if (!slow && by_p && lo == 0) {
+                        bound = max(bound, sample_select<false>(sh.radix, set.limit(found), each).key);
+                        done = 1;
+                    }
+                } else if (over < want) {
+                    bound = sample_select<false>(sh.radix, want - over, each).key;
+                    slow = bound == 0;
+                } else {
+                    slow = true;
+                }
+            }
+            if (slow) {
+                auto each = [&](auto f) {
+                    for (int i = tid; i < row.v; i += kSampleThreads) {
+                        const float x = row.x(i);
+                        if (row.counts(x)) f(sample_rank_key(x, i), row.e(x));
+                    }
+                };
+                const SampleFound f = by_count ? sample_select<true>(sh.radix, want, each)
+                                               : sample_select<false>(sh.radix, want, each);
+                bound = f.key;
+                found = f.sum;
+            }
+            if (tid < nb) {
+                SampleShared* o = cluster.map_shared_rank(&sh, tid);
+                o->bound = bound;
+                o->found = found;
+                o->slow = slow;
+                o->done = done;
+            }
+        }
+        cluster.sync();
+        const uint64_t bound = sh.bound;
+        if (sh.slow) {
+            for (int i = i0 + lane; i < i1; i += 32)
+                if (sample_rank_key(row.x(first + i), first + i) < bound) buf[i] = 0.f;
+        } else {
+            for (uint32_t j = tid; j < listed; j += kSampleThreads)
+                if (sh.list_k[j] < bound) buf[0xffffffffu - (uint32_t)sh.list_k[j] - first] = 0.f;
+            cut = in;
+        }
+        __syncthreads();
+    };
+    if (by_k) locate(true, set.k);
+    if (by_p && !(by_k && sh.done)) locate(false, set.limit(by_k ? sh.found : all));
+
+    // the kept weights of each warp's stretch, block and cluster; the block that the target falls to walks
+    auto kept = [&](int i) -> float {
+        const float e = buf[i];
+        return __float_as_uint(e) > cut && e >= set.mp ? e : 0.f;
+    };
+    uint32_t wh = 0, wl = 0;
+    for (int i = i0 + lane; i < i1; i += 32) sample_weight_add(kept(i), wh, wl);
+    uint64_t mine = ((uint64_t)wh << 20) + wl;
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    __syncthreads();
+    if (lane == 0) sh.red[warp] = mine;
+    __syncthreads();
+    uint64_t start = 0, total = 0;
+    for (int w = 0; w < kSampleWarps; w++) {
+        if (w == warp) start = total;
+        total += sh.red[w];
     }
+    if (tid < nb) *cluster.map_shared_rank(&sh.part[rank], tid) = total;
+    cluster.sync();
+    total = 0;
+    for (int b = 0; b < nb; b++) {
+        if (b == rank) start += total;
+        total += sh.part[b];
+    }
+    const uint64_t target = set.target(total);
+    if (target < start || target >= start + mine) return;
+    const int i = first + sample_walk(i0, i1, start, target, [&](int j) { return sample_weight(kept(j)); });
+    if (lane == 0) a.token[r] = i, a.logprob[r] = sample_logprob(row, i, total);
+}
+
+static void sample(Context& cx, const SampleArgs& a, cudaStream_t st) {
+    // blocks for every SM, each with 1024 logits at least; a row has to fit its cluster
+    int nb = 1;
+    while (nb < kSampleClusterMax && (nb * kSamplePart < a.vocab || (a.rows * nb * 2 <= 148 && a.vocab >= 2048 * nb))) nb *= 2;
+    if (nb * kSamplePart < a.vocab) {
+        k_sample_long<<<a.rows, kSampleThreads, 0, st>>>(a);
+        CUDA_CHECK(cudaGetLastError());
+    } else {
+        const size_t smem = sizeof(SampleShared) + ((size_t)(a.vocab + nb - 1) / nb + 7) / 8 * 8 * sizeof(float);
+        client_smem<k_sample>(cx);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)a.rows * nb);
+        cfg.blockDim = dim3(kSampleThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = nb;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_sample, a));
+    }
+    cx.launches++;
 }
 
 }  // namespace fhe
@@ -684,10 +1075,6 @@ extern "C" int fhe_sample(fhe_ctx* cx, const fhe_sample_cfg* cfg, const void* lo
         cudaStream_t st = client_stream(cx, stream);
         fhe::SampleArgs a{logits, ld, type, rows, vocab, u, cfg->temperature, cfg->top_p, cfg->min_p, cfg->top_k,
                           cfg->temperature_all, cfg->top_p_all, cfg->min_p_all, cfg->top_k_all, token, logprob};
-        const size_t smem = sizeof(fhe::SampleShared);
-        fhe::client_smem<fhe::k_sample>(cx->cx);
-        fhe::k_sample<<<rows, fhe::kSampleThreads, smem, st>>>(a);
-        CUDA_CHECK(cudaGetLastError());
-        cx->cx.launches++;
+        fhe::sample(cx->cx, a, st);
     });
 }
