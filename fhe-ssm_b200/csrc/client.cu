@@ -339,16 +339,19 @@ __global__ void __launch_bounds__(256) k_q4_rows(const fhe_q4 w, const int64_t* 
 //   kept: rank < top_k, sum of the weights ranked before < ceil(top_p * the top_k's sum), e >= min_p;
 //   S = sum of the kept weights, the token is the first in index order whose running sum passes floor(u S).
 //
-// k_sample: a cluster of blocks per row, each with its part of the row's e in shared memory, so that the logits are read
-// once.  Nothing is sorted.  A histogram of e in 128 bins an octave (a count for top_k, 16 bits of each e for top_p) tells
-// the bins around the last kept token; only their tokens, some hundreds, go to a list that one block selects from
-// exactly, while the bins above them are summed exactly.  If the list overflows (thousands of equal logits) or the
-// histogram's guess was off by more than a bin, the block selects on the row itself, by the same radix search.
+// k_sample: a cluster of blocks per row, each with its part of the row in shared memory, so that the logits are read once.
+// Nothing is sorted; some hundreds of tokens at most go to a list that one block selects from exactly.
+//   top_k up to 1024: at least top_k tokens are no smaller than the top_k-th largest of the threads' own maxima, so the
+//   list is what reaches that value, and everything else, exponentials included, is done on the list alone.
+//   otherwise: e replaces the logits, and a histogram of it in 128 bins an octave (counts for top_k, 16 bits of
+//   each e for top_p) tells the bins around the last kept token; their tokens are the list, the bins above are summed.
+// If the list overflows (thousands of equal logits) or the histogram's guess was off by more than a bin, one block selects on
+// the row itself, by a radix search.
 constexpr int kSampleThreads = 1024, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleRadix = 1024;              // bins of one step of the radix search
 constexpr int kSamplePart = 32768;              // logits of a row that one block holds
-constexpr int kSampleBins = 41 * 128 + 1;       // e from 1 down to 2^-41, below which a token has no weight
-constexpr int kSampleList = 3072;
+constexpr int kSampleBins = 41 * 128 + 8;       // e from 1 down to 2^-41, below which a token has no weight
+constexpr int kSampleList = 2560;
 constexpr int kSampleClusterMax = 8;
 constexpr float kSampleOne = 1099511627776.f;   // 2^40
 // exp(-29) 2^40 = 0.28 rounds to no weight: what is further than 29 T below M is out
@@ -374,10 +377,15 @@ __device__ __forceinline__ uint64_t sample_rank_key(float x, uint32_t i) {
     return (uint64_t)k << 32 | (0xffffffffu - i);
 }
 __device__ __forceinline__ uint64_t sample_weight(float e) { return __float2ull_rn(e * kSampleOne); }
-// bin 0: e = 1; bins 128 (i - 1) + 1 .. 128 i: e from 2^(1 - i) down to 2^-i, which is in the last
-__device__ __forceinline__ int sample_bin(float e) { return (int)((0x3fffffffu - __float_as_uint(e)) >> 16) - 127; }
+// bin 7: e = 1; bins 128 (i - 1) + 8 .. 128 i + 7: e from 2^(1 - i), not included, down to 2^-i
+__device__ __forceinline__ int sample_bin(float e) { return (int)((0x3fffffffu - __float_as_uint(e)) >> 16) - 120; }
 // e's bits are above this for the bins below b, and for no others
-__device__ __forceinline__ uint32_t sample_bin_bits(int b) { return 0x3fffffffu - ((uint32_t)(b + 127) << 16); }
+__device__ __forceinline__ uint32_t sample_bin_bits(int b) { return 0x3fffffffu - ((uint32_t)(b + 120) << 16); }
+// a sum of the leading 16 bits of e, in bin b -> units of 2^-40
+__device__ __forceinline__ uint64_t sample_bin_sum(uint64_t v, int b) {
+    const int up = 40 - 15 - (b + 120) / 128;
+    return up >= 0 ? v << up : v >> -up;
+}
 
 // sample_weight in two halves of 20 bits by float32 additions, for sums over many: the conversion to 64 bits is slow
 __device__ __forceinline__ void sample_weight_add(float e, uint32_t& hi, uint32_t& lo) {
@@ -391,7 +399,7 @@ struct SampleRow {
     const void* p;
     int type, v;
     float top, t, rt, reach;
-    bool mul;   // t's reciprocal is far from the ends of float32
+    bool mul;   // t's reciprocal is far from the ends of float32, and M finite
     __device__ void set(const SampleArgs& a, int r) {
         p = static_cast<const uint8_t*>(a.logits) + (long long)r * a.ld * (a.type == FHE_F32 ? 4 : 2);
         type = a.type;
@@ -402,7 +410,7 @@ struct SampleRow {
         t = t_;
         rt = __frcp_rn(t_);
         reach = kSampleReach * t_;
-        mul = t_ > 1e-30f && t_ < 1e30f;
+        mul = t_ > 1e-30f && t_ < 1e30f && top_ < INFINITY;
     }
     __device__ float x(int i) const {
         const float a = ld_any(p, type, i);
@@ -410,22 +418,16 @@ struct SampleRow {
     }
     __device__ float z(float a) const { return a == top ? 0.f : __fdiv_rn(a - top, t); }
     __device__ bool counts(float a) const { return a == top || top - a <= reach; }
-    // exp((a - M) / T), or 0 for a token without weight.  The quotient by the reciprocal and one correction of its exact
-    // remainder (Markstein 1990) is the rounded one.
-    __device__ float e(float a) const {
+    // exp((a - M) / T), or 0 for a token without weight (below 2^-41; one half, which 2^-41 itself gives, rounds to the
+    // even 0).  The quotient by the reciprocal and one correction of its exact remainder (Markstein 1990) is the rounded one; where
+    // the difference is infinite it gives NaN, which has no weight either.
+    __device__ __forceinline__ float e(float a) const {
         const float d = a - top;
-        if (a == top) return 1.f;
-        if (!(-d <= reach)) return 0.f;
-        float z;
-        if (mul) {
-            const float q = d * rt;
-            z = __fmaf_rn(__fmaf_rn(-q, t, d), rt, q);
-        } else {
-            z = __fdiv_rn(d, t);
-        }
-        const float v = expf(z);
-        return v >= 4.547473508864641e-13f ? v : 0.f;   // 2^-41: one half, which rounds to the even 0, has no weight either
+        if (!mul) return a == top ? 1.f : e_cut(expf(__fdiv_rn(d, t)));
+        const float q = d * rt;
+        return e_cut(expf(__fmaf_rn(__fmaf_rn(-q, t, d), rt, q)));
     }
+    __device__ __forceinline__ static float e_cut(float v) { return v >= 4.547473508864641e-13f ? v : 0.f; }
 };
 
 template <class T, class F>
@@ -629,31 +631,161 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample_long(const SampleArgs
     if (lane == 0) a.token[r] = i, a.logprob[r] = sample_logprob(row, i, total);
 }
 
+// ---- selection from the list, by one block
+constexpr int kSampleFew = 64;
+struct SampleList {
+    // tokens: the logit, its index, e (-1: struck off)
+    float x[kSampleList];
+    uint32_t i[kSampleList];
+    float e[kSampleList];
+    uint32_t count[kSampleRadix], hi[kSampleRadix], lo[kSampleRadix];
+    uint64_t few_key[kSampleFew], few_w[kSampleFew];
+    uint64_t red[32];
+    uint64_t got, sum, before;
+    uint32_t n, key_lo, key_hi;
+    int at;
+};
+enum SamplePick { kByCount, kByWeight, kByIndex };
+
+__device__ __forceinline__ uint32_t sample_order(float x) { return (uint32_t)(sample_rank_key(x, 0) >> 32); }
+
+// Of the list's m tokens that are not struck off: the one, in rank order (kByIndex: in index order), at which the running count
+// (kByCount) or sum of weights reaches want (>= 1).  Its rank key, or 0 if none does; *sum: the weights down to it (kByCount: all, if
+// none does).
+template <SamplePick BY>
+__device__ uint64_t sample_pick(SampleList& l, uint32_t m, uint64_t want, uint64_t* sum) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31;
+    bool by_order = BY != kByIndex;   // the search is on the logit's order first, then, among equal ones, on the index
+    uint32_t equal = 0;
+    uint64_t before = 0;
+    const auto key = [&](uint32_t j) { return by_order ? sample_order(l.x[j]) : 0xffffffffu - l.i[j]; };
+    const auto in = [&](uint32_t j) { return l.e[j] >= 0.f && (BY == kByIndex || by_order || sample_order(l.x[j]) == equal); };
+    uint32_t lo = 0, hi = 0xffffffffu;
+    if (m > kSampleFew) {
+        while (true) {
+            if (tid == 0) l.key_lo = 0xffffffffu, l.key_hi = 0;
+            __syncthreads();
+            uint32_t a = 0xffffffffu, b = 0;
+            for (uint32_t j = tid; j < m; j += kSampleThreads)
+                if (in(j)) a = min(a, key(j)), b = max(b, key(j));
+            a = __reduce_min_sync(0xffffffffu, a);
+            b = __reduce_max_sync(0xffffffffu, b);
+            if (lane == 0 && a <= b) atomicMin(&l.key_lo, a), atomicMax(&l.key_hi, b);
+            __syncthreads();
+            lo = l.key_lo;
+            hi = l.key_hi;
+            if (lo > hi) { *sum = before; return 0; }
+            uint32_t n;
+            while (true) {
+                // the tokens with keys in [lo, hi], in up to 1024 bins of equal width
+                const int shift = max(0, 32 - __clz(hi - lo) - 10);
+                l.count[tid] = l.hi[tid] = l.lo[tid] = 0;
+                if (tid == 0) l.at = -1;
+                __syncthreads();
+                for (uint32_t j = tid; j < m; j += kSampleThreads) {
+                    if (!in(j)) continue;
+                    const uint32_t k = key(j);
+                    if (k < lo || k > hi) continue;
+                    const uint32_t b = (hi - k) >> shift;
+                    const uint64_t w = sample_weight(l.e[j]);
+                    atomicAdd(&l.count[b], 1u);
+                    atomicAdd(&l.hi[b], (uint32_t)(w >> 20));        // the list's sums fit 32 bits in these halves
+                    atomicAdd(&l.lo[b], (uint32_t)w & 0xfffffu);
+                }
+                __syncthreads();
+                const uint64_t w = ((uint64_t)l.hi[tid] << 20) + l.lo[tid], own = BY == kByCount ? l.count[tid] : w;
+                const uint64_t run = sample_block_scan(own, l.red);
+                if (run >= want && run - own < want) l.at = tid, l.got = run - own;
+                if (tid == kSampleRadix - 1) l.sum = run;
+                __syncthreads();
+                const int at = l.at;
+                if (at < 0) {
+                    if (BY == kByCount) {
+                        uint64_t all = 0;
+                        for (uint32_t j = tid; j < m; j += kSampleThreads) all += in(j) ? sample_weight(l.e[j]) : 0;
+                        *sum = sample_reduce(all, [](uint64_t x, uint64_t y) { return x + y; }, l.red);
+                    } else {
+                        *sum = before + l.sum;
+                    }
+                    __syncthreads();
+                    return 0;
+                }
+                want -= l.got;
+                if (BY != kByCount) before += l.got;
+                n = l.count[at];
+                const uint32_t top = hi - ((uint32_t)at << shift), width = (1u << shift) - 1;
+                lo = top - lo > width ? top - width : lo;
+                hi = top;
+                __syncthreads();
+                if (n <= kSampleFew || shift == 0) break;
+            }
+            if (n <= kSampleFew) break;
+            by_order = false;   // more equal logits than that
+            equal = hi;
+        }
+    }
+    // few: each against the others
+    if (tid == 0) l.n = 0, l.got = 0, l.sum = before;
+    __syncthreads();
+    for (uint32_t j = tid; j < m; j += kSampleThreads) {
+        if (!in(j) || key(j) < lo || key(j) > hi) continue;
+        const uint32_t at = atomicAdd(&l.n, 1u);
+        l.few_key[at] = BY == kByIndex ? 0xffffffffu - l.i[j] : sample_rank_key(l.x[j], l.i[j]);
+        l.few_w[at] = sample_weight(l.e[j]);
+    }
+    __syncthreads();
+    const uint32_t n = l.n;
+    if (tid < n) {
+        const uint64_t k = l.few_key[tid], w = l.few_w[tid];
+        uint64_t c = 0, s = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < n; j++)
+            if (l.few_key[j] > k) c++, s += l.few_w[j];
+        const uint64_t run = BY == kByCount ? c : s, own = BY == kByCount ? 1 : w;
+        if (run < want && run + own >= want) l.got = k, l.sum = before + s + w;
+    }
+    __syncthreads();
+    const uint64_t k = l.got;
+    if (BY == kByCount) {
+        // the weights down to it, whatever was left out of the few; all of them if no token is the one
+        uint64_t all = 0;
+        for (uint32_t j = tid; j < m; j += kSampleThreads)
+            all += l.e[j] >= 0.f && sample_rank_key(l.x[j], l.i[j]) >= k ? sample_weight(l.e[j]) : 0;
+        *sum = sample_reduce(all, [](uint64_t x, uint64_t y) { return x + y; }, l.red);
+    } else {
+        *sum = l.sum;
+    }
+    __syncthreads();
+    return k;
+}
+
+constexpr int kSampleCoarse = kSampleBins / 8;   // the histogram in eighths, which blocks read of one another first
 struct alignas(16) SampleShared {
-    SampleRadix radix;
+    union {
+        SampleList list;
+        SampleRadix radix;   // where the list will not do
+    };
     uint64_t sum[kSampleClusterMax], above[kSampleClusterMax], part[kSampleClusterMax];   // each block writes its own to all
-    float top[kSampleClusterMax];
+    float top[kSampleClusterMax], reach[kSampleClusterMax];
     uint32_t n[kSampleClusterMax];
     uint64_t bound, found;                  // block 0's answer
-    int slow, done;
+    int slow;
     uint64_t red[32];
     float redf[32];
-    uint64_t run_lo, run_all;
-    int at;
-    uint32_t listed;
-    // tokens of the bins around the last kept one: their index, then their rank key; their e
-    uint64_t list_k[kSampleList];
-    float list_e[kSampleList];
-    uint32_t counts[kSampleBins + 7], sums[kSampleBins + 7];
+    uint64_t run_all, run_at;
+    int at, lo;
+    uint32_t listed, least;
+    uint32_t warp_hi[kSampleWarps], warp_lo[kSampleWarps];
+    uint32_t counts[kSampleBins], sums[kSampleBins];
+    uint32_t coarse_counts[kSampleCoarse], coarse_sums[kSampleCoarse];
 };
-
-static_assert(sizeof(SampleShared) + kSamplePart * sizeof(float) <= 232448, "a block's shared memory");
+static_assert(sizeof(SampleShared) + (kSamplePart + 128) * sizeof(float) <= 232448, "a block's shared memory");
 
 // n logits from row.p + first -> buf, as float32 without NaN; the calling thread's largest
 template <class T>
 __device__ __forceinline__ float sample_load(const SampleRow& row, int first, int n, float* buf) {
     const T* src = static_cast<const T*>(row.p) + first;
-    constexpr int kVec = 16 / sizeof(T), kDeep = 4;
+    constexpr int kVec = 16 / sizeof(T), kDeep = sizeof(T) == 4 ? 7 : 4;
     float top = -INFINITY;
     int done = 0;
     if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
@@ -699,10 +831,21 @@ __device__ __forceinline__ float sample_load(const SampleRow& row, int first, in
     return top;
 }
 
+// Value v of each block of the cluster, v at the same place of its SampleShared
+template <class T>
+__device__ __forceinline__ uint64_t sample_across(const cooperative_groups::cluster_group& cluster, T* v, int nb) {
+    uint64_t sum = 0;
+#pragma unroll
+    for (int q = 0; q < kSampleClusterMax; q++)
+        if (q < nb) sum += *cluster.map_shared_rank(v, q);
+    return sum;
+}
+
 __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) uint8_t ssm[];
     SampleShared& sh = *reinterpret_cast<SampleShared*>(ssm);
+    SampleList& list = sh.list;
     float* buf = reinterpret_cast<float*>(ssm + sizeof(SampleShared));
     cg::cluster_group cluster = cg::this_cluster();
     const int nb = cluster.num_blocks(), rank = cluster.block_rank(), r = blockIdx.x / nb;
@@ -711,173 +854,252 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
     const SampleSettings set(a, r);
     const bool by_k = set.k != 0, by_p = set.p < 1.f;
     const auto add = [](uint64_t x, uint64_t y) { return x + y; };
+    const auto larger = [](float x, float y) { return fmaxf(x, y); };
     SampleRow row;
     row.set(a, r);
     const int part = ((row.v + nb - 1) / nb + 7) / 8 * 8, first = min(row.v, rank * part), n = min(row.v, first + part) - first;
 
-    float top = a.type == FHE_F32   ? sample_load<float>(row, first, n, buf)
-                : a.type == FHE_F16 ? sample_load<__half>(row, first, n, buf)
-                                    : sample_load<__nv_bfloat16>(row, first, n, buf);
-    if (by_k || by_p)
-        for (int b = tid; b < kSampleBins; b += kSampleThreads) sh.counts[b] = 0, sh.sums[b] = 0;
-    top = sample_reduce(top, [](float x, float y) { return fmaxf(x, y); }, sh.redf);
+    const float mine = a.type == FHE_F32   ? sample_load<float>(row, first, n, buf)
+                       : a.type == FHE_F16 ? sample_load<__half>(row, first, n, buf)
+                                           : sample_load<__nv_bfloat16>(row, first, n, buf);
+    const int n4 = (n + 127) / 128 * 128;   // whole warps of four values a lane
+    if (tid < n4 - n) buf[n + tid] = -INFINITY;
+    float top = sample_reduce(mine, larger, sh.redf);
+    // the least value that top_k threads' own maxima reach, to within a 1024th of their range
+    bool few = by_k && set.k <= kSampleRadix;
+    float reach = -INFINITY;
+    if (few) {
+        const float low = -sample_reduce(mine > -INFINITY ? -mine : -INFINITY, larger, sh.redf);
+        list.count[tid] = 0;
+        if (tid == 0) sh.at = -1, sh.least = 0xffffffffu;
+        __syncthreads();
+        const float width = top - low;
+        int b = kSampleRadix;
+        if (mine > -INFINITY) {
+            b = mine == top ? 0 : (int)fminf((top - mine) / width * (kSampleRadix - 1), (float)(kSampleRadix - 1));
+            atomicAdd(&list.count[b], 1u);
+        }
+        __syncthreads();
+        const uint32_t own = list.count[tid], run = sample_block_scan(own, reinterpret_cast<uint32_t*>(sh.red));
+        if (run >= set.k && run - own < set.k) sh.at = tid;
+        __syncthreads();
+        if (b <= sh.at) atomicMin(&sh.least, sample_order(mine));
+        __syncthreads();
+        if (sh.at >= 0) {
+            const uint32_t o = sh.least;
+            reach = __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+        }
+    }
     cluster.barrier_wait();   // every block runs
-    if (tid < nb) *cluster.map_shared_rank(&sh.top[rank], tid) = top;
+    if (tid < nb) {
+        SampleShared* o = cluster.map_shared_rank(&sh, tid);
+        o->top[rank] = top;
+        o->reach[rank] = reach;
+    }
+    if (tid == 0) sh.listed = 0;
     cluster.sync();
-    for (int b = 0; b < nb; b++) top = fmaxf(top, sh.top[b]);
+    for (int b = 0; b < nb; b++) top = fmaxf(top, sh.top[b]), reach = fmaxf(reach, sh.reach[b]);
     if (top == -INFINITY) {   // in every block of the cluster
         if (rank == 0 && tid == 0) a.token[r] = -1, a.logprob[r] = -INFINITY;
         return;
     }
     row.scale(top, set.t);
+    // each warp's stretch
+    const int per = (n4 + 128 * kSampleWarps - 1) / (128 * kSampleWarps) * 128, i0 = min(n4, warp * per), i1 = min(n4, i0 + per);
 
-    // e in the logits' place, each warp its stretch; the histograms
-    const int per = (n + kSampleThreads - 1) / kSampleThreads * 32, i0 = min(n, warp * per), i1 = min(n, i0 + per);
-    uint64_t all = 0;   // the whole sum
-    {
-        uint32_t hi = 0, lo = 0;
-        for (int i = i0 + lane; i < i1; i += 32) {
-            const float e = row.e(buf[i]);
-            buf[i] = e;
-            if (e > 0.f && (by_k || by_p)) {
-                const int b = sample_bin(e);
-                if (by_k) atomicAdd(&sh.counts[b], 1u);
-                if (by_p) {
-                    // 16 bits of e: a block's 2^15 tokens add up to less than 2^31
-                    atomicAdd(&sh.sums[b], (__float_as_uint(e) >> 8 & 0x7fffu) | 0x8000u);
-                    sample_weight_add(e, hi, lo);
+    if (few) {
+        const auto take = [&](float x, int i) {
+            if (x >= reach && x > -INFINITY) {
+                const uint32_t j = atomicAdd(&sh.listed, 1u);
+                if (j < kSampleList) list.x[j] = x, list.i[j] = first + i;
+            }
+        };
+        for (int i = i0 + 4 * lane; i < i1; i += 128) {
+            const float4 x = *reinterpret_cast<const float4*>(buf + i);
+            if (fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= reach) take(x.x, i), take(x.y, i + 1), take(x.z, i + 2), take(x.w, i + 3);
+        }
+        __syncthreads();
+        if (tid < nb) *cluster.map_shared_rank(&sh.n[rank], tid) = sh.listed;
+        cluster.sync();
+        uint32_t m = 0;
+        for (int q = 0; q < nb; q++) m += sh.n[q];
+        if (m <= kSampleList) {
+            if (rank == 0) {
+                uint32_t off = sh.n[0];
+                for (int q = 1; q < nb; q++) {
+                    const SampleList* o = &cluster.map_shared_rank(&sh, q)->list;
+                    for (uint32_t j = tid; j < sh.n[q]; j += kSampleThreads) list.x[off + j] = o->x[j], list.i[off + j] = o->i[j];
+                    off += sh.n[q];
                 }
             }
+            if (nb > 1) cluster.sync();
+            if (rank) return;
+            __syncthreads();
+            const auto strike = [&](uint64_t bound) {
+                for (uint32_t j = tid; j < m; j += kSampleThreads)
+                    if (sample_rank_key(list.x[j], list.i[j]) < bound) list.e[j] = -1.f;
+                __syncthreads();
+            };
+            for (uint32_t j = tid; j < m; j += kSampleThreads) list.e[j] = row.e(list.x[j]);
+            __syncthreads();
+            uint64_t sum, total, unused;
+            strike(sample_pick<kByCount>(list, m, set.k, &sum));
+            if (by_p) strike(sample_pick<kByWeight>(list, m, set.limit(sum), &sum));
+            uint64_t w = 0;
+            for (uint32_t j = tid; j < m; j += kSampleThreads) {
+                if (list.e[j] < set.mp) list.e[j] = -1.f;
+                if (list.e[j] > 0.f) w += sample_weight(list.e[j]);
+            }
+            total = sample_reduce(w, add, sh.red);
+            const uint64_t pick = sample_pick<kByIndex>(list, m, set.target(total) + 1, &unused);
+            if (tid == 0) {
+                const int i = (int)(0xffffffffu - (uint32_t)pick);
+                a.token[r] = i;
+                a.logprob[r] = sample_logprob(row, i, total);
+            }
+            return;
         }
-        if (by_p) {
-            const uint64_t s = sample_reduce(((uint64_t)hi << 20) + lo, add, sh.red);
-            if (tid < nb) *cluster.map_shared_rank(&sh.sum[rank], tid) = s;
+    }
+
+    // e in the logits' place; the histograms
+    if (by_k || by_p)
+        for (int b = tid; b < kSampleBins; b += kSampleThreads) sh.counts[b] = 0, sh.sums[b] = 0;
+    if (tid < kSampleWarps) sh.warp_hi[tid] = sh.warp_lo[tid] = 0;
+    __syncthreads();
+    uint64_t all = 0;   // the whole sum
+    uint32_t hi = 0, lo = 0;
+    for (int i = i0 + 4 * lane; i < i1; i += 128) {
+        const float4 x = *reinterpret_cast<const float4*>(buf + i);
+        float e[4] = {row.e(x.x), row.e(x.y), row.e(x.z), row.e(x.w)};
+        *reinterpret_cast<float4*>(buf + i) = make_float4(e[0], e[1], e[2], e[3]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            sample_weight_add(e[j] >= set.mp || by_p ? e[j] : 0.f, hi, lo);
+            if (e[j] > 0.f) {
+                if (by_k) atomicAdd(&sh.counts[sample_bin(e[j])], 1u);
+                // 16 bits of e: a block's 2^15 tokens add up to less than 2^31
+                if (by_p) atomicAdd(&sh.sums[sample_bin(e[j])], (__float_as_uint(e[j]) >> 8 & 0x7fffu) | 0x8000u);
+            }
         }
-        if (by_k || by_p) cluster.sync();
-        if (by_p)
-            for (int b = 0; b < nb; b++) all += sh.sum[b];
+    }
+    // the weights of this warp's stretch: all of them if top_p needs their sum, else those that min_p keeps
+    const auto stretch = [&](uint32_t hi, uint32_t lo) {
+        uint64_t w = ((uint64_t)hi << 20) + lo;
+        for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        return w;
+    };
+    uint64_t warp_w = stretch(hi, lo);
+    const auto block_sum = [&](uint64_t w) {
+        __syncthreads();
+        if (lane == 0) sh.red[warp] = w;
+        __syncthreads();
+        uint64_t s = sh.red[lane];
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        return s;
+    };
+    if (by_k || by_p) {
+        const uint64_t s = block_sum(warp_w);
+        if (tid < kSampleCoarse) {
+            uint32_t c = 0, v = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) c += sh.counts[tid * 8 + j], v += sh.sums[tid * 8 + j];
+            sh.coarse_counts[tid] = c;
+            sh.coarse_sums[tid] = v;
+        }
+        if (tid < nb) *cluster.map_shared_rank(&sh.sum[rank], tid) = s;
+        cluster.sync();
+        for (int b = 0; b < nb; b++) all += sh.sum[b];
     }
 
     uint32_t cut = 0;   // kept are e with bits above this, and whatever the lists have not struck off
+    bool summed = !by_k && (!by_p || set.mp == 0.f);   // warp_w follows what is kept as it is found
     // One selection.  The histogram tells a guess of the last kept token's bin; the tokens of that bin and its neighbours go to
-    // the list (by count, and where they are few, all the tokens above as well), the weights above are summed, and block 0 selects.
-    auto locate = [&](bool by_count, uint64_t want) {
-        constexpr int kPer = (kSampleBins + kSampleThreads - 1) / kSampleThreads;
-        uint64_t own[kPer], mine = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; j++) {
-            const int b = tid * kPer + j;
-            uint64_t v = 0;
-            if (b < kSampleBins)
-                for (int q = 0; q < nb; q++) {
-                    const SampleShared* o = cluster.map_shared_rank(&sh, q);
-                    v += by_count ? o->counts[b] : o->sums[b];
-                }
-            // a sum is in units of 2^-15 of its octave's top
-            const int up = 40 - 15 - (b + 127) / 128;
-            own[j] = by_count ? v : up >= 0 ? v << up : v >> -up;
-            mine += own[j];
+    // the list, the weights above are summed, and block 0 selects.
+    const auto locate = [&](bool by_count, uint64_t want) {
+        const uint32_t* coarse = by_count ? sh.coarse_counts : sh.coarse_sums;
+        const uint32_t* fine = by_count ? sh.counts : sh.sums;
+        uint64_t own = 0;
+        if (tid < kSampleCoarse) {
+            own = sample_across(cluster, &coarse[tid], nb);
+            if (!by_count) own = sample_bin_sum(own, tid * 8);
         }
-        uint64_t run = sample_block_scan(mine, sh.red);
+        const uint64_t run = sample_block_scan(own, sh.red);
         if (tid == kSampleThreads - 1) sh.run_all = run;
-        if (tid == 0) sh.at = kSampleBins, sh.listed = 0, sh.run_lo = 0;
-        run -= mine;
+        if (tid == 0) sh.at = -1, sh.listed = 0;
         __syncthreads();
-        // the sums' 16 bits are cut off, all alike
         uint64_t guess = want;
         if (!by_count) {
+            // all sums lack the bits below the leading 16 alike
             guess = (uint64_t)((double)want * ((double)sh.run_all / (double)all));
             guess = guess < 1 ? 1 : guess > sh.run_all ? sh.run_all : guess;
         }
-        uint64_t v = run;
-#pragma unroll
-        for (int j = 0; j < kPer; j++) {
-            if (v < guess && v + own[j] >= guess) sh.at = tid * kPer + j;
-            v += own[j];
-        }
+        if (run >= guess && run - own < guess) sh.at = tid, sh.run_at = run - own;
         __syncthreads();
-        const int at = sh.at;
-        if (by_count && at == kSampleBins) {   // no more than top_k have a weight: nothing is struck off
-            if (tid == 0) sh.done = 0, sh.found = all;
+        if (sh.at < 0) {   // no more than top_k have a weight: nothing is struck off
+            __syncthreads();
+            if (tid == 0) sh.found = all;
             __syncthreads();
             return;
         }
-        const int lo = by_count && want <= kSampleRadix ? 0 : max(0, at - 1), hi = min(kSampleBins - 1, at + 1);
-        if (by_count) {
-            v = run;
+        if (warp == 0) {
+            // the bin before the eighth's first (lane 0), its 8 bins (1 to 8)
+            const int b = sh.at * 8 - 1 + lane;
+            uint64_t v = lane < 9 && b >= 0 ? sample_across(cluster, &fine[b], nb) : 0;
+            if (!by_count) v = sample_bin_sum(v, b);
+            const uint64_t upto = sh.run_at - __shfl_sync(0xffffffffu, v, 0) + sample_scan(v);
+            const uint32_t past = __ballot_sync(0xffffffffu, lane >= 1 && lane < 9 && upto >= guess);
+            const int l = past ? __ffs(past) - 1 : 8;   // none: what single bins lose below 2^-40
+            // one bin to either side: equal to the last place, exponentials need not be in their logits' order
+            if (lane == l - 1) sh.lo = max(0, b), sh.run_at = upto - v;
+        }
+        __syncthreads();
+        const int b0 = sh.lo, b1 = min(kSampleBins - 1, b0 + 2);
+        const uint32_t above = sample_bin_bits(b0), in = max(cut, sample_bin_bits(b1 + 1));
+        uint32_t hi = 0, lo = 0;
+        for (int i = i0 + 4 * lane; i < i1; i += 128) {
+            const float4 x = *reinterpret_cast<const float4*>(buf + i);
+            const float e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int j = 0; j < kPer; j++) {
-                if (tid * kPer + j == lo) sh.run_lo = v;
-                v += own[j];
+            for (int j = 0; j < 4; j++) {
+                const uint32_t bits = __float_as_uint(e[j]);
+                sample_weight_add(bits > above ? e[j] : 0.f, hi, lo);
+                if (bits > in && bits <= above) {
+                    const uint32_t at = atomicAdd(&sh.listed, 1u);
+                    if (at < kSampleList) list.i[at] = first + i + j, list.e[at] = e[j];
+                }
             }
         }
-        const uint32_t above = sample_bin_bits(lo), in = max(cut, sample_bin_bits(hi + 1));
-        uint32_t wh = 0, wl = 0;
-        for (int i = i0; i < i1; i += 32) {
-            const float e = i + lane < i1 ? buf[i + lane] : 0.f;
-            const uint32_t bits = __float_as_uint(e);
-            if (bits > above) sample_weight_add(e, wh, wl);
-            const bool hit = bits > in && bits <= above;
-            const uint32_t hits = __ballot_sync(0xffffffffu, hit);
-            if (hits) {
-                uint32_t j = 0;
-                if (lane == 0) j = atomicAdd(&sh.listed, __popc(hits));
-                j = __shfl_sync(0xffffffffu, j, 0) + __popc(hits & ((1u << lane) - 1));
-                if (hit && j < kSampleList) sh.list_k[j] = first + i + lane, sh.list_e[j] = e;
-            }
-        }
-        const uint64_t s = sample_reduce(((uint64_t)wh << 20) + wl, add, sh.red);
-        const uint32_t listed = min(sh.listed, (uint32_t)kSampleList);   // sample_reduce has waited for all
-        for (uint32_t j = tid; j < listed; j += kSampleThreads) {
-            const uint32_t i = (uint32_t)sh.list_k[j];
-            sh.list_k[j] = sample_rank_key(row.x(i), i);
-        }
+        warp_w = stretch(hi, lo);
+        const uint64_t s = block_sum(warp_w);
+        const uint32_t listed = min(sh.listed, (uint32_t)kSampleList);
+        for (uint32_t j = tid; j < listed; j += kSampleThreads) list.x[j] = row.x(list.i[j]);
         if (tid < nb) {
-            *cluster.map_shared_rank(&sh.above[rank], tid) = s;
-            *cluster.map_shared_rank(&sh.n[rank], tid) = sh.listed;
+            SampleShared* o = cluster.map_shared_rank(&sh, tid);
+            o->above[rank] = s;
+            o->n[rank] = sh.listed;
         }
         cluster.sync();
         if (rank == 0) {
-            uint64_t over = 0;
+            uint64_t over = 0, bound = 0, found = 0;
             uint32_t m = 0;
-            bool slow = false;
-            for (int q = 0; q < nb; q++) {
-                over += sh.above[q];
-                m += sh.n[q];
-                slow |= m > kSampleList;   // also if one block's list is cut off
-            }
-            uint64_t bound = 0, found = 0;
-            int done = 0;
+            for (int q = 0; q < nb; q++) over += sh.above[q], m += sh.n[q];
+            bool slow = m > kSampleList || (!by_count && over >= want);
             if (!slow) {
                 uint32_t off = sh.n[0];
                 for (int q = 1; q < nb; q++) {
-                    const SampleShared* o = cluster.map_shared_rank(&sh, q);
+                    const SampleList* o = &cluster.map_shared_rank(&sh, q)->list;
                     for (uint32_t j = tid; j < sh.n[q]; j += kSampleThreads)
-                        sh.list_k[off + j] = o->list_k[j], sh.list_e[off + j] = o->list_e[j];
+                        list.x[off + j] = o->x[j], list.i[off + j] = o->i[j], list.e[off + j] = o->e[j];
                     off += sh.n[q];
                 }
                 __syncthreads();
-                auto each = [&](auto f) {
-                    for (uint32_t j = tid; j < m; j += kSampleThreads) f(sh.list_k[j], sh.list_e[j]);
-                };
-                if (by_count) {
-                    const SampleFound f = sample_select<true>(sh.radix, want - sh.run_lo, each);
-                    bound = f.key;
-                    found = over + f.sum;
-                    slow = bound == 0;
-                    if (!slow && by_p && lo == 0) {
-                        bound = max(bound, sample_select<false>(sh.radix, set.limit(found), each).key);
-                        done = 1;
-                    }
-                } else if (over < want) {
-                    bound = sample_select<false>(sh.radix, want - over, each).key;
-                    slow = bound == 0;
-                } else {
-                    slow = true;
-                }
+                bound = by_count ? sample_pick<kByCount>(list, m, want - sh.run_at, &found)
+                                 : sample_pick<kByWeight>(list, m, want - over, &found);
+                found += over;
+                slow = bound == 0;
             }
             if (slow) {
-                auto each = [&](auto f) {
+                const auto each = [&](auto f) {
                     for (int i = tid; i < row.v; i += kSampleThreads) {
                         const float x = row.x(i);
                         if (row.counts(x)) f(sample_rank_key(x, i), row.e(x));
@@ -893,52 +1115,76 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
                 o->bound = bound;
                 o->found = found;
                 o->slow = slow;
-                o->done = done;
             }
         }
         cluster.sync();
         const uint64_t bound = sh.bound;
         if (sh.slow) {
-            for (int i = i0 + lane; i < i1; i += 32)
+            for (int i = i0 + lane; i < min(i1, n); i += 32)
                 if (sample_rank_key(row.x(first + i), first + i) < bound) buf[i] = 0.f;
+            summed = false;
         } else {
-            for (uint32_t j = tid; j < listed; j += kSampleThreads)
-                if (sh.list_k[j] < bound) buf[0xffffffffu - (uint32_t)sh.list_k[j] - first] = 0.f;
+            for (uint32_t j = tid; j < listed; j += kSampleThreads) {
+                const uint32_t i = list.i[j] - first;
+                if (sample_rank_key(list.x[j], list.i[j]) < bound) {
+                    buf[i] = 0.f;
+                } else if (summed) {
+                    const uint64_t w = sample_weight(list.e[j]);
+                    atomicAdd(&sh.warp_hi[i / per], (uint32_t)(w >> 20));
+                    atomicAdd(&sh.warp_lo[i / per], (uint32_t)w & 0xfffffu);
+                }
+            }
             cut = in;
         }
         __syncthreads();
     };
     if (by_k) locate(true, set.k);
-    if (by_p && !(by_k && sh.done)) locate(false, set.limit(by_k ? sh.found : all));
+    if (by_p) locate(false, set.limit(by_k ? sh.found : all));
 
-    // the kept weights of each warp's stretch, block and cluster; the block that the target falls to walks
-    auto kept = [&](int i) -> float {
-        const float e = buf[i];
-        return __float_as_uint(e) > cut && e >= set.mp ? e : 0.f;
-    };
-    uint32_t wh = 0, wl = 0;
-    for (int i = i0 + lane; i < i1; i += 32) sample_weight_add(kept(i), wh, wl);
-    uint64_t mine = ((uint64_t)wh << 20) + wl;
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    __syncthreads();
-    if (lane == 0) sh.red[warp] = mine;
-    __syncthreads();
-    uint64_t start = 0, total = 0;
-    for (int w = 0; w < kSampleWarps; w++) {
-        if (w == warp) start = total;
-        total += sh.red[w];
+    // the kept weights of each warp's stretch, block and cluster; the warp that the target falls to walks
+    const auto kept = [&](float e) { return __float_as_uint(e) > cut && e >= set.mp ? e : 0.f; };
+    if (summed) {
+        warp_w += ((uint64_t)sh.warp_hi[warp] << 20) + sh.warp_lo[warp];
+    } else {
+        uint32_t hi = 0, lo = 0;
+        for (int i = i0 + 4 * lane; i < i1; i += 128) {
+            const float4 e = *reinterpret_cast<const float4*>(buf + i);
+            sample_weight_add(kept(e.x), hi, lo);
+            sample_weight_add(kept(e.y), hi, lo);
+            sample_weight_add(kept(e.z), hi, lo);
+            sample_weight_add(kept(e.w), hi, lo);
+        }
+        warp_w = stretch(hi, lo);
     }
+    uint64_t total = block_sum(warp_w);
     if (tid < nb) *cluster.map_shared_rank(&sh.part[rank], tid) = total;
     cluster.sync();
     total = 0;
+    uint64_t start = 0;
     for (int b = 0; b < nb; b++) {
-        if (b == rank) start += total;
+        if (b == rank) start = total;
         total += sh.part[b];
     }
+    for (int w = 0; w < warp; w++) start += sh.red[w];   // block_sum's
     const uint64_t target = set.target(total);
-    if (target < start || target >= start + mine) return;
-    const int i = first + sample_walk(i0, i1, start, target, [&](int j) { return sample_weight(kept(j)); });
-    if (lane == 0) a.token[r] = i, a.logprob[r] = sample_logprob(row, i, total);
+    if (target < start || target >= start + warp_w) return;
+    for (int i = i0 + 4 * lane;; i += 128) {   // ends: the stretch's weights pass the target
+        const float4 e = *reinterpret_cast<const float4*>(buf + i);
+        const uint64_t w[4] = {sample_weight(kept(e.x)), sample_weight(kept(e.y)), sample_weight(kept(e.z)),
+                               sample_weight(kept(e.w))};
+        uint64_t run = start + sample_scan(w[0] + w[1] + w[2] + w[3]);
+        const uint32_t past = __ballot_sync(0xffffffffu, run > target);
+        if (past) {
+            if (lane == __ffs(past) - 1) {
+                int j = 3;
+                while (run - w[j] > target) run -= w[j--];
+                a.token[r] = first + i + j;
+                a.logprob[r] = sample_logprob(row, first + i + j, total);
+            }
+            return;
+        }
+        start = __shfl_sync(0xffffffffu, run, 31);
+    }
 }
 
 static void sample(Context& cx, const SampleArgs& a, cudaStream_t st) {
@@ -949,7 +1195,7 @@ static void sample(Context& cx, const SampleArgs& a, cudaStream_t st) {
         k_sample_long<<<a.rows, kSampleThreads, 0, st>>>(a);
         CUDA_CHECK(cudaGetLastError());
     } else {
-        const size_t smem = sizeof(SampleShared) + ((size_t)(a.vocab + nb - 1) / nb + 7) / 8 * 8 * sizeof(float);
+        const size_t smem = sizeof(SampleShared) + (((size_t)a.vocab + nb - 1) / nb + 8 + 128) * sizeof(float);
         client_smem<k_sample>(cx);
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)a.rows * nb);

@@ -217,6 +217,30 @@ def test_sample_settings_of_each_row(cx):
     assert token[7] == -1 and token[9] == 17
 
 
+@pytest.mark.parametrize("vocab", [40, 3266, 20000])
+def test_sample_few_allowed(cx, vocab):
+    """Rows that allow fewer tokens than top_k, one to thirty, spread over the whole row or all at its end."""
+    rng = np.random.default_rng(vocab)
+    for kw in (dict(k=50, p=0.9), dict(p=0.9), dict(k=2, p=0.99), dict(k=1500, p=0.7), dict(mp=0.3)):
+        x = np.full((6, vocab), -np.inf, np.float32)
+        for r in range(6):
+            at = rng.choice(vocab, 1 + 5 * r, replace=False) if r % 2 else np.arange(vocab - 1 - 5 * r, vocab)
+            x[r, at] = rng.normal(0, 2, len(at))
+        u = torch.from_numpy(rng.uniform(0, 0.999, 6).astype(np.float32)).cuda()
+        check_sample(cx, torch.from_numpy(x).cuda(), u, **kw)
+
+
+@pytest.mark.parametrize("xt", ["f32", "f16"])
+def test_sample_long_rows(cx, xt):
+    """Rows longer than a cluster of blocks holds, and the longest that it does."""
+    rng = np.random.default_rng(8)
+    for vocab in (262144, 262145, 400001):
+        x = torch.from_numpy(rng.normal(0, 1.5, (2, vocab)).astype(np.float32)).to(TYPES[xt]).cuda()
+        u = torch.from_numpy(rng.uniform(0, 0.999, 2).astype(np.float32)).cuda()
+        for kw in (dict(t=0.6, k=50, p=0.95), dict(t=0.8, p=0.9), dict(k=3000, p=0.8, mp=0.001)):
+            check_sample(cx, x, u, **kw)
+
+
 @pytest.mark.parametrize("xt", ["f32", "bf16"])
 @pytest.mark.parametrize("vocab", [6, 100, 2049, 5000, 70001])
 def test_sample_ties_by_index(cx, vocab, xt):
