@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample_long(const SampleArgs
 }
 
 // ---- selection from the list, by one block
-constexpr int kSampleFew = 64;
+constexpr int kSampleFew = 64, kSampleSmall = 256;
 struct SampleList {
     // tokens: the logit, its index, e (-1: struck off)
     float x[kSampleList];
@@ -640,6 +640,7 @@ struct SampleList {
     float e[kSampleList];
     uint32_t count[kSampleRadix], hi[kSampleRadix], lo[kSampleRadix];
     uint64_t few_key[kSampleFew], few_w[kSampleFew];
+    uint64_t small_k[kSampleSmall], small_w[kSampleSmall];
     uint64_t red[32];
     uint64_t got, sum, before;
     uint32_t n, key_lo, key_hi;
@@ -853,8 +854,18 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
     cluster.barrier_arrive();
     const SampleSettings set(a, r);
     const bool by_k = set.k != 0, by_p = set.p < 1.f;
-    const auto add = [](uint64_t x, uint64_t y) { return x + y; };
     const auto larger = [](float x, float y) { return fmaxf(x, y); };
+    const auto warp_sum = [&](uint64_t w) {
+        for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        return w;
+    };
+    const auto warps_sum = [&](uint64_t w) {   // of one value a warp, which stay in sh.red
+        __syncthreads();
+        if (lane == 0) sh.red[warp] = w;
+        __syncthreads();
+        return warp_sum(sh.red[lane]);
+    };
+    const auto block_sum = [&](uint64_t w) { return warps_sum(warp_sum(w)); };
     SampleRow row;
     row.set(a, r);
     const int part = ((row.v + nb - 1) / nb + 7) / 8 * 8, first = min(row.v, rank * part), n = min(row.v, first + part) - first;
@@ -935,6 +946,42 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
             if (nb > 1) cluster.sync();
             if (rank) return;
             __syncthreads();
+            uint64_t sum, total, pick;
+            if (m <= kSampleSmall) {
+                // Each token against the others, 4 to 32 threads a token: how many are ranked before it and their weights say
+                // whether it is kept, the kept ones of lower index where its share of the sum begins.
+                const int wide = m <= 32 ? 32 : m <= 64 ? 16 : m <= 128 ? 8 : 4;
+                const uint32_t j = tid / wide, sub = tid & (wide - 1);
+                if (tid < m) {
+                    list.small_k[tid] = sample_rank_key(list.x[tid], list.i[tid]);
+                    list.small_w[tid] = sample_weight(list.e[tid] = row.e(list.x[tid]));
+                }
+                __syncthreads();
+                const uint64_t k = j < m ? list.small_k[j] : 0, w = j < m ? list.small_w[j] : 0;
+                uint32_t c = 0;
+                uint64_t s = 0;
+                for (uint32_t l = sub; l < m; l += wide)
+                    if (list.small_k[l] > k) c++, s += list.small_w[l];
+                for (int o = wide / 2; o; o >>= 1) {
+                    c += __shfl_xor_sync(0xffffffffu, c, o);
+                    s += __shfl_xor_sync(0xffffffffu, s, o);
+                }
+                bool in = j < m && c < set.k;
+                sum = block_sum(in && sub == 0 ? w : 0);
+                in = in && (!by_p || s < set.limit(sum)) && list.e[j] >= set.mp;
+                if (sub == 0 && j < m) list.small_w[j] = in ? w : 0;   // block_sum has waited for the readers
+                total = block_sum(in && sub == 0 ? w : 0);
+                const uint64_t target = set.target(total);
+                s = 0;
+                for (uint32_t l = sub; l < m; l += wide)
+                    if ((uint32_t)list.small_k[l] > (uint32_t)k) s += list.small_w[l];
+                for (int o = wide / 2; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (in && sub == 0 && s <= target && s + w > target) {
+                    a.token[r] = list.i[j];
+                    a.logprob[r] = sample_logprob(row, list.i[j], total);
+                }
+                return;
+            }
             const auto strike = [&](uint64_t bound) {
                 for (uint32_t j = tid; j < m; j += kSampleThreads)
                     if (sample_rank_key(list.x[j], list.i[j]) < bound) list.e[j] = -1.f;
@@ -942,7 +989,7 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
             };
             for (uint32_t j = tid; j < m; j += kSampleThreads) list.e[j] = row.e(list.x[j]);
             __syncthreads();
-            uint64_t sum, total, unused;
+            uint64_t unused;
             strike(sample_pick<kByCount>(list, m, set.k, &sum));
             if (by_p) strike(sample_pick<kByWeight>(list, m, set.limit(sum), &sum));
             uint64_t w = 0;
@@ -950,8 +997,8 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
                 if (list.e[j] < set.mp) list.e[j] = -1.f;
                 if (list.e[j] > 0.f) w += sample_weight(list.e[j]);
             }
-            total = sample_reduce(w, add, sh.red);
-            const uint64_t pick = sample_pick<kByIndex>(list, m, set.target(total) + 1, &unused);
+            total = block_sum(w);
+            pick = sample_pick<kByIndex>(list, m, set.target(total) + 1, &unused);
             if (tid == 0) {
                 const int i = (int)(0xffffffffu - (uint32_t)pick);
                 a.token[r] = i;
@@ -983,22 +1030,10 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
         }
     }
     // the weights of this warp's stretch: all of them if top_p needs their sum, else those that min_p keeps
-    const auto stretch = [&](uint32_t hi, uint32_t lo) {
-        uint64_t w = ((uint64_t)hi << 20) + lo;
-        for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-        return w;
-    };
+    const auto stretch = [&](uint32_t hi, uint32_t lo) { return warp_sum(((uint64_t)hi << 20) + lo); };
     uint64_t warp_w = stretch(hi, lo);
-    const auto block_sum = [&](uint64_t w) {
-        __syncthreads();
-        if (lane == 0) sh.red[warp] = w;
-        __syncthreads();
-        uint64_t s = sh.red[lane];
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        return s;
-    };
     if (by_k || by_p) {
-        const uint64_t s = block_sum(warp_w);
+        const uint64_t s = warps_sum(warp_w);
         if (tid < kSampleCoarse) {
             uint32_t c = 0, v = 0;
 #pragma unroll
@@ -1070,7 +1105,7 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
             }
         }
         warp_w = stretch(hi, lo);
-        const uint64_t s = block_sum(warp_w);
+        const uint64_t s = warps_sum(warp_w);
         const uint32_t listed = min(sh.listed, (uint32_t)kSampleList);
         for (uint32_t j = tid; j < listed; j += kSampleThreads) list.x[j] = row.x(list.i[j]);
         if (tid < nb) {
@@ -1156,7 +1191,7 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
         }
         warp_w = stretch(hi, lo);
     }
-    uint64_t total = block_sum(warp_w);
+    uint64_t total = warps_sum(warp_w);
     if (tid < nb) *cluster.map_shared_rank(&sh.part[rank], tid) = total;
     cluster.sync();
     total = 0;
@@ -1165,7 +1200,7 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
         if (b == rank) start = total;
         total += sh.part[b];
     }
-    for (int w = 0; w < warp; w++) start += sh.red[w];   // block_sum's
+    for (int w = 0; w < warp; w++) start += sh.red[w];   // warps_sum's
     const uint64_t target = set.target(total);
     if (target < start || target >= start + warp_w) return;
     for (int i = i0 + 4 * lane;; i += 128) {   // ends: the stretch's weights pass the target
