@@ -303,10 +303,58 @@ static void q4_mma_split(Context& cx, const Q4Args& a, cudaStream_t st) {
     else q4_mma_launch<NT, 4>(cx, a, st);
 }
 
+#include "q4_gemm.cuh"
+
+template <int N, int KC, class XT>
+static void q4_gemm_launch(Context& cx, QgArgs a, cudaStream_t st) {
+    constexpr int kSlot = N * KC * 2 * (std::is_same<XT, float>::value ? 2 : 1), kJob = 128 / KC;
+    const int waves = (a.w.rows + 148 * kQgRowsMax - 1) / (148 * kQgRowsMax), xt = (a.m + N - 1) / N;
+    a.block_rows = std::min(kQgRowsMax, ((a.w.rows + 148 * waves - 1) / (148 * waves) + 31) / 32 * 32);
+    a.chunks = (a.w.cols + 127) / 128 * kJob;
+    a.slots = std::min({kQgSlotsMax, kQgXBytes / kSlot, a.chunks});
+    a.groups = std::min((a.slots * KC + a.w.group - 2) / a.w.group + 1, (a.w.cols + a.w.group - 1) / a.w.group + 1);
+    a.run = KC == 64 && a.w.group % 128 == 0 ? 2 : 1;
+    const size_t smem = 2 * kQgStages * kQgStageBytes + (size_t)a.slots * kSlot + (size_t)a.groups * 1024 + sizeof(QgBars);
+    const size_t image = (size_t)xt * a.chunks * kSlot;
+    CUDA_CHECK(cudaMallocAsync((void**)&a.image, image + (size_t)xt * N * sizeof(int), st));
+    a.powers = reinterpret_cast<int*>(a.image + image);
+    try {
+        client_smem<k_q4_gemm<N, KC, XT>>(cx);
+        k_q4_pack<N, KC, XT><<<xt * N, 128, 0, st>>>(a);
+        CUDA_CHECK(cudaGetLastError());
+        launch_pdl(cx, k_q4_gemm<N, KC, XT>, dim3((a.w.rows + a.block_rows - 1) / a.block_rows, xt), dim3(kQgThreads), smem, st, a,
+                   cx.d_err);
+    } catch (...) {
+        cudaFreeAsync(a.image, st);
+        throw;
+    }
+    CUDA_CHECK(cudaFreeAsync(a.image, st));
+    cx.launches += 2;
+}
+template <int N, class XT>
+static void q4_gemm_group(Context& cx, const QgArgs& a, cudaStream_t st) {
+    if (a.w.group % 64 == 0) q4_gemm_launch<N, 64, XT>(cx, a, st);
+    else q4_gemm_launch<N, 32, XT>(cx, a, st);
+}
+template <class XT>
+static void q4_gemm(Context& cx, const QgArgs& a, cudaStream_t st) {
+    if (a.m <= 16) q4_gemm_group<16, XT>(cx, a, st);
+    else if (a.m <= 32) q4_gemm_group<32, XT>(cx, a, st);
+    else q4_gemm_group<64, XT>(cx, a, st);
+}
+
 static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
-    a.terms = a.xt == FHE_F32 ? 3 : a.xt == FHE_F16 ? 2 : 1;
     const long long row = a.ldx * (a.xt == FHE_F32 ? 4 : 2);
     a.wide = (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(a.m > 1 ? row : 0)) % 16 == 0;
+    a.terms = a.xt == FHE_F32 ? 3 : a.xt == FHE_F16 ? 2 : 1;
+    static const int lim = getenv("QGMIN") ? atoi(getenv("QGMIN")) : 9;
+    if (a.m >= lim) {
+        const QgArgs q{a.w, a.x, a.m, a.ldx, a.out, a.ot, a.ldo, a.wide, 0, 0, 0, 0, 0, nullptr, nullptr};
+        if (a.xt == FHE_F32) q4_gemm<float>(cx, q, st);
+        else if (a.xt == FHE_F16) q4_gemm<__half>(cx, q, st);
+        else q4_gemm<__nv_bfloat16>(cx, q, st);
+        return;
+    }
     const int cols = a.m * a.terms;
     if (cols <= 8) q4_mma_split<1>(cx, a, st);
     else if (cols <= 16) q4_mma_split<2>(cx, a, st);

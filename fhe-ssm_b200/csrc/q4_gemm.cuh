@@ -1,0 +1,497 @@
+// q4_gemm.cuh -- products of several rows with a 4-bit table on the 5th-generation tensor cores (tcgen05).
+//
+//     out[r][i] = sum_g s[i][g] sum_{c in g} (q[i][c] - 8) x[r][c]
+//
+// The inner sum is a 16-bit tensor-core product of whole numbers with x; the scale is applied to it in float32, as it
+// leaves tensor memory.  So nothing is rounded before the float32 sums but a float32 x, which is carried as two float16
+// pieces of 11 bits (scaled by a power of two of the row's maximum); float16 and bfloat16 are taken as they are.
+//
+// k_q4_pack writes x's operand as the shared-memory image of its chunks of columns; k_q4_gemm starts while it runs
+// (programmatic dependent launch) and waits for it where it first loads the image.
+//
+// Per block of k_q4_gemm: up to 4 tiles of 128 table rows (lanes of tensor memory) x N rows of x (its columns).  Roles:
+//   warps 0-7    drain: accumulators of a chunk of columns -> registers, times the rows' scales; output
+//   warps 8-15   two groups in turn: table bytes (cp.async ring) -> 16-bit operands in tensor memory
+//   warp 16      issues the products
+//   warp 17      loads x's chunks (bulk copies)
+//   warps 18-19  scales -> shared memory, a tile ahead of the drain
+// The table operand goes to tensor memory and not to shared memory, whose bandwidth the products would then share with
+// its writes: 16 KB written and 16 KB a piece read for each 128 x 64 tile, four times the time of the product itself.
+// x's operand stays in shared memory for as many columns as fit (a range); the tiles pass over it one after the other, and
+// between ranges a tile's sums wait in tensor memory, so the drain needs registers for one tile only.
+//
+// Included by client.cu inside namespace fhe.
+
+constexpr int kQgThreads = 640;
+constexpr int kQgRowsMax = 512;               // table rows of a block
+constexpr int kQgStages = 4;                  // 128 rows x 128 columns of table bytes each, for each group
+constexpr int kQgStageBytes = 128 * 64;
+constexpr int kQgAMax = 8, kQgDMax = 4;       // operand and accumulator slots in tensor memory
+constexpr int kQgSlotsMax = 16;               // chunks of x's operand
+constexpr int kQgXBytes = 131072;             // shared memory for them
+constexpr uint32_t kQgACol = 384;             // tensor memory: tiles' sums (several ranges only), accumulators, operands
+// A wait sleeps up to this long at a time (ns), at most so often: about a second.  Waits that poll instead take the issue slots of
+// the warps that work.
+constexpr int kQgSleep = 20000, kQgWaits = 1 << 16;
+
+struct QgBars {
+    uint64_t a_full[kQgAMax], a_empty[kQgAMax], d_full[kQgDMax], d_empty[kQgDMax], x_full[kQgSlotsMax], x_empty[kQgSlotsMax],
+        s_full[2], s_empty[2], end;
+    uint32_t tmem;
+    int dead;      // a wait ran out: nobody waits any more, the output is NaN
+};
+
+struct QgArgs {
+    fhe_q4 w;
+    const void* x;
+    int m;
+    long long ldx;
+    void* out;
+    int ot;
+    long long ldo;
+    int wide;         // rows of x start on 16-byte boundaries
+    int block_rows;   // table rows of a block
+    int slots;        // chunks of a range
+    int chunks;       // chunks of all columns, a multiple of a job's (128 columns)
+    int groups;       // most groups that a range meets
+    int run;          // chunks that one accumulator takes before the scale is applied
+    uint8_t* image;   // x's operand [tile of N rows][chunk][piece], then the rows' powers of two
+    int* powers;
+};
+
+__device__ __forceinline__ void qg_init(uint64_t* bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(tc_smem(bar)), "r"(count));
+}
+__device__ __forceinline__ void qg_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc_smem(bar)) : "memory");
+}
+__device__ __forceinline__ void qg_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tc_smem(bar)) : "memory");
+}
+__device__ __forceinline__ bool qg_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(tc_smem(bar)), "r"(parity), "r"(kQgSleep)
+        : "memory");
+    return ok;
+}
+// Waits until the phase of the given parity has passed; after a wait that ran out, anywhere in the block, it does not wait
+__device__ __forceinline__ void qg_wait(uint64_t* bar, uint32_t parity, QgBars* b) {
+    if (qg_try(bar, parity)) return;
+    for (int it = 0; it < kQgWaits; it++)
+        if (qg_try(bar, parity) || *(volatile int*)&b->dead) return;
+    *(volatile int*)&b->dead = 1;
+}
+
+// kind::f16, D float32, both operands of one type (0 float16, 1 bfloat16) and K-major, M = 128, N = n
+__device__ constexpr uint32_t qg_idesc(int n, int type) {
+    return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void qg_mma(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0), "r"(0), "r"(0), "r"(0));
+}
+
+#define QG_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define QG_W8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+// CNT columns of the warp's 32 lanes
+template <int CNT>
+__device__ __forceinline__ void qg_ld(uint32_t t, uint32_t* v) {
+    if constexpr (CNT == 32)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+            : QG_R8(v, 0), QG_R8(v, 8), QG_R8(v, 16), QG_R8(v, 24)
+            : "r"(t));
+    else if constexpr (CNT == 16)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : QG_R8(v, 0), QG_R8(v, 8)
+            : "r"(t));
+    else
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : QG_R8(v, 0) : "r"(t));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+template <int CNT>
+__device__ __forceinline__ void qg_st(uint32_t t, const uint32_t* v) {
+    if constexpr (CNT == 32)
+        asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(t),
+            QG_W8(v, 0), QG_W8(v, 8), QG_W8(v, 16), QG_W8(v, 24)
+            : "memory");
+    else if constexpr (CNT == 16)
+        asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+            "%16};" ::"r"(t),
+            QG_W8(v, 0), QG_W8(v, 8)
+            : "memory");
+    else
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(t), QG_W8(v, 0)
+                     : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// 8 values of 4 bits -> pairs (0,4), (1,5), (2,6), (3,7) of q - 8
+template <class H>
+__device__ __forceinline__ void qg_unpack(uint32_t w, uint32_t* p) {
+    if constexpr (std::is_same<H, __half>::value) {
+        // 0x6400 is 1024, whose last bits count in ones: 1024 + q, or 1024 + 16 q from the high half of a byte
+        const __half2 off = __float2half2_rn(1032.f), by = __float2half2_rn(0.0625f), low = __float2half2_rn(-72.f);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const uint32_t a = (w & 0x000f000fu) | 0x64006400u, b = (w & 0x00f000f0u) | 0x64006400u;
+            const __half2 u = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+            const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&b), by, low);
+            p[i] = *reinterpret_cast<const uint32_t*>(&u);
+            p[i + 1] = *reinterpret_cast<const uint32_t*>(&v);
+            w >>= 8;
+        }
+    } else {
+        q4_unpack(w, p);
+    }
+}
+
+template <int KC>
+__host__ __device__ constexpr uint32_t qg_sbo() { return KC / 8 * 128; }   // bytes of 8 rows of a chunk of x's operand
+
+// x -> operand image.  One block per row; a thread takes 8 columns, in the order of qg_unpack's pairs.
+template <int N, int KC, class XT>
+__global__ void __launch_bounds__(128) k_q4_pack(const QgArgs a) {
+    constexpr bool kF32 = std::is_same<XT, float>::value;
+    using H = typename std::conditional<std::is_same<XT, __nv_bfloat16>::value, __nv_bfloat16, __half>::type;
+    constexpr int kPieces = kF32 ? 2 : 1, kPieceBytes = N * KC * 2;
+    pdl_trigger();
+    const int r = blockIdx.x, n = r % N, units = a.chunks * (KC / 8);
+    uint8_t* to = a.image + (size_t)(r / N) * a.chunks * kPieces * kPieceBytes + (n >> 3) * qg_sbo<KC>() + (n & 7) * 16;
+    const auto load = [&](int u, XT* v) {
+        const int k = u * 8;
+        const XT* src = static_cast<const XT*>(a.x) + r * a.ldx + k;
+        if (r < a.m && a.wide && k + 8 <= a.w.cols) {
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(XT) / 2; j++) reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(src)[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = r < a.m && k + j < a.w.cols ? src[j] : XT(0.f);
+        }
+    };
+    const auto pair = [](H x, H y) {
+        return (uint32_t)*reinterpret_cast<const uint16_t*>(&x) | (uint32_t)*reinterpret_cast<const uint16_t*>(&y) << 16;
+    };
+    __align__(16) XT v[8];
+    load(threadIdx.x, v);
+    float up = 1.f;
+    if constexpr (kF32) {
+        // the row's largest finite magnitude maps to 2^14 .. 2^15; a value under 2^-16 of it is held to 2^-39 of it
+        uint32_t most = 0;
+        const auto see = [&](const XT* u) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t bits = __float_as_uint(u[j]) & 0x7fffffffu;
+                most = max(most, bits < 0x7f800000u ? bits : 0u);
+            }
+        };
+        see(v);
+        for (int u = threadIdx.x + 128; u < units; u += 128) {
+            __align__(16) XT w[8];
+            load(u, w);
+            see(w);
+        }
+        __shared__ uint32_t sm[4];
+        most = __reduce_max_sync(0xffffffffu, most);
+        if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = most;
+        __syncthreads();
+        const int e = max(14, (int)(max(max(sm[0], sm[1]), max(sm[2], sm[3])) >> 23));
+        up = __uint_as_float((uint32_t)(268 - e) << 23);
+        if (threadIdx.x == 0) a.powers[r] = e - 141;
+    }
+    for (int u = threadIdx.x; u < units; u += 128) {
+        if (u != threadIdx.x) load(u, v);
+        uint8_t* dst = to + (size_t)(u / (KC / 8)) * kPieces * kPieceBytes + u % (KC / 8) * 128;
+        H h[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if constexpr (kF32) h[j] = __float2half_rn(v[j] * up);
+            else h[j] = v[j];
+        }
+        *reinterpret_cast<uint4*>(dst) = make_uint4(pair(h[0], h[4]), pair(h[1], h[5]), pair(h[2], h[6]), pair(h[3], h[7]));
+        if constexpr (kF32) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                // what the first piece leaves; an infinity or NaN is all in the first
+                const float f = __half2float(h[j]), rest = v[j] * up - f;
+                h[j] = __float2half_rn(fabsf(f) < INFINITY ? rest : 0.f);
+            }
+            *reinterpret_cast<uint4*>(dst + kPieceBytes) =
+                make_uint4(pair(h[0], h[4]), pair(h[1], h[5]), pair(h[2], h[6]), pair(h[3], h[7]));
+        }
+    }
+}
+
+// N rows of x (16, 32 or 64), KC columns a chunk (64, or 32 where the group is no multiple of 64), XT: x's type
+template <int N, int KC, class XT>
+__global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsigned int* err) {
+    constexpr bool kF32 = std::is_same<XT, float>::value, kBf = std::is_same<XT, __nv_bfloat16>::value;
+    using H = typename std::conditional<kBf, __nv_bfloat16, __half>::type;
+    constexpr int kPieces = kF32 ? 2 : 1;
+    constexpr int kItems = 128 / KC;                    // chunks of a job
+    // 128 columns of operand slots: two jobs, so that a slot is always filled by the same of the two groups, which cannot get
+    // further ahead of it than the one phase that a parity tells
+    constexpr int kQgA = 2 * kItems;
+    constexpr int kPieceBytes = N * KC * 2, kSlotBytes = kPieceBytes * kPieces;
+    extern __shared__ __align__(1024) uint8_t gsm[];
+    uint8_t* ring = gsm;
+    uint8_t* xs = gsm + 2 * kQgStages * kQgStageBytes;
+    float* scales = reinterpret_cast<float*>(xs + (size_t)a.slots * kSlotBytes);   // [2][group of the range][128 rows]
+    QgBars* bars = reinterpret_cast<QgBars*>(scales + 2 * a.groups * 128);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int row0 = blockIdx.x * a.block_rows, row1 = min(a.w.rows, row0 + a.block_rows), tiles = (row1 - row0 + 127) / 128;
+    const int x0 = blockIdx.y * N;
+    const int ranges = (a.chunks + a.slots - 1) / a.slots;
+    const auto range_chunks = [&](int kr) { return min(a.slots, a.chunks - kr * a.slots); };
+    const uint32_t dcol = ranges > 1 ? tiles * N : 0, nd = min((uint32_t)kQgDMax, (kQgACol - dcol) / N);
+
+    if (tid == 0) {
+        for (int i = 0; i < kQgA; i++) qg_init(&bars->a_full[i], 4), qg_init(&bars->a_empty[i], 1);
+        for (int i = 0; i < kQgDMax; i++) qg_init(&bars->d_full[i], 1), qg_init(&bars->d_empty[i], 8);
+        for (int i = 0; i < a.slots; i++) qg_init(&bars->x_full[i], 1), qg_init(&bars->x_empty[i], 1);
+        for (int i = 0; i < 2; i++) qg_init(&bars->s_full[i], 64), qg_init(&bars->s_empty[i], 8);
+        qg_init(&bars->end, 1);
+        bars->dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;");
+    }
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc_smem(&bars->tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    const uint32_t tm = bars->tmem, lanes = (uint32_t)(32 * (warp & 3)) << 16;
+
+    if (warp < 8) {
+        // ---- drain: row = lane of the tile, half of the columns
+        constexpr int kC = N / 2;
+        const int half = warp >> 2, per_group = a.w.group / (KC * a.run);
+        uint32_t slot = 0, phase = 0, tile = 0;
+        for (int kr = 0; kr < ranges; kr++) {
+            const int drains = range_chunks(kr) / a.run;
+            for (int b = 0; b < tiles; b++, tile++) {
+                const int row = row0 + b * 128 + (warp & 3) * 32 + lane;
+                int left = per_group - kr * a.slots / a.run % per_group;
+                const float* sp = scales + (tile & 1) * a.groups * 128 + (warp & 3) * 32 + lane;
+                qg_wait(&bars->s_full[tile & 1], tile >> 1 & 1, bars);
+                float acc[kC];
+#pragma unroll
+                for (int j = 0; j < kC; j++) acc[j] = 0.f;
+                for (int c = 0; c < drains; c++) {
+                    const float s = *sp;
+                    if (--left == 0) left = per_group, sp += 128;
+                    qg_wait(&bars->d_full[slot], phase, bars);
+                    __syncwarp();
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    uint32_t v[kC];
+                    qg_ld<kC>(tm + dcol + slot * N + half * kC + lanes, v);
+                    asm volatile("tcgen05.fence::before_thread_sync;");
+                    __syncwarp();
+                    if (lane == 0) qg_arrive(&bars->d_empty[slot]);
+#pragma unroll
+                    for (int j = 0; j < kC; j++) acc[j] = fmaf(s, __uint_as_float(v[j]), acc[j]);
+                    if (++slot == nd) slot = 0, phase ^= 1;
+                }
+                __syncwarp();
+                if (lane == 0) qg_arrive(&bars->s_empty[tile & 1]);
+                const uint32_t keep = tm + b * N + half * kC + lanes;
+                if (kr) {
+                    uint32_t v[kC];
+                    qg_ld<kC>(keep, v);
+#pragma unroll
+                    for (int j = 0; j < kC; j++) acc[j] += __uint_as_float(v[j]);
+                }
+                if (kr + 1 < ranges) {
+                    qg_st<kC>(keep, reinterpret_cast<const uint32_t*>(acc));
+                    continue;
+                }
+                if (*(volatile int*)&bars->dead) {
+#pragma unroll
+                    for (int j = 0; j < kC; j++) acc[j] = __int_as_float(0x7fffffff);
+                }
+                const int r0 = x0 + half * kC, nr = min(kC, a.m - r0);
+                if (kF32 && nr > 0) {
+                    pdl_wait();
+#pragma unroll
+                    for (int j = 0; j < kC; j++) {
+                        // 2^p in two factors, either of which float32 has
+                        const int p = j < nr ? a.powers[r0 + j] : 0;
+                        acc[j] = acc[j] * __uint_as_float((uint32_t)(127 + (p >> 1)) << 23) * __uint_as_float((uint32_t)(127 + p - (p >> 1)) << 23);
+                    }
+                }
+                if (row >= row1) continue;
+                const auto store = [&](auto* out) {
+                    out += r0 * a.ldo + row;
+#pragma unroll
+                    for (int j = 0; j < kC; j++, out += a.ldo)
+                        if (j < nr) st_any(out, sizeof(*out) == 4 ? FHE_F32 : std::is_same<decltype(out), __half*>::value ? FHE_F16 : FHE_BF16, 0, acc[j]);
+                };
+                if (a.ot == FHE_F32) store(static_cast<float*>(a.out));
+                else if (a.ot == FHE_F16) store(static_cast<__half*>(a.out));
+                else store(static_cast<__nv_bfloat16*>(a.out));
+            }
+        }
+    } else if (warp < 16) {
+        // ---- the table: jobs of 128 rows x 128 columns, every second one
+        const int grp = (warp >> 2) - 2, t = tid & 127;
+        uint8_t* my = ring + grp * kQgStages * kQgStageBytes;
+        const int units = (a.w.cols + 31) / 32;   // 16-byte units of a row
+        int jobs = 0;
+        for (int kr = 0; kr < ranges; kr++) jobs += tiles * (range_chunks(kr) / kItems);
+        int fkr = 0, fb = 0, fc = grp;   // the job to fetch next
+        const auto fetch = [&](int s) {
+            while (fkr < ranges) {
+                const int n = range_chunks(fkr) / kItems;
+                if (fc < n) break;
+                fc -= n;
+                if (++fb == tiles) fb = 0, fkr++;
+            }
+            if (fkr < ranges) {
+                const int unit = (fkr * a.slots / kItems + fc) * 4 + (t & 3);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int r = (t >> 2) + 32 * i, row = row0 + fb * 128 + r;
+                    if (row < row1 && unit < units) {
+                        const uint32_t dst = tc_smem(my + (s % kQgStages) * kQgStageBytes + r * 64 + (((t & 3) ^ (r >> 1 & 3)) << 4));
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst),
+                                     "l"(a.w.q + row * a.w.ldq + unit * 16ll)
+                                     : "memory");
+                    }
+                }
+                fc += 2;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int s = 0; s < kQgStages - 1; s++) fetch(s);
+        for (int j = grp, s = 0; j < jobs; j += 2, s++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kQgStages - 2) : "memory");
+            // all copies of the stage are there; the one before it is read
+            if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+            else asm volatile("bar.sync 2, 128;" ::: "memory");
+            fetch(s + kQgStages - 1);
+            const uint8_t* st = my + (s % kQgStages) * kQgStageBytes + t * 64;
+#pragma unroll
+            for (int h = 0; h < kItems; h++) {
+                uint32_t v[KC / 2];
+#pragma unroll
+                for (int q = 0; q < KC / 32; q++) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(st + (((h * (KC / 32) + q) ^ (t >> 1 & 3)) << 4));
+                    qg_unpack<H>(u.x, v + q * 16);
+                    qg_unpack<H>(u.y, v + q * 16 + 4);
+                    qg_unpack<H>(u.z, v + q * 16 + 8);
+                    qg_unpack<H>(u.w, v + q * 16 + 12);
+                }
+                const uint32_t i = grp * kItems + h;   // the slot: a group's own, a job on in each phase
+                qg_wait(&bars->a_empty[i], (s & 1) ^ 1, bars);
+                __syncwarp();
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                qg_st<KC / 2>(tm + kQgACol + i * (KC / 2) + lanes, v);
+                asm volatile("tcgen05.fence::before_thread_sync;");
+                __syncwarp();
+                if (lane == 0) qg_arrive(&bars->a_full[i]);
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == 16) {
+        // ---- products: one lane issues them, the warp stays together
+        constexpr uint32_t idesc = qg_idesc(N, kBf ? 1 : 0);
+        uint32_t elected;
+        asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(elected));
+        const uint32_t base = __reduce_or_sync(0xffffffffu, tm);   // the same in all lanes, as the compiler now sees
+        const uint64_t xdesc = tc_desc(tc_smem(xs), 128, qg_sbo<KC>());
+        uint32_t i = 0, aphase = 0, slot = 0, dphase = 1, in_run = 0;
+        for (int kr = 0; kr < ranges; kr++) {
+            const int nch = range_chunks(kr);
+            for (int b = 0; b < tiles; b++)
+                for (int c = 0; c < nch; c++) {
+                    if (b == 0) qg_wait(&bars->x_full[c], kr & 1, bars);
+                    qg_wait(&bars->a_full[i], aphase, bars);
+                    if (in_run == 0) qg_wait(&bars->d_empty[slot], dphase, bars);
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    const uint32_t at = base + kQgACol + i * (KC / 2), dt = base + dcol + slot * N;
+                    const uint64_t xd = xdesc + (uint32_t)(c * kSlotBytes >> 4);
+                    const bool last = in_run + 1 == a.run;
+                    if (elected) {
+#pragma unroll
+                        for (int p = 0; p < kPieces; p++)
+#pragma unroll
+                            for (int ks = 0; ks < KC / 16; ks++)
+                                qg_mma(dt, at + ks * 8, xd + ((p * kPieceBytes + ks * 256) >> 4), idesc, p + ks > 0 ? 1u : in_run);
+                        qg_commit(&bars->a_empty[i]);
+                        if (b == tiles - 1) qg_commit(&bars->x_empty[c]);
+                        if (last) qg_commit(&bars->d_full[slot]);
+                    }
+                    __syncwarp();
+                    if (++i == kQgA) i = 0, aphase ^= 1;
+                    if (last && ++slot == nd) slot = 0, dphase ^= 1;
+                    in_run = last ? 0 : in_run + 1;
+                }
+        }
+        if (elected) {
+            qg_commit(&bars->end);   // all products, before tensor memory is given back
+            for (int it = 0; it < kQgWaits && !qg_try(&bars->end, 0); it++) {}
+        }
+        __syncwarp();
+    } else if (warp == 17) {
+        // ---- x
+        if (lane == 0) {
+            pdl_wait();
+            const uint8_t* src = a.image + (size_t)blockIdx.y * a.chunks * kSlotBytes;
+            for (int ch = 0, c = 0, kr = 0; ch < a.chunks; ch++) {
+                if (kr) qg_wait(&bars->x_empty[c], (kr - 1) & 1, bars);
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(&bars->x_full[c])), "r"(kSlotBytes)
+                             : "memory");
+                tc_bulk_g2s(xs + (size_t)c * kSlotBytes, src + (size_t)ch * kSlotBytes, kSlotBytes, &bars->x_full[c]);
+                if (++c == a.slots) c = 0, kr++;
+            }
+            // the last copies, if nobody else has waited for them
+            const int left = range_chunks(ranges - 1);
+            for (int c = 0; c < left; c++)
+                for (int it = 0; it < kQgWaits && !qg_try(&bars->x_full[c], (ranges - 1) & 1); it++) {}
+        }
+        __syncwarp();
+    } else {
+        // ---- scales: 0 past the last column's group
+        const int t = tid - 18 * 32, groups = (a.w.cols + a.w.group - 1) / a.w.group;
+        uint32_t tile = 0;
+        const auto fill = [&](auto* src) {
+            for (int kr = 0; kr < ranges; kr++) {
+                const int first = kr * a.slots * KC / a.w.group;
+                for (int b = 0; b < tiles; b++, tile++) {
+                    float* to = scales + (tile & 1) * a.groups * 128;
+                    if (tile > 1) qg_wait(&bars->s_empty[tile & 1], (tile >> 1 & 1) ^ 1, bars);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const auto* p = src + min(row0 + b * 128 + t + h * 64, a.w.rows - 1) * a.w.lds + first;
+#pragma unroll 8
+                        for (int g = 0; g < a.groups; g++)
+                            to[g * 128 + t + h * 64] = first + g < groups ? q4_float(p[g]) : 0.f;
+                    }
+                    qg_arrive(&bars->s_full[tile & 1]);
+                }
+            }
+        };
+        if (a.w.scale_type == FHE_F32) fill(static_cast<const float*>(a.w.scale));
+        else if (a.w.scale_type == FHE_F16) fill(static_cast<const __half*>(a.w.scale));
+        else fill(static_cast<const __nv_bfloat16*>(a.w.scale));
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    __syncthreads();
+    if (tid == 0 && bars->dead) atomicExch(err, 1u);
+    if (warp == 16) {
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512));
+    }
+}

@@ -58,6 +58,7 @@ def check_product(got, x, w, ot):
     (32, 640, 1024, 64, "f32", "f16", "bf16"), (33, 385, 2050, 128, "f32", "f16", "f32"),
     (48, 200, 200, 1024, "f16", "f16", "f16"), (63, 129, 999, 160, "f32", "bf16", "f32"),
     (64, 4099, 1024, 64, "f32", "f16", "f32"), (64, 300, 4096, 32, "bf16", "f16", "f32"),
+    (24, 50304, 1024, 32, "f32", "f16", "f32"), (64, 20000, 2048, 96, "bf16", "f16", "f32"),
     (65, 130, 320, 64, "f32", "f16", "f32"), (130, 77, 161, 32, "bf16", "f32", "f32"),
     (200, 1000, 128, 128, "f16", "f16", "f32")])
 def test_matvec(cx, m, rows, cols, group, xt, st, ot):
