@@ -307,15 +307,15 @@ static void q4_mma_split(Context& cx, const Q4Args& a, cudaStream_t st) {
 
 template <int N, int KC, class XT>
 static void q4_gemm_launch(Context& cx, QgArgs a, cudaStream_t st) {
-    constexpr int kSlot = N * KC * 2 * (std::is_same<XT, float>::value ? 2 : 1), kJob = 128 / KC;
+    constexpr int kSlot = N * 256 * (std::is_same<XT, float>::value ? 2 : 1);   // a job's 128 columns of x
     const int waves = (a.w.rows + 148 * kQgRowsMax - 1) / (148 * kQgRowsMax), xt = (a.m + N - 1) / N;
     a.block_rows = std::min(kQgRowsMax, ((a.w.rows + 148 * waves - 1) / (148 * waves) + 31) / 32 * 32);
-    a.chunks = (a.w.cols + 127) / 128 * kJob;
-    a.slots = std::min({kQgSlotsMax, kQgXBytes / kSlot, a.chunks});
-    a.groups = std::min((a.slots * KC + a.w.group - 2) / a.w.group + 1, (a.w.cols + a.w.group - 1) / a.w.group + 1);
+    a.jobs = (a.w.cols + 127) / 128;
+    a.slots = std::min({kQgSlotsMax, kQgXBytes / kSlot, a.jobs});
+    a.groups = std::min((a.slots * 128 + a.w.group - 2) / a.w.group + 1, (a.w.cols + a.w.group - 1) / a.w.group + 1);
     a.run = KC == 64 && a.w.group % 128 == 0 ? 2 : 1;
     const size_t smem = 2 * kQgStages * kQgStageBytes + (size_t)a.slots * kSlot + (size_t)a.groups * 1024 + sizeof(QgBars);
-    const size_t image = (size_t)xt * a.chunks * kSlot;
+    const size_t image = (size_t)xt * a.jobs * kSlot;
     CUDA_CHECK(cudaMallocAsync((void**)&a.image, image + (size_t)xt * N * sizeof(int), st));
     a.powers = reinterpret_cast<int*>(a.image + image);
     try {

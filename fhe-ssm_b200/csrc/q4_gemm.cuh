@@ -26,13 +26,13 @@ constexpr int kQgThreads = 640;
 constexpr int kQgRowsMax = 512;               // table rows of a block
 constexpr int kQgStages = 4;                  // 128 rows x 128 columns of table bytes each, for each group
 constexpr int kQgStageBytes = 128 * 64;
-constexpr int kQgAMax = 8, kQgDMax = 4;       // operand and accumulator slots in tensor memory
-constexpr int kQgSlotsMax = 16;               // chunks of x's operand
+constexpr int kQgAMax = 4, kQgDMax = 4;       // operand (a job each) and accumulator (a chunk each) slots in tensor memory
+constexpr int kQgSlotsMax = 8;                // jobs of x's operand
 constexpr int kQgXBytes = 131072;             // shared memory for them
-constexpr uint32_t kQgACol = 384;             // tensor memory: tiles' sums (several ranges only), accumulators, operands
-// A wait sleeps up to this long at a time (ns), at most so often: about a second.  Waits that poll instead take the issue slots of
-// the warps that work.
-constexpr int kQgSleep = 20000, kQgWaits = 1 << 16;
+// A wait that has nothing to wait for costs 110 cycles, a commit 46 (measured alone), so they are few: operands change hands by
+// the job of 128 columns, and one wait of the products' warp sees to several barriers, a lane each.  (Waits with a sleep
+// time as a hint wake later: the whole kernel took 1.3 times as long with 20 us.)
+constexpr int kQgWaits = 1 << 22;             // bounded: some seconds
 
 struct QgBars {
     uint64_t a_full[kQgAMax], a_empty[kQgAMax], d_full[kQgDMax], d_empty[kQgDMax], x_full[kQgSlotsMax], x_empty[kQgSlotsMax],
@@ -51,8 +51,8 @@ struct QgArgs {
     long long ldo;
     int wide;         // rows of x start on 16-byte boundaries
     int block_rows;   // table rows of a block
-    int slots;        // chunks of a range
-    int chunks;       // chunks of all columns, a multiple of a job's (128 columns)
+    int slots;        // jobs of a range
+    int jobs;         // jobs of all columns, 128 each
     int groups;       // most groups that a range meets
     int run;          // chunks that one accumulator takes before the scale is applied
     uint8_t* image;   // x's operand [tile of N rows][chunk][piece], then the rows' powers of two
@@ -71,9 +71,9 @@ __device__ __forceinline__ void qg_commit(uint64_t* bar) {
 __device__ __forceinline__ bool qg_try(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
         : "=r"(ok)
-        : "r"(tc_smem(bar)), "r"(parity), "r"(kQgSleep)
+        : "r"(tc_smem(bar)), "r"(parity)
         : "memory");
     return ok;
 }
@@ -133,7 +133,6 @@ __device__ __forceinline__ void qg_st(uint32_t t, const uint32_t* v) {
     else
         asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(t), QG_W8(v, 0)
                      : "memory");
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // 8 values of 4 bits -> pairs (0,4), (1,5), (2,6), (3,7) of q - 8
@@ -166,8 +165,8 @@ __global__ void __launch_bounds__(128) k_q4_pack(const QgArgs a) {
     using H = typename std::conditional<std::is_same<XT, __nv_bfloat16>::value, __nv_bfloat16, __half>::type;
     constexpr int kPieces = kF32 ? 2 : 1, kPieceBytes = N * KC * 2;
     pdl_trigger();
-    const int r = blockIdx.x, n = r % N, units = a.chunks * (KC / 8);
-    uint8_t* to = a.image + (size_t)(r / N) * a.chunks * kPieces * kPieceBytes + (n >> 3) * qg_sbo<KC>() + (n & 7) * 16;
+    const int r = blockIdx.x, n = r % N, units = a.jobs * 16;
+    uint8_t* to = a.image + (size_t)(r / N) * a.jobs * (128 / KC) * kPieces * kPieceBytes + (n >> 3) * qg_sbo<KC>() + (n & 7) * 16;
     const auto load = [&](int u, XT* v) {
         const int k = u * 8;
         const XT* src = static_cast<const XT*>(a.x) + r * a.ldx + k;
@@ -239,10 +238,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
     using H = typename std::conditional<kBf, __nv_bfloat16, __half>::type;
     constexpr int kPieces = kF32 ? 2 : 1;
     constexpr int kItems = 128 / KC;                    // chunks of a job
-    // 128 columns of operand slots: two jobs, so that a slot is always filled by the same of the two groups, which cannot get
-    // further ahead of it than the one phase that a parity tells
-    constexpr int kQgA = 2 * kItems;
-    constexpr int kPieceBytes = N * KC * 2, kSlotBytes = kPieceBytes * kPieces;
+    constexpr int kPieceBytes = N * KC * 2, kChunkBytes = kPieceBytes * kPieces, kSlotBytes = kChunkBytes * kItems;
     extern __shared__ __align__(1024) uint8_t gsm[];
     uint8_t* ring = gsm;
     uint8_t* xs = gsm + 2 * kQgStages * kQgStageBytes;
@@ -251,12 +247,15 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row0 = blockIdx.x * a.block_rows, row1 = min(a.w.rows, row0 + a.block_rows), tiles = (row1 - row0 + 127) / 128;
     const int x0 = blockIdx.y * N;
-    const int ranges = (a.chunks + a.slots - 1) / a.slots;
-    const auto range_chunks = [&](int kr) { return min(a.slots, a.chunks - kr * a.slots); };
-    const uint32_t dcol = ranges > 1 ? tiles * N : 0, nd = min((uint32_t)kQgDMax, (kQgACol - dcol) / N);
+    const int ranges = (a.jobs + a.slots - 1) / a.slots;
+    const auto range_jobs = [&](int kr) { return min(a.slots, a.jobs - kr * a.slots); };
+    // tensor memory: the tiles' sums (several ranges only), accumulators, operands.  Two or four operand slots: a slot is
+    // always filled by the same of the two groups, which so cannot get more than the one phase that a parity tells ahead of it.
+    const uint32_t dcol = ranges > 1 ? tiles * N : 0, nd = min((uint32_t)kQgDMax, (384 - dcol) / N), acol = dcol + nd * N;
+    const int na = acol <= 256 ? 4 : 2;
 
     if (tid == 0) {
-        for (int i = 0; i < kQgA; i++) qg_init(&bars->a_full[i], 4), qg_init(&bars->a_empty[i], 1);
+        for (int i = 0; i < kQgAMax; i++) qg_init(&bars->a_full[i], 4), qg_init(&bars->a_empty[i], 1);
         for (int i = 0; i < kQgDMax; i++) qg_init(&bars->d_full[i], 1), qg_init(&bars->d_empty[i], 8);
         for (int i = 0; i < a.slots; i++) qg_init(&bars->x_full[i], 1), qg_init(&bars->x_empty[i], 1);
         for (int i = 0; i < 2; i++) qg_init(&bars->s_full[i], 64), qg_init(&bars->s_empty[i], 8);
@@ -279,10 +278,10 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         const int half = warp >> 2, per_group = a.w.group / (KC * a.run);
         uint32_t slot = 0, phase = 0, tile = 0;
         for (int kr = 0; kr < ranges; kr++) {
-            const int drains = range_chunks(kr) / a.run;
+            const int drains = range_jobs(kr) * kItems / a.run;
             for (int b = 0; b < tiles; b++, tile++) {
                 const int row = row0 + b * 128 + (warp & 3) * 32 + lane;
-                int left = per_group - kr * a.slots / a.run % per_group;
+                int left = per_group - kr * a.slots * kItems / a.run % per_group;
                 const float* sp = scales + (tile & 1) * a.groups * 128 + (warp & 3) * 32 + lane;
                 qg_wait(&bars->s_full[tile & 1], tile >> 1 & 1, bars);
                 float acc[kC];
@@ -314,6 +313,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                 }
                 if (kr + 1 < ranges) {
                     qg_st<kC>(keep, reinterpret_cast<const uint32_t*>(acc));
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     continue;
                 }
                 if (*(volatile int*)&bars->dead) {
@@ -347,18 +347,17 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         const int grp = (warp >> 2) - 2, t = tid & 127;
         uint8_t* my = ring + grp * kQgStages * kQgStageBytes;
         const int units = (a.w.cols + 31) / 32;   // 16-byte units of a row
-        int jobs = 0;
-        for (int kr = 0; kr < ranges; kr++) jobs += tiles * (range_chunks(kr) / kItems);
+        const int jobs = tiles * a.jobs;
         int fkr = 0, fb = 0, fc = grp;   // the job to fetch next
         const auto fetch = [&](int s) {
             while (fkr < ranges) {
-                const int n = range_chunks(fkr) / kItems;
+                const int n = range_jobs(fkr);
                 if (fc < n) break;
                 fc -= n;
                 if (++fb == tiles) fb = 0, fkr++;
             }
             if (fkr < ranges) {
-                const int unit = (fkr * a.slots / kItems + fc) * 4 + (t & 3);
+                const int unit = (fkr * a.slots + fc) * 4 + (t & 3);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int r = (t >> 2) + 32 * i, row = row0 + fb * 128 + r;
@@ -375,6 +374,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         };
 #pragma unroll
         for (int s = 0; s < kQgStages - 1; s++) fetch(s);
+        uint32_t slot = grp, phase = 1;
         for (int j = grp, s = 0; j < jobs; j += 2, s++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kQgStages - 2) : "memory");
             // all copies of the stage are there; the one before it is read
@@ -393,15 +393,18 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                     qg_unpack<H>(u.z, v + q * 16 + 8);
                     qg_unpack<H>(u.w, v + q * 16 + 12);
                 }
-                const uint32_t i = grp * kItems + h;   // the slot: a group's own, a job on in each phase
-                qg_wait(&bars->a_empty[i], (s & 1) ^ 1, bars);
-                __syncwarp();
-                asm volatile("tcgen05.fence::after_thread_sync;");
-                qg_st<KC / 2>(tm + kQgACol + i * (KC / 2) + lanes, v);
-                asm volatile("tcgen05.fence::before_thread_sync;");
-                __syncwarp();
-                if (lane == 0) qg_arrive(&bars->a_full[i]);
+                if (h == 0) {
+                    qg_wait(&bars->a_empty[slot], phase, bars);
+                    __syncwarp();
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                }
+                qg_st<KC / 2>(tm + acol + slot * 64 + h * (KC / 2) + lanes, v);
             }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            __syncwarp();
+            if (lane == 0) qg_arrive(&bars->a_full[slot]);
+            if ((slot += 2) >= na) slot = grp, phase ^= 1;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == 16) {
@@ -411,32 +414,47 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(elected));
         const uint32_t base = __reduce_or_sync(0xffffffffu, tm);   // the same in all lanes, as the compiler now sees
         const uint64_t xdesc = tc_desc(tc_smem(xs), 128, qg_sbo<KC>());
-        uint32_t i = 0, aphase = 0, slot = 0, dphase = 1, in_run = 0;
+        uint32_t i = 0, aphase = 0, slot = 0, dphase = 1;
         for (int kr = 0; kr < ranges; kr++) {
-            const int nch = range_chunks(kr);
+            const int n = range_jobs(kr);
             for (int b = 0; b < tiles; b++)
-                for (int c = 0; c < nch; c++) {
-                    if (b == 0) qg_wait(&bars->x_full[c], kr & 1, bars);
-                    qg_wait(&bars->a_full[i], aphase, bars);
-                    if (in_run == 0) qg_wait(&bars->d_empty[slot], dphase, bars);
-                    asm volatile("tcgen05.fence::after_thread_sync;");
-                    const uint32_t at = base + kQgACol + i * (KC / 2), dt = base + dcol + slot * N;
+                for (int c = 0; c < n; c++) {
+                    const uint32_t at = base + acol + i * 64;
                     const uint64_t xd = xdesc + (uint32_t)(c * kSlotBytes >> 4);
-                    const bool last = in_run + 1 == a.run;
-                    if (elected) {
 #pragma unroll
-                        for (int p = 0; p < kPieces; p++)
+                    for (int h = 0; h < kItems; h += 2) {   // two chunks at a time, of one accumulator or two
+                        const bool wrap = slot + 1 == nd;
+                        const uint32_t slot1 = a.run == 2 ? slot : wrap ? 0 : slot + 1, phase1 = a.run == 1 && wrap ? dphase ^ 1 : dphase;
+                        uint64_t* bar = lane == 0   ? &bars->a_full[i]
+                                        : lane == 1 ? &bars->d_empty[slot]
+                                        : lane == 2 ? &bars->d_empty[slot1]
+                                                    : &bars->x_full[c];
+                        qg_wait(bar, lane == 0 ? aphase : lane == 1 ? dphase : lane == 2 ? phase1 : kr & 1, bars);
+                        __syncwarp();
+                        asm volatile("tcgen05.fence::after_thread_sync;");
+                        if (elected) {
 #pragma unroll
-                            for (int ks = 0; ks < KC / 16; ks++)
-                                qg_mma(dt, at + ks * 8, xd + ((p * kPieceBytes + ks * 256) >> 4), idesc, p + ks > 0 ? 1u : in_run);
-                        qg_commit(&bars->a_empty[i]);
-                        if (b == tiles - 1) qg_commit(&bars->x_empty[c]);
-                        if (last) qg_commit(&bars->d_full[slot]);
+                            for (int g = 0; g < 2; g++) {
+#pragma unroll
+                                for (int p = 0; p < kPieces; p++)
+#pragma unroll
+                                    for (int ks = 0; ks < KC / 16; ks++)
+                                        qg_mma(base + dcol + (g ? slot1 : slot) * N, at + (h + g) * (KC / 2) + ks * 8,
+                                               xd + (((h + g) * kChunkBytes + p * kPieceBytes + ks * 256) >> 4), idesc,
+                                               p + ks > 0 || (g && a.run == 2));
+                                if (g || a.run == 1) qg_commit(&bars->d_full[g ? slot1 : slot]);
+                            }
+                            if (h + 2 == kItems) {
+                                qg_commit(&bars->a_empty[i]);
+                                if (b == tiles - 1 && kr + 1 < ranges) qg_commit(&bars->x_empty[c]);
+                            }
+                        }
+                        __syncwarp();
+                        slot = slot1;
+                        dphase = phase1;
+                        if (++slot == nd) slot = 0, dphase ^= 1;
                     }
-                    __syncwarp();
-                    if (++i == kQgA) i = 0, aphase ^= 1;
-                    if (last && ++slot == nd) slot = 0, dphase ^= 1;
-                    in_run = last ? 0 : in_run + 1;
+                    if (++i == na) i = 0, aphase ^= 1;
                 }
         }
         if (elected) {
@@ -448,8 +466,8 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         // ---- x
         if (lane == 0) {
             pdl_wait();
-            const uint8_t* src = a.image + (size_t)blockIdx.y * a.chunks * kSlotBytes;
-            for (int ch = 0, c = 0, kr = 0; ch < a.chunks; ch++) {
+            const uint8_t* src = a.image + (size_t)blockIdx.y * a.jobs * kSlotBytes;
+            for (int ch = 0, c = 0, kr = 0; ch < a.jobs; ch++) {
                 if (kr) qg_wait(&bars->x_empty[c], (kr - 1) & 1, bars);
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(&bars->x_full[c])), "r"(kSlotBytes)
                              : "memory");
@@ -457,7 +475,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                 if (++c == a.slots) c = 0, kr++;
             }
             // the last copies, if nobody else has waited for them
-            const int left = range_chunks(ranges - 1);
+            const int left = range_jobs(ranges - 1);
             for (int c = 0; c < left; c++)
                 for (int it = 0; it < kQgWaits && !qg_try(&bars->x_full[c], (ranges - 1) & 1); it++) {}
         }
@@ -468,7 +486,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         uint32_t tile = 0;
         const auto fill = [&](auto* src) {
             for (int kr = 0; kr < ranges; kr++) {
-                const int first = kr * a.slots * KC / a.w.group;
+                const int first = kr * a.slots * 128 / a.w.group;
                 for (int b = 0; b < tiles; b++, tile++) {
                     float* to = scales + (tile & 1) * a.groups * 128;
                     if (tile > 1) qg_wait(&bars->s_empty[tile & 1], (tile >> 1 & 1) ^ 1, bars);
