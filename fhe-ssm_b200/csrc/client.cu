@@ -307,22 +307,24 @@ static void q4_mma_split(Context& cx, const Q4Args& a, cudaStream_t st) {
 
 template <int N, int KC, class XT>
 static void q4_gemm_launch(Context& cx, QgArgs a, cudaStream_t st) {
-    constexpr int kSlot = N * 256 * (std::is_same<XT, float>::value ? 2 : 1);   // a job's 128 columns of x
+    constexpr int kPieces = std::is_same<XT, float>::value ? 2 : 1, kSlot = N * 256 * kPieces;   // a job's 128 columns of x
     const int waves = (a.w.rows + 148 * kQgRowsMax - 1) / (148 * kQgRowsMax), xt = (a.m + N - 1) / N;
     a.block_rows = std::min(kQgRowsMax, ((a.w.rows + 148 * waves - 1) / (148 * waves) + 31) / 32 * 32);
     a.jobs = (a.w.cols + 127) / 128;
     a.slots = std::min({kQgSlotsMax, kQgXBytes / kSlot, a.jobs});
-    a.groups = std::min((a.slots * 128 + a.w.group - 2) / a.w.group + 1, (a.w.cols + a.w.group - 1) / a.w.group + 1);
+    // groups of a range, those past the last column's among them (zeros, but read)
+    a.groups = (int)std::min(((long long)a.slots * 128 + a.w.group - 2) / a.w.group + 1,
+                             ((long long)a.jobs * 128 + a.w.group - 1) / a.w.group);
     a.run = KC == 64 && a.w.group % 128 == 0 ? 2 : 1;
-    const size_t smem = 2 * kQgStages * kQgStageBytes + (size_t)a.slots * kSlot + (size_t)a.groups * 1024 + sizeof(QgBars);
+    const size_t smem = 2 * kQgStages * kQgStageBytes + (size_t)a.slots * kSlot + (size_t)a.groups * 1024 + N * sizeof(float) + sizeof(QgBars);
     const size_t image = (size_t)xt * a.jobs * kSlot;
     CUDA_CHECK(cudaMallocAsync((void**)&a.image, image + (size_t)xt * N * sizeof(int), st));
-    a.powers = reinterpret_cast<int*>(a.image + image);
+    a.powers = reinterpret_cast<float*>(a.image + image);
     try {
-        client_smem<k_q4_gemm<N, KC, XT>>(cx);
+        client_smem<k_q4_gemm<N, KC, kPieces>>(cx);
         k_q4_pack<N, KC, XT><<<xt * N, 128, 0, st>>>(a);
         CUDA_CHECK(cudaGetLastError());
-        launch_pdl(cx, k_q4_gemm<N, KC, XT>, dim3((a.w.rows + a.block_rows - 1) / a.block_rows, xt), dim3(kQgThreads), smem, st, a,
+        launch_pdl(cx, k_q4_gemm<N, KC, kPieces>, dim3((a.w.rows + a.block_rows - 1) / a.block_rows, xt), dim3(kQgThreads), smem, st, a,
                    cx.d_err);
     } catch (...) {
         cudaFreeAsync(a.image, st);
@@ -347,37 +349,65 @@ static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
     const long long row = a.ldx * (a.xt == FHE_F32 ? 4 : 2);
     a.wide = (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(a.m > 1 ? row : 0)) % 16 == 0;
     a.terms = a.xt == FHE_F32 ? 3 : a.xt == FHE_F16 ? 2 : 1;
-    static const int lim = getenv("QGMIN") ? atoi(getenv("QGMIN")) : 9;
-    if (a.m >= lim) {
+    // By the columns of pieces.  On 50,304 x 1024: 9 columns (3 float32 rows) take 18.5 us by k_q4_mma and 18.5 by k_q4_gemm, 8 of
+    // bfloat16 15 and 18, 16 of bfloat16 26 and 18; on 4,096 x 1024, where k_q4_gemm's two launches weigh more, 16 take 7.7 and 9.
+    const int pieces = a.m * a.terms;
+    if (pieces > (a.w.rows >= 16384 ? 9 : 20)) {
         const QgArgs q{a.w, a.x, a.m, a.ldx, a.out, a.ot, a.ldo, a.wide, 0, 0, 0, 0, 0, nullptr, nullptr};
         if (a.xt == FHE_F32) q4_gemm<float>(cx, q, st);
         else if (a.xt == FHE_F16) q4_gemm<__half>(cx, q, st);
         else q4_gemm<__nv_bfloat16>(cx, q, st);
         return;
     }
-    const int cols = a.m * a.terms;
-    if (cols <= 8) q4_mma_split<1>(cx, a, st);
-    else if (cols <= 16) q4_mma_split<2>(cx, a, st);
-    else if (cols <= 24) q4_mma_split<3>(cx, a, st);
-    else q4_mma_split<6>(cx, a, st);
+    if (pieces <= 8) q4_mma_split<1>(cx, a, st);
+    else if (pieces <= 16) q4_mma_split<2>(cx, a, st);
+    else q4_mma_split<3>(cx, a, st);
 }
 
 // ---- rows of a 4-bit table by token id --------------------------------------------------------
-// One warp per row; a token outside the table gives zeros.
-__global__ void __launch_bounds__(256) k_q4_rows(const fhe_q4 w, const int64_t* __restrict__ tokens, int m,
-                                                 void* __restrict__ out, int ot, long long ldo) {
-    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (r >= m) return;
+// A thread takes 8 columns: one 32-bit load, one scale, 16 or 32 bytes out.  What it costs is one round trip for the token, one
+// for its row and scale, and the output's bytes.  A token outside the table gives zeros.
+template <class T>
+__global__ void __launch_bounds__(128) k_q4_rows(const fhe_q4 w, const int64_t* __restrict__ tokens, T* __restrict__ out,
+                                                 long long ldo, uint32_t group_magic) {
+    const int c = (blockIdx.y * 128 + threadIdx.x) * 8;
+    if (c >= w.cols) return;
+    const long long r = blockIdx.x;
     const int64_t t = tokens[r];
-    const bool in = t >= 0 && t < w.rows;
-    for (int c = lane; c < w.cols; c += 32) {
-        float v = 0.f;
-        if (in) {
-            const int q = w.q[t * w.ldq + c / 2] >> (4 * (c & 1)) & 15;
-            v = (float)(q - 8) * ld_any(w.scale, w.scale_type, t * w.lds + c / w.group);
-        }
-        st_any(out, ot, (long long)r * ldo + c, v);
+    float v[8];
+    if (t >= 0 && t < w.rows) {
+        const uint32_t q = *reinterpret_cast<const uint32_t*>(w.q + t * w.ldq + c / 2), ch = c / 32;
+        const float s = ld_any(w.scale, w.scale_type, t * w.lds + (group_magic ? __umulhi(ch, group_magic) : ch));
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = (float)((int)(q >> (4 * j) & 15) - 8) * s;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = 0.f;
     }
+    T* o = out + r * ldo + c;
+    __align__(16) T u[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) qg_store(&u[j], v[j]);
+    if (c + 8 <= w.cols && reinterpret_cast<uintptr_t>(o) % 16 == 0) {
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; j++) reinterpret_cast<uint4*>(o)[j] = reinterpret_cast<const uint4*>(u)[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (c + j < w.cols) o[j] = u[j];
+    }
+}
+
+static uint32_t q4_group_magic(const fhe_q4& w) {
+    const int gpc = std::min(w.group, FHE_Q4_MAX_COLS) / 32;
+    return gpc == 1 ? 0u : (uint32_t)(((1ull << 32) + gpc - 1) / gpc);
+}
+
+template <class T>
+static void q4_rows(Context& cx, const fhe_q4& w, const int64_t* tokens, int m, void* out, long long ldo, cudaStream_t st) {
+    k_q4_rows<T><<<dim3(m, (w.cols + 1023) / 1024), 128, 0, st>>>(w, tokens, static_cast<T*>(out), ldo, q4_group_magic(w));
+    CUDA_CHECK(cudaGetLastError());
+    cx.launches++;
 }
 
 // ---- the choice of a token -----------------------------------------------------------------
@@ -1373,9 +1403,9 @@ extern "C" int fhe_q4_rows(fhe_ctx* cx, const fhe_q4* w, const int64_t* tokens, 
         client_ptr(cx->cx, tokens, 8, "tokens");
         client_ptr(cx->cx, out, ob, "out");
         cudaStream_t st = client_stream(cx, stream);
-        fhe::k_q4_rows<<<(m + 7) / 8, 256, 0, st>>>(*w, tokens, m, out, out_type, ldo);
-        CUDA_CHECK(cudaGetLastError());
-        cx->cx.launches++;
+        if (out_type == FHE_F32) fhe::q4_rows<float>(cx->cx, *w, tokens, m, out, ldo, st);
+        else if (out_type == FHE_F16) fhe::q4_rows<__half>(cx->cx, *w, tokens, m, out, ldo, st);
+        else fhe::q4_rows<__nv_bfloat16>(cx->cx, *w, tokens, m, out, ldo, st);
     });
 }
 

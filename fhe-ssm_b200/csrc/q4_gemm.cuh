@@ -3,8 +3,9 @@
 //     out[r][i] = sum_g s[i][g] sum_{c in g} (q[i][c] - 8) x[r][c]
 //
 // The inner sum is a 16-bit tensor-core product of whole numbers with x; the scale is applied to it in float32, as it
-// leaves tensor memory.  So nothing is rounded before the float32 sums but a float32 x, which is carried as two float16
-// pieces of 11 bits (scaled by a power of two of the row's maximum); float16 and bfloat16 are taken as they are.
+// leaves tensor memory.  x is carried in float16, scaled by a power of two of its row's maximum: float16 and bfloat16 as they are, float32 as two
+// pieces of 11 bits, the one rounding before the float32 sums.  (The table in bfloat16 takes 11 instructions for 8 values
+// to unpack, in float16 9, and the issue slots bound this kernel.)
 //
 // k_q4_pack writes x's operand as the shared-memory image of its chunks of columns; k_q4_gemm starts while it runs
 // (programmatic dependent launch) and waits for it where it first loads the image.
@@ -36,7 +37,7 @@ constexpr int kQgWaits = 1 << 22;             // bounded: some seconds
 
 struct QgBars {
     uint64_t a_full[kQgAMax], a_empty[kQgAMax], d_full[kQgDMax], d_empty[kQgDMax], x_full[kQgSlotsMax], x_empty[kQgSlotsMax],
-        s_full[2], s_empty[2], end;
+        s_full[2], s_empty[2], p_full, end;
     uint32_t tmem;
     int dead;      // a wait ran out: nobody waits any more, the output is NaN
 };
@@ -55,8 +56,8 @@ struct QgArgs {
     int jobs;         // jobs of all columns, 128 each
     int groups;       // most groups that a range meets
     int run;          // chunks that one accumulator takes before the scale is applied
-    uint8_t* image;   // x's operand [tile of N rows][chunk][piece], then the rows' powers of two
-    int* powers;
+    uint8_t* image;   // x's operand [tile of N rows][chunk][piece], then the rows' powers
+    float* powers;    // 2^p, by which the rows' sums are multiplied
 };
 
 __device__ __forceinline__ void qg_init(uint64_t* bar, int count) {
@@ -80,15 +81,15 @@ __device__ __forceinline__ bool qg_try(uint64_t* bar, uint32_t parity) {
 // Waits until the phase of the given parity has passed; after a wait that ran out, anywhere in the block, it does not wait
 __device__ __forceinline__ void qg_wait(uint64_t* bar, uint32_t parity, QgBars* b) {
     if (qg_try(bar, parity)) return;
-    for (int it = 0; it < kQgWaits; it++)
-        if (qg_try(bar, parity) || *(volatile int*)&b->dead) return;
+    for (int it = 0; it < kQgWaits; it++) {
+        if (qg_try(bar, parity)) return;
+        if ((it & 63) == 63 && *(volatile int*)&b->dead) return;
+    }
     *(volatile int*)&b->dead = 1;
 }
 
-// kind::f16, D float32, both operands of one type (0 float16, 1 bfloat16) and K-major, M = 128, N = n
-__device__ constexpr uint32_t qg_idesc(int n, int type) {
-    return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
+// kind::f16, D float32, both operands float16 and K-major, M = 128, N = n
+__device__ constexpr uint32_t qg_idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 __device__ __forceinline__ void qg_mma(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -135,25 +136,35 @@ __device__ __forceinline__ void qg_st(uint32_t t, const uint32_t* v) {
                      : "memory");
 }
 
-// 8 values of 4 bits -> pairs (0,4), (1,5), (2,6), (3,7) of q - 8
-template <class H>
+// 8 values of 4 bits -> float16 pairs (0,4), (1,5), (2,6), (3,7) of q - 8.  0x6400 is 1024, whose last bits count in ones: 1024 + q,
+// or 1024 + 16 q from the high half of a byte.
 __device__ __forceinline__ void qg_unpack(uint32_t w, uint32_t* p) {
-    if constexpr (std::is_same<H, __half>::value) {
-        // 0x6400 is 1024, whose last bits count in ones: 1024 + q, or 1024 + 16 q from the high half of a byte
-        const __half2 off = __float2half2_rn(1032.f), by = __float2half2_rn(0.0625f), low = __float2half2_rn(-72.f);
+    const __half2 off = __float2half2_rn(1032.f), by = __float2half2_rn(0.0625f), low = __float2half2_rn(-72.f);
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            const uint32_t a = (w & 0x000f000fu) | 0x64006400u, b = (w & 0x00f000f0u) | 0x64006400u;
-            const __half2 u = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
-            const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&b), by, low);
-            p[i] = *reinterpret_cast<const uint32_t*>(&u);
-            p[i + 1] = *reinterpret_cast<const uint32_t*>(&v);
-            w >>= 8;
-        }
-    } else {
-        q4_unpack(w, p);
+    for (int i = 0; i < 4; i += 2) {
+        const uint32_t a = (w & 0x000f000fu) | 0x64006400u, b = (w & 0x00f000f0u) | 0x64006400u;
+        const __half2 u = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+        const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&b), by, low);
+        p[i] = *reinterpret_cast<const uint32_t*>(&u);
+        p[i + 1] = *reinterpret_cast<const uint32_t*>(&v);
+        w >>= 8;
     }
 }
+__device__ __forceinline__ uint64_t qg_pack2(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+// two float32 multiply-adds
+__device__ __forceinline__ uint64_t qg_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+__device__ __forceinline__ void qg_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void qg_store(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void qg_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 template <int KC>
 __host__ __device__ constexpr uint32_t qg_sbo() { return KC / 8 * 128; }   // bytes of 8 rows of a chunk of x's operand
@@ -161,8 +172,7 @@ __host__ __device__ constexpr uint32_t qg_sbo() { return KC / 8 * 128; }   // by
 // x -> operand image.  One block per row; a thread takes 8 columns, in the order of qg_unpack's pairs.
 template <int N, int KC, class XT>
 __global__ void __launch_bounds__(128) k_q4_pack(const QgArgs a) {
-    constexpr bool kF32 = std::is_same<XT, float>::value;
-    using H = typename std::conditional<std::is_same<XT, __nv_bfloat16>::value, __nv_bfloat16, __half>::type;
+    constexpr bool kF32 = std::is_same<XT, float>::value, kF16 = std::is_same<XT, __half>::value;
     constexpr int kPieces = kF32 ? 2 : 1, kPieceBytes = N * KC * 2;
     pdl_trigger();
     const int r = blockIdx.x, n = r % N, units = a.jobs * 16;
@@ -178,19 +188,17 @@ __global__ void __launch_bounds__(128) k_q4_pack(const QgArgs a) {
             for (int j = 0; j < 8; j++) v[j] = r < a.m && k + j < a.w.cols ? src[j] : XT(0.f);
         }
     };
-    const auto pair = [](H x, H y) {
-        return (uint32_t)*reinterpret_cast<const uint16_t*>(&x) | (uint32_t)*reinterpret_cast<const uint16_t*>(&y) << 16;
-    };
+    const auto pair = [](__half x, __half y) { return (uint32_t)__half_as_ushort(x) | (uint32_t)__half_as_ushort(y) << 16; };
     __align__(16) XT v[8];
     load(threadIdx.x, v);
     float up = 1.f;
-    if constexpr (kF32) {
+    if constexpr (!kF16) {
         // the row's largest finite magnitude maps to 2^14 .. 2^15; a value under 2^-16 of it is held to 2^-39 of it
         uint32_t most = 0;
         const auto see = [&](const XT* u) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const uint32_t bits = __float_as_uint(u[j]) & 0x7fffffffu;
+                const uint32_t bits = __float_as_uint(q4_float(u[j])) & 0x7fffffffu;
                 most = max(most, bits < 0x7f800000u ? bits : 0u);
             }
         };
@@ -204,18 +212,20 @@ __global__ void __launch_bounds__(128) k_q4_pack(const QgArgs a) {
         most = __reduce_max_sync(0xffffffffu, most);
         if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = most;
         __syncthreads();
-        const int e = max(14, (int)(max(max(sm[0], sm[1]), max(sm[2], sm[3])) >> 23));
+        const int e = max(15, (int)(max(max(sm[0], sm[1]), max(sm[2], sm[3])) >> 23));
         up = __uint_as_float((uint32_t)(268 - e) << 23);
-        if (threadIdx.x == 0) a.powers[r] = e - 141;
+        if (threadIdx.x == 0) a.powers[r] = __uint_as_float((uint32_t)(e - 14) << 23);
+    } else if (threadIdx.x == 0) {
+        a.powers[r] = 1.f;
     }
     for (int u = threadIdx.x; u < units; u += 128) {
         if (u != threadIdx.x) load(u, v);
         uint8_t* dst = to + (size_t)(u / (KC / 8)) * kPieces * kPieceBytes + u % (KC / 8) * 128;
-        H h[8];
+        __half h[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            if constexpr (kF32) h[j] = __float2half_rn(v[j] * up);
-            else h[j] = v[j];
+            if constexpr (kF16) h[j] = v[j];
+            else h[j] = __float2half_rn(q4_float(v[j]) * up);
         }
         *reinterpret_cast<uint4*>(dst) = make_uint4(pair(h[0], h[4]), pair(h[1], h[5]), pair(h[2], h[6]), pair(h[3], h[7]));
         if constexpr (kF32) {
@@ -231,19 +241,17 @@ __global__ void __launch_bounds__(128) k_q4_pack(const QgArgs a) {
     }
 }
 
-// N rows of x (16, 32 or 64), KC columns a chunk (64, or 32 where the group is no multiple of 64), XT: x's type
-template <int N, int KC, class XT>
+// N rows of x (16, 32 or 64) in kPieces pieces, KC columns a chunk (64, or 32 where the group is no multiple of 64)
+template <int N, int KC, int kPieces>
 __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsigned int* err) {
-    constexpr bool kF32 = std::is_same<XT, float>::value, kBf = std::is_same<XT, __nv_bfloat16>::value;
-    using H = typename std::conditional<kBf, __nv_bfloat16, __half>::type;
-    constexpr int kPieces = kF32 ? 2 : 1;
     constexpr int kItems = 128 / KC;                    // chunks of a job
     constexpr int kPieceBytes = N * KC * 2, kChunkBytes = kPieceBytes * kPieces, kSlotBytes = kChunkBytes * kItems;
     extern __shared__ __align__(1024) uint8_t gsm[];
     uint8_t* ring = gsm;
     uint8_t* xs = gsm + 2 * kQgStages * kQgStageBytes;
     float* scales = reinterpret_cast<float*>(xs + (size_t)a.slots * kSlotBytes);   // [2][group of the range][128 rows]
-    QgBars* bars = reinterpret_cast<QgBars*>(scales + 2 * a.groups * 128);
+    float* powers = scales + 2 * a.groups * 128;                                    // [N]
+    QgBars* bars = reinterpret_cast<QgBars*>(powers + N);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row0 = blockIdx.x * a.block_rows, row1 = min(a.w.rows, row0 + a.block_rows), tiles = (row1 - row0 + 127) / 128;
     const int x0 = blockIdx.y * N;
@@ -259,6 +267,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         for (int i = 0; i < kQgDMax; i++) qg_init(&bars->d_full[i], 1), qg_init(&bars->d_empty[i], 8);
         for (int i = 0; i < a.slots; i++) qg_init(&bars->x_full[i], 1), qg_init(&bars->x_empty[i], 1);
         for (int i = 0; i < 2; i++) qg_init(&bars->s_full[i], 64), qg_init(&bars->s_empty[i], 8);
+        qg_init(&bars->p_full, 1);
         qg_init(&bars->end, 1);
         bars->dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;");
@@ -284,9 +293,9 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                 int left = per_group - kr * a.slots * kItems / a.run % per_group;
                 const float* sp = scales + (tile & 1) * a.groups * 128 + (warp & 3) * 32 + lane;
                 qg_wait(&bars->s_full[tile & 1], tile >> 1 & 1, bars);
-                float acc[kC];
+                uint64_t acc2[kC / 2];
 #pragma unroll
-                for (int j = 0; j < kC; j++) acc[j] = 0.f;
+                for (int j = 0; j < kC / 2; j++) acc2[j] = 0;
                 for (int c = 0; c < drains; c++) {
                     const float s = *sp;
                     if (--left == 0) left = per_group, sp += 128;
@@ -298,10 +307,14 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                     asm volatile("tcgen05.fence::before_thread_sync;");
                     __syncwarp();
                     if (lane == 0) qg_arrive(&bars->d_empty[slot]);
+                    const uint64_t s2 = qg_pack2(__float_as_uint(s), __float_as_uint(s));
 #pragma unroll
-                    for (int j = 0; j < kC; j++) acc[j] = fmaf(s, __uint_as_float(v[j]), acc[j]);
+                    for (int j = 0; j < kC / 2; j++) acc2[j] = qg_fma2(s2, qg_pack2(v[2 * j], v[2 * j + 1]), acc2[j]);
                     if (++slot == nd) slot = 0, phase ^= 1;
                 }
+                float acc[kC];
+#pragma unroll
+                for (int j = 0; j < kC; j++) acc[j] = __uint_as_float((uint32_t)(acc2[j / 2] >> (32 * (j & 1))));
                 __syncwarp();
                 if (lane == 0) qg_arrive(&bars->s_empty[tile & 1]);
                 const uint32_t keep = tm + b * N + half * kC + lanes;
@@ -321,21 +334,23 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                     for (int j = 0; j < kC; j++) acc[j] = __int_as_float(0x7fffffff);
                 }
                 const int r0 = x0 + half * kC, nr = min(kC, a.m - r0);
-                if (kF32 && nr > 0) {
-                    pdl_wait();
+                qg_wait(&bars->p_full, 0, bars);
 #pragma unroll
-                    for (int j = 0; j < kC; j++) {
-                        // 2^p in two factors, either of which float32 has
-                        const int p = j < nr ? a.powers[r0 + j] : 0;
-                        acc[j] = acc[j] * __uint_as_float((uint32_t)(127 + (p >> 1)) << 23) * __uint_as_float((uint32_t)(127 + p - (p >> 1)) << 23);
-                    }
+                for (int j = 0; j < kC; j += 4) {
+                    const float4 p = *reinterpret_cast<const float4*>(powers + half * kC + j);
+                    acc[j] *= p.x, acc[j + 1] *= p.y, acc[j + 2] *= p.z, acc[j + 3] *= p.w;
                 }
                 if (row >= row1) continue;
                 const auto store = [&](auto* out) {
                     out += r0 * a.ldo + row;
+                    if (nr >= kC) {
 #pragma unroll
-                    for (int j = 0; j < kC; j++, out += a.ldo)
-                        if (j < nr) st_any(out, sizeof(*out) == 4 ? FHE_F32 : std::is_same<decltype(out), __half*>::value ? FHE_F16 : FHE_BF16, 0, acc[j]);
+                        for (int j = 0; j < kC; j++, out += a.ldo) qg_store(out, acc[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kC; j++, out += a.ldo)
+                            if (j < nr) qg_store(out, acc[j]);
+                    }
                 };
                 if (a.ot == FHE_F32) store(static_cast<float*>(a.out));
                 else if (a.ot == FHE_F16) store(static_cast<__half*>(a.out));
@@ -382,16 +397,16 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
             else asm volatile("bar.sync 2, 128;" ::: "memory");
             fetch(s + kQgStages - 1);
             const uint8_t* st = my + (s % kQgStages) * kQgStageBytes + t * 64;
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < kItems; h++) {
                 uint32_t v[KC / 2];
 #pragma unroll
                 for (int q = 0; q < KC / 32; q++) {
                     const uint4 u = *reinterpret_cast<const uint4*>(st + (((h * (KC / 32) + q) ^ (t >> 1 & 3)) << 4));
-                    qg_unpack<H>(u.x, v + q * 16);
-                    qg_unpack<H>(u.y, v + q * 16 + 4);
-                    qg_unpack<H>(u.z, v + q * 16 + 8);
-                    qg_unpack<H>(u.w, v + q * 16 + 12);
+                    qg_unpack(u.x, v + q * 16);
+                    qg_unpack(u.y, v + q * 16 + 4);
+                    qg_unpack(u.z, v + q * 16 + 8);
+                    qg_unpack(u.w, v + q * 16 + 12);
                 }
                 if (h == 0) {
                     qg_wait(&bars->a_empty[slot], phase, bars);
@@ -409,7 +424,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == 16) {
         // ---- products: one lane issues them, the warp stays together
-        constexpr uint32_t idesc = qg_idesc(N, kBf ? 1 : 0);
+        constexpr uint32_t idesc = qg_idesc(N);
         uint32_t elected;
         asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(elected));
         const uint32_t base = __reduce_or_sync(0xffffffffu, tm);   // the same in all lanes, as the compiler now sees
@@ -464,8 +479,11 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         __syncwarp();
     } else if (warp == 17) {
         // ---- x
+        pdl_wait();
+        for (int j = lane; j < N; j += 32) powers[j] = a.powers[x0 + j];
+        __syncwarp();
         if (lane == 0) {
-            pdl_wait();
+            qg_arrive(&bars->p_full);
             const uint8_t* src = a.image + (size_t)blockIdx.y * a.jobs * kSlotBytes;
             for (int ch = 0, c = 0, kr = 0; ch < a.jobs; ch++) {
                 if (kr) qg_wait(&bars->x_empty[c], (kr - 1) & 1, bars);

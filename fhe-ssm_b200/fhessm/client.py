@@ -15,6 +15,7 @@ GPU, like any torch operation, and do not synchronise.  A call that cannot be se
 ``FheError``; nothing is converted or copied silently.
 """
 import ctypes as C
+import struct
 
 import numpy as np
 import torch
@@ -25,17 +26,11 @@ _VP = C.c_void_p
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _LEGACY_STREAM = 1      # cudaStreamLegacy: torch calls its default stream 0, which the C-ABI takes for the context's
 MAX_VOCAB = 1 << 20
+MAX_COLS = 1 << 20
 
-
-class Q4C(C.Structure):
-    _fields_ = [("q", _VP), ("scale", _VP), ("scale_type", C.c_int), ("rows", C.c_int), ("cols", C.c_int),
-                ("group", C.c_int), ("ldq", C.c_longlong), ("lds", C.c_longlong)]
-
-
-class SampleC(C.Structure):
-    _fields_ = [("temperature", _VP), ("top_k", _VP), ("top_p", _VP), ("min_p", _VP), ("temperature_all", C.c_float),
-                ("top_k_all", C.c_int32), ("top_p_all", C.c_float), ("min_p_all", C.c_float)]
-
+# fhe_q4 and fhe_sample_cfg as the bytes that the C-ABI reads (packed in 0.4 us; a ctypes structure takes 1.2)
+_Q4 = struct.Struct("@PPiiiiqq")
+_SAMPLE = struct.Struct("@PPPPfiff")
 
 _fns = None
 
@@ -45,10 +40,9 @@ def _sigs():
     if _fns is None:
         h = lib()
         for name, args in [
-            ("fhe_q4_matvec", [_VP, C.POINTER(Q4C), _VP, C.c_int, C.c_longlong, C.c_int, _VP, C.c_int, C.c_longlong,
-                               _VP]),
-            ("fhe_q4_rows", [_VP, C.POINTER(Q4C), _VP, C.c_int, _VP, C.c_int, C.c_longlong, _VP]),
-            ("fhe_sample", [_VP, C.POINTER(SampleC), _VP, C.c_int, C.c_longlong, C.c_int, C.c_int, _VP, _VP, _VP, _VP]),
+            ("fhe_q4_matvec", [_VP, C.c_char_p, _VP, C.c_int, C.c_longlong, C.c_int, _VP, C.c_int, C.c_longlong, _VP]),
+            ("fhe_q4_rows", [_VP, C.c_char_p, _VP, C.c_int, _VP, C.c_int, C.c_longlong, _VP]),
+            ("fhe_sample", [_VP, C.c_char_p, _VP, C.c_int, C.c_longlong, C.c_int, C.c_int, _VP, _VP, _VP, _VP]),
         ]:
             f = getattr(h, name)
             f.restype = C.c_int
@@ -67,23 +61,27 @@ def _stream(device):
 
 
 def _on_gpu(device, t, what):
-    if t.get_device() != device or t.device.type != "cuda":
+    if not t.is_cuda or t.get_device() != device:
         raise _bad(f"{what} is not on the context's GPU (cuda:{device})")
 
 
 def _rows_of(t, what):
     """(type, row count, row length, row stride) of a 2-d tensor with contiguous rows."""
-    if t.dim() != 2:
-        raise _bad(f"{what}: expected rows x columns, got {tuple(t.shape)}")
-    if t.dtype not in _TYPES:
+    shape = t.shape
+    if len(shape) != 2:
+        raise _bad(f"{what}: expected rows x columns, got {tuple(shape)}")
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
         raise _bad(f"{what}: float32, float16 or bfloat16, got {t.dtype}")
-    m, n = t.shape
-    if n > 1 and t.stride(1) != 1:
+    m, n = shape
+    if t.is_contiguous():
+        return kind, m, n, n
+    ld, step = t.stride()
+    if n > 1 and step != 1:
         raise _bad(f"{what}: the values of a row are not contiguous")
-    ld = t.stride(0) if m > 1 else n
     if m > 1 and ld < n:
         raise _bad(f"{what}: rows overlap")
-    return _TYPES[t.dtype], m, n, ld
+    return kind, m, n, ld if m > 1 else n
 
 
 class Q4Table:
@@ -92,29 +90,31 @@ class Q4Table:
     weight[i, c // 2].  weight: uint8 (rows, bytes), a row padded to a multiple of 16 bytes;
     scale: float32, float16 or bfloat16 (rows, ceil(cols / group)); group: a multiple of 32."""
 
-    __slots__ = ("weight", "scale", "rows", "cols", "group", "c", "ref")
+    __slots__ = ("weight", "scale", "rows", "cols", "group", "device", "c")
 
     def __init__(self, weight, scale, *, cols, group):
         if weight.dtype != torch.uint8 or weight.dim() != 2:
             raise _bad("q4 table: weight is a uint8 tensor, rows x bytes")
         rows, nbytes = weight.shape
-        if cols < 1 or group < 32 or group % 32:
-            raise _bad("q4 table: cols >= 1 and group a multiple of 32")
+        if not 1 <= cols <= MAX_COLS or group < 32 or group % 32 or group >= 1 << 31:
+            raise _bad(f"q4 table: 1 to {MAX_COLS} columns and a group that is a multiple of 32")
         if nbytes < -(-cols // 32) * 16:
             raise _bad("q4 table: rows are padded to a multiple of 16 bytes (32 columns)")
         st, srows, groups, lds = _rows_of(scale, "q4 scales")
         if srows != rows or groups != -(-cols // group):
             raise _bad(f"q4 scales: expected {(rows, -(-cols // group))}, got {tuple(scale.shape)}")
-        if weight.stride(1) != 1:
-            raise _bad("q4 table: the bytes of a row are not contiguous")
-        if scale.device != weight.device:
+        self.device = weight.get_device()
+        if scale.get_device() != self.device:
             raise _bad("q4 table: weight and scale are on different devices")
-        ldq = weight.stride(0) if rows > 1 else -(-nbytes // 16) * 16
-        if rows > 1 and ldq < nbytes:
-            raise _bad("q4 table: rows overlap")
+        ldq = nbytes
+        if not weight.is_contiguous():
+            ldq, step = weight.stride()
+            if step != 1 or (rows > 1 and ldq < nbytes):
+                raise _bad("q4 table: the bytes of a row are not contiguous, or rows overlap")
+        if rows <= 1:
+            ldq = -(-nbytes // 16) * 16
         self.weight, self.scale, self.rows, self.cols, self.group = weight, scale, rows, cols, group
-        self.c = Q4C(weight.data_ptr(), scale.data_ptr(), st, rows, cols, group, ldq, lds)
-        self.ref = C.byref(self.c)
+        self.c = _Q4.pack(weight.data_ptr(), scale.data_ptr(), st, rows, cols, group, ldq, lds)
 
     @classmethod
     def quantise(cls, w, *, group=64, scale_dtype=torch.float16, device="cpu"):
@@ -143,17 +143,17 @@ class Q4Table:
         return q * self.scale.float().repeat_interleave(self.group, dim=1)[:, :self.cols]
 
 
-def _out(out, like, shape, dtype, device):
+def _out(out, like, m, n, dtype, device):
     """(output, its type, its row stride): a new one, or the caller's."""
-    if dtype not in _TYPES:
+    kind = _TYPES.get(dtype)
+    if kind is None:
         raise _bad(f"out: float32, float16 or bfloat16, got {dtype}")
     if out is None:
-        return like.new_empty(shape, dtype=dtype), _TYPES[dtype], shape[1]
-    if tuple(out.shape) != shape or out.dtype != dtype:
-        raise _bad(f"out: expected {dtype} {shape}, got {out.dtype} {tuple(out.shape)}")
+        return like.new_empty((m, n), dtype=dtype), kind, n
+    if tuple(out.shape) != (m, n) or out.dtype != dtype:
+        raise _bad(f"out: expected {dtype} {(m, n)}, got {out.dtype} {tuple(out.shape)}")
     _on_gpu(device, out, "out")
-    ot, _, _, ldo = _rows_of(out, "out")
-    return out, ot, ldo
+    return out, kind, _rows_of(out, "out")[3]
 
 
 def q4_matvec(cx, x, table, *, dtype=torch.float32, out=None):
@@ -164,9 +164,10 @@ def q4_matvec(cx, x, table, *, dtype=torch.float32, out=None):
         raise _bad(f"x has {k} columns, the table {table.cols}")
     device = cx.p.device
     _on_gpu(device, x, "x")
-    _on_gpu(device, table.weight, "q4 table")
-    out, ot, ldo = _out(out, x, (m, table.rows), dtype, device)
-    _check((_fns or _sigs()).fhe_q4_matvec(cx.h, table.ref, x.data_ptr(), xt, ldx, m, out.data_ptr(), ot, ldo,
+    if table.device != device:
+        raise _bad(f"q4 table is not on the context's GPU (cuda:{device})")
+    out, ot, ldo = _out(out, x, m, table.rows, dtype, device)
+    _check((_fns or _sigs()).fhe_q4_matvec(cx.h, table.c, x.data_ptr(), xt, ldx, m, out.data_ptr(), ot, ldo,
                                            _stream(device)))
     return out
 
@@ -174,23 +175,24 @@ def q4_matvec(cx, x, table, *, dtype=torch.float32, out=None):
 def q4_rows(cx, tokens, table, *, dtype=torch.float32, out=None):
     """Rows of the table by token id: tokens (m,) int64 -> (m, cols) of `dtype` (fhe_q4_rows); a token
     outside the table (the -1 of an empty row) gives zeros."""
-    if tokens.dim() != 1 or tokens.dtype != torch.int64 or (tokens.numel() > 1 and tokens.stride(0) != 1):
+    if tokens.dim() != 1 or tokens.dtype != torch.int64 or not tokens.is_contiguous():
         raise _bad("tokens: a contiguous int64 vector")
     device = cx.p.device
     _on_gpu(device, tokens, "tokens")
-    _on_gpu(device, table.weight, "q4 table")
+    if table.device != device:
+        raise _bad(f"q4 table is not on the context's GPU (cuda:{device})")
     m = tokens.shape[0]
-    out, ot, ldo = _out(out, tokens, (m, table.cols), dtype, device)
-    _check((_fns or _sigs()).fhe_q4_rows(cx.h, table.ref, tokens.data_ptr(), m, out.data_ptr(), ot, ldo,
+    out, ot, ldo = _out(out, tokens, m, table.cols, dtype, device)
+    _check((_fns or _sigs()).fhe_q4_rows(cx.h, table.c, tokens.data_ptr(), m, out.data_ptr(), ot, ldo,
                                          _stream(device)))
     return out
 
 
 def _setting(device, v, rows, dtype, what):
-    """(device pointer or None, plain value) of a setting given as one number or as a value per row."""
-    if not torch.is_tensor(v):
-        return None, v
-    if v.dim() != 1 or v.shape[0] != rows or v.dtype != dtype or (rows > 1 and v.stride(0) != 1):
+    """(device pointer or 0, plain value) of a setting given as one number or as a value per row."""
+    if not isinstance(v, torch.Tensor):
+        return 0, v
+    if v.dim() != 1 or v.shape[0] != rows or v.dtype != dtype or not v.is_contiguous():
         raise _bad(f"{what}: one number, or a contiguous {dtype} vector with a value for each row")
     _on_gpu(device, v, what)
     return v.data_ptr(), 0
@@ -207,16 +209,19 @@ def sample(cx, logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if not 1 <= vocab <= MAX_VOCAB:
         raise _bad(f"logits: a vocabulary of 1 to {MAX_VOCAB}")
     up, _ = _setting(device, u, rows, torch.float32, "u")
-    if up is None:
+    if not isinstance(u, torch.Tensor):
         raise _bad("u: a float32 vector with a random number for each row")
     t, t1 = _setting(device, temperature, rows, torch.float32, "temperature")
     k, k1 = _setting(device, top_k, rows, torch.int32, "top_k")
     p, p1 = _setting(device, top_p, rows, torch.float32, "top_p")
     mp, mp1 = _setting(device, min_p, rows, torch.float32, "min_p")
     token, logprob = u.new_empty(rows, dtype=torch.int64), u.new_empty(rows)
-    cfg = SampleC(t, k, p, mp, t1, min(k1, vocab), p1, mp1)
-    _check((_fns or _sigs()).fhe_sample(cx.h, C.byref(cfg), logits.data_ptr(), lt, ld, rows, vocab, up,
-                                        token.data_ptr(), logprob.data_ptr(), _stream(device)))
+    try:
+        cfg = _SAMPLE.pack(t, k, p, mp, t1, k1 if k1 < vocab else vocab, p1, mp1)
+    except (struct.error, OverflowError, TypeError) as e:
+        raise _bad(f"sample: a setting is not a number of its type ({e})")
+    _check((_fns or _sigs()).fhe_sample(cx.h, cfg, logits.data_ptr(), lt, ld, rows, vocab, up, token.data_ptr(),
+                                        logprob.data_ptr(), _stream(device)))
     return token, logprob
 
 

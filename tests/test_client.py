@@ -85,7 +85,17 @@ def test_null_arguments_are_refused():
 
 
 def test_c_struct_sizes():
-    """The ctypes views have the header's layout (x86-64: natural alignment)."""
-    from fhessm.client import Q4C, SampleC
-    assert C.sizeof(Q4C) == 8 + 8 + 4 * 4 + 16 and Q4C.ldq.offset == 32
-    assert C.sizeof(SampleC) == 4 * 8 + 4 * 4 and SampleC.temperature_all.offset == 32
+    """The packed bytes have the header's layout (x86-64: natural alignment)."""
+    from fhessm import client
+
+    class Q4(C.Structure):
+        _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("scale_type", C.c_int), ("rows", C.c_int), ("cols", C.c_int),
+                    ("group", C.c_int), ("ldq", C.c_longlong), ("lds", C.c_longlong)]
+
+    class Cfg(C.Structure):
+        _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                    ("temperature_all", C.c_float), ("top_k_all", C.c_int32), ("top_p_all", C.c_float),
+                    ("min_p_all", C.c_float)]
+
+    assert client._Q4.pack(1 << 40, 2, 3, 4, 5, 6, 1 << 33, 8) == bytes(Q4(1 << 40, 2, 3, 4, 5, 6, 1 << 33, 8))
+    assert client._SAMPLE.pack(1, 2, 3, 4, 0.5, -6, 7.5, 8.25) == bytes(Cfg(1, 2, 3, 4, 0.5, -6, 7.5, 8.25))

@@ -7,8 +7,6 @@ Tolerances, from the definitions:
   * a token: equal, decisions within 2^-20 of their limits going either way (client_ref.OPEN);
   * a log-probability: z is a rounded quotient (2^-23 |z|), the logarithm of a sum that is good to 2^-21.
 """
-import ctypes as C
-
 import numpy as np
 import pytest
 import torch
@@ -58,6 +56,7 @@ def check_product(got, x, w, ot):
     (32, 640, 1024, 64, "f32", "f16", "bf16"), (33, 385, 2050, 128, "f32", "f16", "f32"),
     (48, 200, 200, 1024, "f16", "f16", "f16"), (63, 129, 999, 160, "f32", "bf16", "f32"),
     (64, 4099, 1024, 64, "f32", "f16", "f32"), (64, 300, 4096, 32, "bf16", "f16", "f32"),
+    (128, 512, 48, 32, "f32", "f16", "f32"), (40, 200, 33, 32, "bf16", "f32", "f32"), (70, 513, 136, 32, "f16", "bf16", "f32"),
     (24, 50304, 1024, 32, "f32", "f16", "f32"), (64, 20000, 2048, 96, "bf16", "f16", "f32"),
     (65, 130, 320, 64, "f32", "f16", "f32"), (130, 77, 161, 32, "bf16", "f32", "f32"),
     (200, 1000, 128, 128, "f16", "f16", "f32")])
@@ -329,7 +328,7 @@ def test_calls_on_the_context_stream_and_in_a_graph(cx):
     torch.cuda.synchronize()
     h = client._sigs()
     before = cx.launches()
-    assert h.fhe_q4_matvec(cx.h, C.byref(t.c), x.data_ptr(), 0, 256, 8, out.data_ptr(), 0, 3000, None) == 0
+    assert h.fhe_q4_matvec(cx.h, t.c, x.data_ptr(), 0, 256, 8, out.data_ptr(), 0, 3000, None) == 0
     cx.sync()
     assert cx.launches() > before
     assert torch.equal(out, client.q4_matvec(cx, x, t))
@@ -394,13 +393,13 @@ def test_refusals(cx):
     h = client._sigs()
     host = np.zeros((2, 64), np.float32)
     out = torch.empty(2, 30, device="cuda")
-    assert h.fhe_q4_matvec(cx.h, C.byref(t.c), host.ctypes.data, 0, 64, 2, out.data_ptr(), 0, 30, None) == -1
-    assert h.fhe_q4_matvec(cx.h, C.byref(t.c), x.data_ptr(), 3, 64, 2, out.data_ptr(), 0, 30, None) == -1
-    assert h.fhe_q4_matvec(cx.h, C.byref(t.c), x.data_ptr(), 0, 63, 2, out.data_ptr(), 0, 30, None) == -1
-    assert h.fhe_q4_matvec(cx.h, C.byref(t.c), x.data_ptr(), 0, 64, 2, out.data_ptr(), 0, 29, None) == -1
-    assert h.fhe_q4_matvec(cx.h, C.byref(t.c), x.data_ptr(), 0, 64, -1, out.data_ptr(), 0, 30, None) == -1
-    assert h.fhe_q4_matvec(cx.h, C.byref(t.c), x.data_ptr() + 2, 0, 64, 1, out.data_ptr(), 0, 30, None) == -1
-    assert h.fhe_q4_matvec(cx.h, C.byref(t.c), None, 0, 64, 2, out.data_ptr(), 0, 30, None) == -1
+    assert h.fhe_q4_matvec(cx.h, t.c, host.ctypes.data, 0, 64, 2, out.data_ptr(), 0, 30, None) == -1
+    assert h.fhe_q4_matvec(cx.h, t.c, x.data_ptr(), 3, 64, 2, out.data_ptr(), 0, 30, None) == -1
+    assert h.fhe_q4_matvec(cx.h, t.c, x.data_ptr(), 0, 63, 2, out.data_ptr(), 0, 30, None) == -1
+    assert h.fhe_q4_matvec(cx.h, t.c, x.data_ptr(), 0, 64, 2, out.data_ptr(), 0, 29, None) == -1
+    assert h.fhe_q4_matvec(cx.h, t.c, x.data_ptr(), 0, 64, -1, out.data_ptr(), 0, 30, None) == -1
+    assert h.fhe_q4_matvec(cx.h, t.c, x.data_ptr() + 2, 0, 64, 1, out.data_ptr(), 0, 30, None) == -1
+    assert h.fhe_q4_matvec(cx.h, t.c, None, 0, 64, 2, out.data_ptr(), 0, 30, None) == -1
 
 
 def test_encrypted_decode_loop():
