@@ -503,17 +503,43 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         const int t = tid - 18 * 32, groups = (a.w.cols + a.w.group - 1) / a.w.group;
         uint32_t tile = 0;
         const auto fill = [&](auto* src) {
+            using S = typename std::remove_cv<typename std::remove_pointer<decltype(src)>::type>::type;
+            constexpr int kPer = 16 / sizeof(S), kDeep = 4;   // scales of a load; loads in flight for each of two rows
+            // whole 16-byte loads: the range's first group and the row's last one have to lie on their bounds
+            const bool wide = (a.w.lds | groups) % kPer == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0;
             for (int kr = 0; kr < ranges; kr++) {
                 const int first = kr * a.slots * 128 / a.w.group;
                 for (int b = 0; b < tiles; b++, tile++) {
-                    float* to = scales + (tile & 1) * a.groups * 128;
+                    float* to = scales + (tile & 1) * a.groups * 128 + t;
+                    const S* p0 = src + min(row0 + b * 128 + t, a.w.rows - 1) * a.w.lds + first;
+                    const S* p1 = src + min(row0 + b * 128 + t + 64, a.w.rows - 1) * a.w.lds + first;
                     if (tile > 1) qg_wait(&bars->s_empty[tile & 1], (tile >> 1 & 1) ^ 1, bars);
+                    if (wide && first % kPer == 0) {
+                        for (int g0 = 0; g0 < a.groups; g0 += kDeep * kPer) {
+                            uint4 u[2][kDeep];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const auto* p = src + min(row0 + b * 128 + t + h * 64, a.w.rows - 1) * a.w.lds + first;
+                            for (int i = 0; i < kDeep; i++)
+                                if (g0 + i * kPer < a.groups && first + g0 + i * kPer < groups) {
+                                    u[0][i] = reinterpret_cast<const uint4*>(p0 + g0)[i];
+                                    u[1][i] = reinterpret_cast<const uint4*>(p1 + g0)[i];
+                                } else {
+                                    u[0][i] = u[1][i] = make_uint4(0, 0, 0, 0);
+                                }
+#pragma unroll
+                            for (int i = 0; i < kDeep; i++)
+#pragma unroll
+                                for (int j = 0; j < kPer; j++)
+                                    if (g0 + i * kPer + j < a.groups) {
+                                        to[(g0 + i * kPer + j) * 128] = q4_float(reinterpret_cast<const S*>(&u[0][i])[j]);
+                                        to[(g0 + i * kPer + j) * 128 + 64] = q4_float(reinterpret_cast<const S*>(&u[1][i])[j]);
+                                    }
+                        }
+                    } else {
 #pragma unroll 8
-                        for (int g = 0; g < a.groups; g++)
-                            to[g * 128 + t + h * 64] = first + g < groups ? q4_float(p[g]) : 0.f;
+                        for (int g = 0; g < a.groups; g++) {
+                            to[g * 128] = first + g < groups ? q4_float(p0[g]) : 0.f;
+                            to[g * 128 + 64] = first + g < groups ? q4_float(p1[g]) : 0.f;
+                        }
                     }
                     qg_arrive(&bars->s_full[tile & 1]);
                 }
