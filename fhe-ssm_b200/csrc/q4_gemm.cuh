@@ -363,39 +363,46 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         uint8_t* my = ring + grp * kQgStages * kQgStageBytes;
         const int units = (a.w.cols + 31) / 32;   // 16-byte units of a row
         const int jobs = tiles * a.jobs;
-        int fkr = 0, fb = 0, fc = grp;   // the job to fetch next
-        const auto fetch = [&](int s) {
-            while (fkr < ranges) {
-                const int n = range_jobs(fkr);
-                if (fc < n) break;
-                fc -= n;
-                if (++fb == tiles) fb = 0, fkr++;
-            }
-            if (fkr < ranges) {
-                const int unit = (fkr * a.slots + fc) * 4 + (t & 3);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int r = (t >> 2) + 32 * i, row = row0 + fb * 128 + r;
-                    if (row < row1 && unit < units) {
-                        const uint32_t dst = tc_smem(my + (s % kQgStages) * kQgStageBytes + r * 64 + (((t & 3) ^ (r >> 1 & 3)) << 4));
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst),
-                                     "l"(a.w.q + row * a.w.ldq + unit * 16ll)
-                                     : "memory");
-                    }
+        // the job to fetch next; a thread copies the same 16-byte unit of 4 rows
+        int fkr = 0, fb = 0, fc = grp, fn = range_jobs(0), fat = 0;
+        const long long ld32 = 32 * a.w.ldq;
+        const uint8_t* fsrc = a.w.q + (row0 + (t >> 2)) * a.w.ldq + (t & 3) * 16;
+        const uint32_t fdst = tc_smem(my) + (t >> 2) * 64 + (((t & 3) ^ (t >> 3 & 3)) << 4);
+        const auto fetch = [&]() {
+            while (fc >= fn) {
+                fc -= fn;
+                if (++fb < tiles) {
+                    fsrc += 4 * ld32;
+                } else if (++fkr < ranges) {
+                    fsrc += a.slots * 64 - (tiles - 1) * 4 * ld32;
+                    fb = 0;
+                    fn = range_jobs(fkr);
+                } else {
+                    fn = 1 << 30;   // no more
                 }
-                fc += 2;
             }
+            if (fkr < ranges && (fkr * a.slots + fc) * 4 + (t & 3) < units) {
+                const uint8_t* src = fsrc + fc * 64;
+                const int row = row0 + fb * 128 + (t >> 2);
+#pragma unroll
+                for (int i = 0; i < 4; i++, src += ld32)
+                    if (row + 32 * i < row1)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(fdst + fat * kQgStageBytes + i * 2048), "l"(src)
+                                     : "memory");
+            }
+            fc += 2;
+            fat = (fat + 1) % kQgStages;
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
-        for (int s = 0; s < kQgStages - 1; s++) fetch(s);
+        for (int s = 0; s < kQgStages - 1; s++) fetch();
         uint32_t slot = grp, phase = 1;
         for (int j = grp, s = 0; j < jobs; j += 2, s++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kQgStages - 2) : "memory");
             // all copies of the stage are there; the one before it is read
             if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
             else asm volatile("bar.sync 2, 128;" ::: "memory");
-            fetch(s + kQgStages - 1);
+            fetch();
             const uint8_t* st = my + (s % kQgStages) * kQgStageBytes + t * 64;
 #pragma unroll 1
             for (int h = 0; h < kItems; h++) {
