@@ -742,11 +742,13 @@ __device__ uint64_t sample_pick(SampleList& l, uint32_t m, uint64_t want, uint64
     uint32_t lo = 0, hi = 0xffffffffu;
     if (m > kSampleFew) {
         while (true) {
-            if (tid == 0) l.key_lo = 0xffffffffu, l.key_hi = 0;
+            // the least and largest key from lo to hi
+            if (tid == 0) l.key_lo = 0xffffffffu, l.key_hi = 0, l.at = -1;
+            l.count[tid] = l.hi[tid] = l.lo[tid] = 0;
             __syncthreads();
             uint32_t a = 0xffffffffu, b = 0;
             for (uint32_t j = tid; j < m; j += kSampleThreads)
-                if (in(j)) a = min(a, key(j)), b = max(b, key(j));
+                if (in(j) && key(j) >= lo && key(j) <= hi) a = min(a, key(j)), b = max(b, key(j));
             a = __reduce_min_sync(0xffffffffu, a);
             b = __reduce_max_sync(0xffffffffu, b);
             if (lane == 0 && a <= b) atomicMin(&l.key_lo, a), atomicMax(&l.key_hi, b);
@@ -754,53 +756,50 @@ __device__ uint64_t sample_pick(SampleList& l, uint32_t m, uint64_t want, uint64
             lo = l.key_lo;
             hi = l.key_hi;
             if (lo > hi) { *sum = before; return 0; }
-            uint32_t n;
-            while (true) {
-                // the tokens with keys in [lo, hi], in up to 1024 bins of equal width
-                const int shift = max(0, 32 - __clz(hi - lo) - 10);
-                l.count[tid] = l.hi[tid] = l.lo[tid] = 0;
-                if (tid == 0) l.at = -1;
+            if (by_order && lo == hi) {   // many equal logits
+                by_order = false;
+                equal = hi;
+                lo = 0, hi = 0xffffffffu;
                 __syncthreads();
-                for (uint32_t j = tid; j < m; j += kSampleThreads) {
-                    if (!in(j)) continue;
-                    const uint32_t k = key(j);
-                    if (k < lo || k > hi) continue;
-                    const uint32_t b = (hi - k) >> shift;
-                    const uint64_t w = sample_weight(l.e[j]);
-                    atomicAdd(&l.count[b], 1u);
-                    atomicAdd(&l.hi[b], (uint32_t)(w >> 20));        // the list's sums fit 32 bits in these halves
-                    atomicAdd(&l.lo[b], (uint32_t)w & 0xfffffu);
-                }
-                __syncthreads();
-                const uint64_t w = ((uint64_t)l.hi[tid] << 20) + l.lo[tid], own = BY == kByCount ? l.count[tid] : w;
-                const uint64_t run = sample_block_scan(own, l.red);
-                if (run >= want && run - own < want) l.at = tid, l.got = run - own;
-                if (tid == kSampleRadix - 1) l.sum = run;
-                __syncthreads();
-                const int at = l.at;
-                if (at < 0) {
-                    if (BY == kByCount) {
-                        uint64_t all = 0;
-                        for (uint32_t j = tid; j < m; j += kSampleThreads) all += in(j) ? sample_weight(l.e[j]) : 0;
-                        *sum = sample_reduce(all, [](uint64_t x, uint64_t y) { return x + y; }, l.red);
-                    } else {
-                        *sum = before + l.sum;
-                    }
-                    __syncthreads();
-                    return 0;
-                }
-                want -= l.got;
-                if (BY != kByCount) before += l.got;
-                n = l.count[at];
-                const uint32_t top = hi - ((uint32_t)at << shift), width = (1u << shift) - 1;
-                lo = top - lo > width ? top - width : lo;
-                hi = top;
-                __syncthreads();
-                if (n <= kSampleFew || shift == 0) break;
+                continue;
             }
+            // the tokens between them, in up to 1024 bins of equal width
+            const int shift = max(0, 32 - __clz(hi - lo) - 10);
+            for (uint32_t j = tid; j < m; j += kSampleThreads) {
+                if (!in(j)) continue;
+                const uint32_t k = key(j);
+                if (k < lo || k > hi) continue;
+                const uint32_t b = (hi - k) >> shift;
+                const uint64_t w = sample_weight(l.e[j]);
+                atomicAdd(&l.count[b], 1u);
+                atomicAdd(&l.hi[b], (uint32_t)(w >> 20));        // the list's sums fit 32 bits in these halves
+                atomicAdd(&l.lo[b], (uint32_t)w & 0xfffffu);
+            }
+            __syncthreads();
+            const uint64_t w = ((uint64_t)l.hi[tid] << 20) + l.lo[tid], own = BY == kByCount ? l.count[tid] : w;
+            const uint64_t run = sample_block_scan(own, l.red);
+            if (run >= want && run - own < want) l.at = tid, l.got = run - own;
+            if (tid == kSampleRadix - 1) l.sum = run;
+            __syncthreads();
+            const int at = l.at;
+            if (at < 0) {
+                if (BY == kByCount) {
+                    uint64_t all = 0;
+                    for (uint32_t j = tid; j < m; j += kSampleThreads) all += in(j) ? sample_weight(l.e[j]) : 0;
+                    *sum = sample_reduce(all, [](uint64_t x, uint64_t y) { return x + y; }, l.red);
+                } else {
+                    *sum = before + l.sum;
+                }
+                __syncthreads();
+                return 0;
+            }
+            want -= l.got;
+            if (BY != kByCount) before += l.got;
+            const uint32_t n = l.count[at], top = hi - ((uint32_t)at << shift), width = (1u << shift) - 1;
+            lo = top - lo > width ? top - width : lo;
+            hi = top;
+            __syncthreads();
             if (n <= kSampleFew) break;
-            by_order = false;   // more equal logits than that
-            equal = hi;
         }
     }
     // few: each against the others
@@ -843,6 +842,7 @@ struct alignas(16) SampleShared {
     union {
         SampleList list;
         SampleRadix radix;   // where the list will not do
+        uint32_t coarse_in[kSampleClusterMax][kSampleCoarse];   // before the list
     };
     uint64_t sum[kSampleClusterMax], above[kSampleClusterMax], part[kSampleClusterMax];   // each block writes its own to all
     float top[kSampleClusterMax], reach[kSampleClusterMax];
@@ -996,6 +996,13 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
     // each warp's stretch
     const int per = (n4 + 128 * kSampleWarps - 1) / (128 * kSampleWarps) * 128, i0 = min(n4, warp * per), i1 = min(n4, i0 + per);
 
+    // token j of all blocks' lists, one after the other: the block's list and its place there
+    const auto other = [&](uint32_t j, uint32_t& from) -> const SampleList* {
+        int q = 0;
+        while (j >= sh.n[q]) j -= sh.n[q++];
+        from = j;
+        return &cluster.map_shared_rank(&sh, q)->list;
+    };
     if (few) {
         const auto take = [&](float x, int i) {
             if (x >= reach && x > -INFINITY) {
@@ -1014,11 +1021,10 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
         for (int q = 0; q < nb; q++) m += sh.n[q];
         if (m <= kSampleList) {
             if (rank == 0) {
-                uint32_t off = sh.n[0];
-                for (int q = 1; q < nb; q++) {
-                    const SampleList* o = &cluster.map_shared_rank(&sh, q)->list;
-                    for (uint32_t j = tid; j < sh.n[q]; j += kSampleThreads) list.x[off + j] = o->x[j], list.i[off + j] = o->i[j];
-                    off += sh.n[q];
+                for (uint32_t j = sh.n[0] + tid; j < m; j += kSampleThreads) {
+                    uint32_t from;
+                    const SampleList* o = other(j, from);
+                    list.x[j] = o->x[from], list.i[j] = o->i[from];
                 }
             }
             if (nb > 1) cluster.sync();
@@ -1118,6 +1124,8 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
             for (int j = 0; j < 8; j++) c += sh.counts[tid * 8 + j], v += sh.sums[tid * 8 + j];
             sh.coarse_counts[tid] = c;
             sh.coarse_sums[tid] = v;
+            // what the first selection reads, to every block (loads across blocks take 500 cycles each way)
+            for (int q = 0; q < nb; q++) cluster.map_shared_rank(&sh, q)->coarse_in[rank][tid] = by_k ? c : v;
         }
         if (tid < nb) *cluster.map_shared_rank(&sh.sum[rank], tid) = s;
         cluster.sync();
@@ -1133,7 +1141,10 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
         const uint32_t* fine = by_count ? sh.counts : sh.sums;
         uint64_t own = 0;
         if (tid < kSampleCoarse) {
-            own = sample_across(cluster, &coarse[tid], nb);
+            if (by_count == by_k)
+                for (int q = 0; q < nb; q++) own += sh.coarse_in[q][tid];
+            else
+                own = sample_across(cluster, &coarse[tid], nb);
             if (!by_count) own = sample_bin_sum(own, tid * 8);
         }
         const uint64_t run = sample_block_scan(own, sh.red);
@@ -1198,12 +1209,10 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
             for (int q = 0; q < nb; q++) over += sh.above[q], m += sh.n[q];
             bool slow = m > kSampleList || (!by_count && over >= want);
             if (!slow) {
-                uint32_t off = sh.n[0];
-                for (int q = 1; q < nb; q++) {
-                    const SampleList* o = &cluster.map_shared_rank(&sh, q)->list;
-                    for (uint32_t j = tid; j < sh.n[q]; j += kSampleThreads)
-                        list.x[off + j] = o->x[j], list.i[off + j] = o->i[j], list.e[off + j] = o->e[j];
-                    off += sh.n[q];
+                for (uint32_t j = sh.n[0] + tid; j < m; j += kSampleThreads) {
+                    uint32_t from;
+                    const SampleList* o = other(j, from);
+                    list.x[j] = o->x[from], list.i[j] = o->i[from], list.e[j] = o->e[from];
                 }
                 __syncthreads();
                 bound = by_count ? sample_pick<kByCount>(list, m, want - sh.run_at, &found)
