@@ -851,11 +851,11 @@ struct alignas(16) SampleShared {
     int slow;
     uint64_t red[32];
     float redf[32];
-    uint64_t run_all, run_at;
+    uint64_t want, guess, run_at;
     int at, lo;
     uint32_t listed, least;
     uint32_t warp_hi[kSampleWarps], warp_lo[kSampleWarps];
-    uint32_t counts[kSampleBins], sums[kSampleBins];
+    alignas(16) uint32_t counts[kSampleBins], sums[kSampleBins];
     uint32_t coarse_counts[kSampleCoarse], coarse_sums[kSampleCoarse];
 };
 static_assert(sizeof(SampleShared) + (kSamplePart + 128) * sizeof(float) <= 232448, "a block's shared memory");
@@ -1119,9 +1119,11 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
     if (by_k || by_p) {
         const uint64_t s = warps_sum(warp_w);
         if (tid < kSampleCoarse) {
-            uint32_t c = 0, v = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) c += sh.counts[tid * 8 + j], v += sh.sums[tid * 8 + j];
+            const auto eight = [&](const uint32_t* h) {
+                const uint4 u = reinterpret_cast<const uint4*>(h)[2 * tid], v = reinterpret_cast<const uint4*>(h)[2 * tid + 1];
+                return u.x + u.y + u.z + u.w + v.x + v.y + v.z + v.w;
+            };
+            const uint32_t c = by_k ? eight(sh.counts) : 0, v = by_p ? eight(sh.sums) : 0;
             sh.coarse_counts[tid] = c;
             sh.coarse_sums[tid] = v;
             // what the first selection reads, to every block (loads across blocks take 500 cycles each way)
@@ -1136,7 +1138,7 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
     bool summed = !by_k && (!by_p || set.mp == 0.f);   // warp_w follows what is kept as it is found
     // One selection.  The histogram tells a guess of the last kept token's bin; the tokens of that bin and its neighbours go to
     // the list, the weights above are summed, and block 0 selects.
-    const auto locate = [&](bool by_count, uint64_t want) {
+    const auto locate = [&](bool by_count, uint64_t of) {
         const uint32_t* coarse = by_count ? sh.coarse_counts : sh.coarse_sums;
         const uint32_t* fine = by_count ? sh.counts : sh.sums;
         uint64_t own = 0;
@@ -1148,15 +1150,22 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
             if (!by_count) own = sample_bin_sum(own, tid * 8);
         }
         const uint64_t run = sample_block_scan(own, sh.red);
-        if (tid == kSampleThreads - 1) sh.run_all = run;
         if (tid == 0) sh.at = -1, sh.listed = 0;
-        __syncthreads();
-        uint64_t guess = want;
-        if (!by_count) {
-            // all sums lack the bits below the leading 16 alike
-            guess = (uint64_t)((double)want * ((double)sh.run_all / (double)all));
-            guess = guess < 1 ? 1 : guess > sh.run_all ? sh.run_all : guess;
+        if (tid == kSampleThreads - 1) {
+            // what is asked for: top_k, or top_p's part of the sum; in the histogram's sums, which lack the bits below the leading
+            // 16 of each all alike, a little less
+            uint64_t want = set.k, guess = want;
+            if (!by_count) {
+                want = set.limit(of);
+                const float lack = run < all ? (float)(all - run) / (float)all : 0.f;
+                guess = want - (uint64_t)((float)want * lack);
+                guess = guess < 1 ? 1 : guess > run ? run : guess;
+            }
+            sh.want = want;
+            sh.guess = guess;
         }
+        __syncthreads();
+        const uint64_t want = sh.want, guess = sh.guess;
         if (run >= guess && run - own < guess) sh.at = tid, sh.run_at = run - own;
         __syncthreads();
         if (sh.at < 0) {   // no more than top_k have a weight: nothing is struck off
@@ -1260,8 +1269,8 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
         }
         __syncthreads();
     };
-    if (by_k) locate(true, set.k);
-    if (by_p) locate(false, set.limit(by_k ? sh.found : all));
+    if (by_k) locate(true, 0);
+    if (by_p) locate(false, by_k ? sh.found : all);
 
     // the kept weights of each warp's stretch, block and cluster; the warp that the target falls to walks
     const auto kept = [&](float e) { return __float_as_uint(e) > cut && e >= set.mp ? e : 0.f; };
