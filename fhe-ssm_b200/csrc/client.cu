@@ -311,27 +311,52 @@ static void q4_gemm_launch(Context& cx, QgArgs a, cudaStream_t st) {
     const int waves = (a.w.rows + 148 * kQgRowsMax - 1) / (148 * kQgRowsMax), xt = (a.m + N - 1) / N;
     a.block_rows = std::min(kQgRowsMax, ((a.w.rows + 148 * waves - 1) / (148 * waves) + 31) / 32 * 32);
     a.jobs = (a.w.cols + 127) / 128;
-    a.slots = std::min({kQgSlotsMax, kQgXBytes / kSlot, a.jobs});
+    a.part_jobs = a.jobs;
+    // A short table of many columns: whole tiles, the columns in parts.  A job takes 0.5 us of a block, the sum of the parts a
+    // launch: 64 float16 rows on 1,005 x 3,829 take NN us in one part and NN in 15, on 4,096 x 1,024 (8 jobs) no less than before.
+    const int tiles = (a.w.rows + 127) / 128;
+    if ((long long)tiles * xt * 2 <= 148 && a.jobs >= 12) {
+        a.block_rows = 128;
+        const int parts = std::min(148 / (tiles * xt), a.jobs / 2);
+        a.part_jobs = (a.jobs + parts - 1) / parts;
+    }
+    const int parts = (a.jobs + a.part_jobs - 1) / a.part_jobs;
+    a.slots = std::min({kQgSlotsMax, kQgXBytes / kSlot, a.part_jobs});
     // groups of a range, those past the last column's among them (zeros, but read)
     a.groups = (int)std::min(((long long)a.slots * 128 + a.w.group - 2) / a.w.group + 1,
                              ((long long)a.jobs * 128 + a.w.group - 1) / a.w.group);
     a.run = KC == 64 && a.w.group % 128 == 0 ? 2 : 1;
-    const size_t smem = 2 * kQgStages * kQgStageBytes + (size_t)a.slots * kSlot + (size_t)a.groups * 1024 + N * sizeof(float) + sizeof(QgBars);
-    const size_t image = (size_t)xt * a.jobs * kSlot;
-    CUDA_CHECK(cudaMallocAsync((void**)&a.image, image + (size_t)xt * N * sizeof(int), st));
-    a.powers = reinterpret_cast<float*>(a.image + image);
+    const size_t smem = 2 * kQgStages * kQgStageBytes + (size_t)a.slots * kSlot + (size_t)a.groups * 1024 + N * sizeof(float) +
+                        sizeof(QgBars);
+    const size_t image = (size_t)xt * a.jobs * kSlot, powers = (size_t)xt * N * sizeof(float);
+    uint8_t* work = nullptr;
+    CUDA_CHECK(cudaMallocAsync((void**)&work, image + powers + (parts > 1 ? (size_t)parts * a.m * a.w.rows * sizeof(float) : 0), st));
+    a.image = work;
+    a.powers = reinterpret_cast<float*>(work + image);
+    a.parts = parts > 1 ? reinterpret_cast<float*>(work + image + powers) : nullptr;
     try {
         client_smem<k_q4_gemm<N, KC, kPieces>>(cx);
         k_q4_pack<N, KC, XT><<<xt * N, 128, 0, st>>>(a);
         CUDA_CHECK(cudaGetLastError());
-        launch_pdl(cx, k_q4_gemm<N, KC, kPieces>, dim3((a.w.rows + a.block_rows - 1) / a.block_rows, xt), dim3(kQgThreads), smem, st, a,
-                   cx.d_err);
+        launch_pdl(cx, k_q4_gemm<N, KC, kPieces>, dim3((a.w.rows + a.block_rows - 1) / a.block_rows, xt, parts), dim3(kQgThreads),
+                   smem, st, a, cx.d_err);
+        cx.launches += 2;
+        if (parts > 1) {
+            const dim3 grid((unsigned)std::min<long long>(592, ((long long)a.m * a.w.rows + 255) / 256));
+            const auto sum = [&](auto* out) {
+                using T = typename std::remove_pointer<decltype(out)>::type;
+                launch_pdl(cx, k_q4_sum<T>, grid, dim3(256), 0, st, a.parts, parts, a.m, a.w.rows, out, a.ldo);
+            };
+            if (a.ot == FHE_F32) sum(static_cast<float*>(a.out));
+            else if (a.ot == FHE_F16) sum(static_cast<__half*>(a.out));
+            else sum(static_cast<__nv_bfloat16*>(a.out));
+            cx.launches++;
+        }
     } catch (...) {
-        cudaFreeAsync(a.image, st);
+        cudaFreeAsync(work, st);
         throw;
     }
-    CUDA_CHECK(cudaFreeAsync(a.image, st));
-    cx.launches += 2;
+    CUDA_CHECK(cudaFreeAsync(work, st));
 }
 template <int N, class XT>
 static void q4_gemm_group(Context& cx, const QgArgs& a, cudaStream_t st) {
@@ -353,7 +378,7 @@ static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
     // bfloat16 15 and 18, 16 of bfloat16 26 and 18; on 4,096 x 1024, where k_q4_gemm's two launches weigh more, 16 take 7.7 and 9.
     const int pieces = a.m * a.terms;
     if (pieces > (a.w.rows >= 16384 ? 9 : 20)) {
-        const QgArgs q{a.w, a.x, a.m, a.ldx, a.out, a.ot, a.ldo, a.wide, 0, 0, 0, 0, 0, nullptr, nullptr};
+        const QgArgs q{a.w, a.x, a.m, a.ldx, a.out, a.ot, a.ldo, a.wide, 0, 0, 0, 0, 0, nullptr, 0, nullptr, nullptr};
         if (a.xt == FHE_F32) q4_gemm<float>(cx, q, st);
         else if (a.xt == FHE_F16) q4_gemm<__half>(cx, q, st);
         else q4_gemm<__nv_bfloat16>(cx, q, st);

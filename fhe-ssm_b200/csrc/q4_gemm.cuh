@@ -55,6 +55,8 @@ struct QgArgs {
     int slots;        // jobs of a range
     int jobs;         // jobs of all columns, 128 each
     int groups;       // most groups that a range meets
+    int part_jobs;    // jobs of a part (blockIdx.z)
+    float* parts;     // [part][row of x][table row], or null: one part, which writes the output
     int run;          // chunks that one accumulator takes before the scale is applied
     uint8_t* image;   // x's operand [tile of N rows][chunk][piece], then the rows' powers
     float* powers;    // 2^p, by which the rows' sums are multiplied
@@ -255,8 +257,10 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row0 = blockIdx.x * a.block_rows, row1 = min(a.w.rows, row0 + a.block_rows), tiles = (row1 - row0 + 127) / 128;
     const int x0 = blockIdx.y * N;
-    const int ranges = (a.jobs + a.slots - 1) / a.slots;
-    const auto range_jobs = [&](int kr) { return min(a.slots, a.jobs - kr * a.slots); };
+    const int job0 = blockIdx.z * a.part_jobs, all_jobs = min(a.part_jobs, a.jobs - job0);
+    const int ranges = (all_jobs + a.slots - 1) / a.slots;
+    const auto range_jobs = [&](int kr) { return min(a.slots, all_jobs - kr * a.slots); };
+    if (a.parts) pdl_trigger();   // k_q4_sum, which waits for this kernel
     // tensor memory: the tiles' sums (several ranges only), accumulators, operands.  Two or four operand slots: a slot is
     // always filled by the same of the two groups, which so cannot get more than the one phase that a parity tells ahead of it.
     const uint32_t dcol = ranges > 1 ? tiles * N : 0, nd = min((uint32_t)kQgDMax, (384 - dcol) / N), acol = dcol + nd * N;
@@ -290,7 +294,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
             const int drains = range_jobs(kr) * kItems / a.run;
             for (int b = 0; b < tiles; b++, tile++) {
                 const int row = row0 + b * 128 + (warp & 3) * 32 + lane;
-                int left = per_group - kr * a.slots * kItems / a.run % per_group;
+                int left = per_group - (job0 + kr * a.slots) * kItems / a.run % per_group;
                 const float* sp = scales + (tile & 1) * a.groups * 128 + (warp & 3) * 32 + lane;
                 qg_wait(&bars->s_full[tile & 1], tile >> 1 & 1, bars);
                 uint64_t acc2[kC / 2];
@@ -341,20 +345,21 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                     acc[j] *= p.x, acc[j + 1] *= p.y, acc[j + 2] *= p.z, acc[j + 3] *= p.w;
                 }
                 if (row >= row1) continue;
-                const auto store = [&](auto* out) {
-                    out += r0 * a.ldo + row;
+                const auto store = [&](auto* out, long long ldo) {
+                    out += r0 * ldo + row;
                     if (nr >= kC) {
 #pragma unroll
-                        for (int j = 0; j < kC; j++, out += a.ldo) qg_store(out, acc[j]);
+                        for (int j = 0; j < kC; j++, out += ldo) qg_store(out, acc[j]);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < kC; j++, out += a.ldo)
+                        for (int j = 0; j < kC; j++, out += ldo)
                             if (j < nr) qg_store(out, acc[j]);
                     }
                 };
-                if (a.ot == FHE_F32) store(static_cast<float*>(a.out));
-                else if (a.ot == FHE_F16) store(static_cast<__half*>(a.out));
-                else store(static_cast<__nv_bfloat16*>(a.out));
+                if (a.parts) store(a.parts + (long long)blockIdx.z * a.m * a.w.rows, a.w.rows);
+                else if (a.ot == FHE_F32) store(static_cast<float*>(a.out), a.ldo);
+                else if (a.ot == FHE_F16) store(static_cast<__half*>(a.out), a.ldo);
+                else store(static_cast<__nv_bfloat16*>(a.out), a.ldo);
             }
         }
     } else if (warp < 16) {
@@ -362,11 +367,11 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         const int grp = (warp >> 2) - 2, t = tid & 127;
         uint8_t* my = ring + grp * kQgStages * kQgStageBytes;
         const int units = (a.w.cols + 31) / 32;   // 16-byte units of a row
-        const int jobs = tiles * a.jobs;
+        const int jobs = tiles * all_jobs;
         // the job to fetch next; a thread copies the same 16-byte unit of 4 rows
         int fkr = 0, fb = 0, fc = grp, fn = range_jobs(0), fat = 0;
         const long long ld32 = 32 * a.w.ldq;
-        const uint8_t* fsrc = a.w.q + (row0 + (t >> 2)) * a.w.ldq + (t & 3) * 16;
+        const uint8_t* fsrc = a.w.q + (row0 + (t >> 2)) * a.w.ldq + job0 * 64 + (t & 3) * 16;
         const uint32_t fdst = tc_smem(my) + (t >> 2) * 64 + (((t & 3) ^ (t >> 3 & 3)) << 4);
         const auto fetch = [&]() {
             while (fc >= fn) {
@@ -381,7 +386,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                     fn = 1 << 30;   // no more
                 }
             }
-            if (fkr < ranges && (fkr * a.slots + fc) * 4 + (t & 3) < units) {
+            if (fkr < ranges && (job0 + fkr * a.slots + fc) * 4 + (t & 3) < units) {
                 const uint8_t* src = fsrc + fc * 64;
                 const int row = row0 + fb * 128 + (t >> 2);
 #pragma unroll
@@ -491,8 +496,8 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         __syncwarp();
         if (lane == 0) {
             qg_arrive(&bars->p_full);
-            const uint8_t* src = a.image + (size_t)blockIdx.y * a.jobs * kSlotBytes;
-            for (int ch = 0, c = 0, kr = 0; ch < a.jobs; ch++) {
+            const uint8_t* src = a.image + ((size_t)blockIdx.y * a.jobs + job0) * kSlotBytes;
+            for (int ch = 0, c = 0, kr = 0; ch < all_jobs; ch++) {
                 if (kr) qg_wait(&bars->x_empty[c], (kr - 1) & 1, bars);
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(&bars->x_full[c])), "r"(kSlotBytes)
                              : "memory");
@@ -515,7 +520,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
             // whole 16-byte loads: the range's first group and the row's last one have to lie on their bounds
             const bool wide = (a.w.lds | groups) % kPer == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0;
             for (int kr = 0; kr < ranges; kr++) {
-                const int first = kr * a.slots * 128 / a.w.group;
+                const int first = (job0 + kr * a.slots) * 128 / a.w.group;
                 for (int b = 0; b < tiles; b++, tile++) {
                     float* to = scales + (tile & 1) * a.groups * 128 + t;
                     const S* p0 = src + min(row0 + b * 128 + t, a.w.rows - 1) * a.w.lds + first;
@@ -562,5 +567,19 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
     if (warp == 16) {
         asm volatile("tcgen05.fence::after_thread_sync;");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512));
+    }
+}
+
+// out = the parts' sum, in their order
+template <class T>
+__global__ void __launch_bounds__(256) k_q4_sum(const float* __restrict__ parts, int n, int m, int rows, T* __restrict__ out,
+                                                long long ldo) {
+    pdl_wait();
+    const long long each = (long long)m * rows;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < each; i += gridDim.x * 256ll) {
+        float v = 0.f;
+#pragma unroll 4
+        for (int z = 0; z < n; z++) v += parts[z * each + i];
+        qg_store(out + i / rows * ldo + i % rows, v);
     }
 }
