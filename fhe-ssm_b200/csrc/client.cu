@@ -58,7 +58,6 @@ constexpr int kQ4Stages = 4;
 constexpr int kQ4Pitch = kQ4Stage * 16 + 16;   // bytes of a row in a stage: 20 banks apart, 8 rows x 4 words meet all 32
 constexpr int kQ4StageBytes = 16 * kQ4Pitch;
 constexpr int kQ4RingBytes = kQ4Warps * kQ4Stages * kQ4StageBytes;
-constexpr int kQ4MaxBytes = 163840;     // shared memory for x's pieces and the scales
 
 struct Q4Args {
     fhe_q4 w;
@@ -282,15 +281,17 @@ static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
     a.per = NT * 8 / a.terms;
     a.ks_log2 = 0;
     while (a.ks_log2 < 3 && (tiles << a.ks_log2) < 148 * 8 && chunks >= (4 << a.ks_log2) * kQ4Stage) a.ks_log2++;
-    const int step = kQ4Stage << a.ks_log2;
-    // as many columns at a time as fit: 512 bytes a chunk and tile of pieces, 512 a chunk for the scales of 8 warps' rows
-    a.kb_chunks = std::min((chunks + step - 1) / step * step, kQ4MaxBytes / (512 * (NT + 1)) / step * step);
+    // As many columns at a time as fit (512 bytes a chunk and tile of pieces, 512 a scale for 8 warps' rows), in equal blocks.  Two
+    // blocks an SM where there are as many: one row on 16,384 x 4096 takes 18.1 us by 2,048 columns, 21.9 by all of them.
+    const int each = kQ4Warps >> a.ks_log2, grid = (tiles + each - 1) / each;
+    const int step = kQ4Stage << a.ks_log2, room = (grid > 148 ? 114688 : 212992) - kQ4RingBytes;
+    const int fit = std::max(step, room / (512 * NT + 512 / P) / step * step), turns = (chunks + fit - 1) / fit;
+    a.kb_chunks = ((chunks + turns - 1) / turns + step - 1) / step * step;
     a.units = (a.kb_chunks >> a.ks_log2) / P;
     a.group_magic = gpc == 1 ? 0u : (uint32_t)(((1ull << 32) + gpc - 1) / gpc);
     const size_t smem = kQ4RingBytes + (size_t)a.kb_chunks * NT * 512 + (size_t)a.units * kQ4Warps * 64;
     if (smem > 48 * 1024) client_smem<k_q4_mma<NT, P>>(cx);
-    const int each = kQ4Warps >> a.ks_log2;
-    k_q4_mma<NT, P><<<dim3((tiles + each - 1) / each, (a.m + a.per - 1) / a.per), kQ4Threads, smem, st>>>(a);
+    k_q4_mma<NT, P><<<dim3(grid, (a.m + a.per - 1) / a.per), kQ4Threads, smem, st>>>(a);
     CUDA_CHECK(cudaGetLastError());
     cx.launches++;
 }
@@ -374,10 +375,13 @@ static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
     const long long row = a.ldx * (a.xt == FHE_F32 ? 4 : 2);
     a.wide = (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(a.m > 1 ? row : 0)) % 16 == 0;
     a.terms = a.xt == FHE_F32 ? 3 : a.xt == FHE_F16 ? 2 : 1;
-    // By the columns of pieces.  On 50,304 x 1024: 9 columns (3 float32 rows) take 18.5 us by k_q4_mma and 18.5 by k_q4_gemm, 8 of
-    // bfloat16 15 and 18, 16 of bfloat16 26 and 18; on 4,096 x 1024, where k_q4_gemm's two launches weigh more, 16 take 7.7 and 9.
+    // By the columns of pieces; k_q4_mma grows with them, k_q4_gemm hardly does.  bfloat16 rows, us by k_q4_mma and k_q4_gemm:
+    //     4,096 x 1024    8: 5.5, 9.0    16: 7.6, 9.0    24: 9.9, 9.6      16,384 x 1024   8: 7.9, 9.2    12: 9.9, 9.3
+    //     1,024 x 2048    4: 5.8, 7.2     8: 7.2, 7.2    12: 8.9, 7.2      50,304 x 1024   8: 15.4, 18.0  12: 23.1, 18.0
+    //     1,024 x 4096    4: 8.2, 9.2     6: 9.6, 9.2    12: 19.9, 9.3     16,384 x 4096   1: 18.0, 22.1   4: 20.3, 21.9   8: 24.0, 21.9
     const int pieces = a.m * a.terms;
-    if (pieces > (a.w.rows >= 16384 ? 9 : 20)) {
+    const int most = a.w.cols < 1536 ? (a.w.rows < 16384 ? 18 : 9) : a.w.rows > 9472 && a.w.cols >= 2560 ? (a.w.group % 64 ? 14 : 5) : 7;
+    if (pieces > most) {
         const QgArgs q{a.w, a.x, a.m, a.ldx, a.out, a.ot, a.ldo, a.wide, 0, 0, 0, 0, 0, nullptr, 0, nullptr, nullptr};
         if (a.xt == FHE_F32) q4_gemm<float>(cx, q, st);
         else if (a.xt == FHE_F16) q4_gemm<__half>(cx, q, st);
