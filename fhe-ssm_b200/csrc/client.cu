@@ -282,7 +282,7 @@ static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
     a.ks_log2 = 0;
     while (a.ks_log2 < 3 && (tiles << a.ks_log2) < 148 * 8 && chunks >= (4 << a.ks_log2) * kQ4Stage) a.ks_log2++;
     // As many columns at a time as fit (512 bytes a chunk and tile of pieces, 512 a scale for 8 warps' rows), in equal blocks.  Two
-    // blocks an SM where there are as many: one row on 16,384 x 4096 takes 18.1 us by 2,048 columns, 21.9 by all of them.
+    // blocks an SM where there are as many: one row on 16,384 x 4,096 takes 17.5 us by 2,048 columns, 21.9 by all of them.
     const int each = kQ4Warps >> a.ks_log2, grid = (tiles + each - 1) / each;
     const int step = kQ4Stage << a.ks_log2, room = (grid > 148 ? 114688 : 212992) - kQ4RingBytes;
     const int fit = std::max(step, room / (512 * NT + 512 / P) / step * step), turns = (chunks + fit - 1) / fit;
@@ -314,7 +314,7 @@ static void q4_gemm_launch(Context& cx, QgArgs a, cudaStream_t st) {
     a.jobs = (a.w.cols + 127) / 128;
     a.part_jobs = a.jobs;
     // A short table of many columns: whole tiles, the columns in parts.  A job takes 0.5 us of a block, the sum of the parts a
-    // launch: 64 float16 rows on 1,005 x 3,829 take NN us in one part and NN in 15, on 4,096 x 1,024 (8 jobs) no less than before.
+    // launch: 64 float16 rows on 1,005 x 3,829 take 31.6 us in one part and 12.4 in 15.
     const int tiles = (a.w.rows + 127) / 128;
     if ((long long)tiles * xt * 2 <= 148 && a.jobs >= 12) {
         a.block_rows = 128;
@@ -375,12 +375,17 @@ static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
     const long long row = a.ldx * (a.xt == FHE_F32 ? 4 : 2);
     a.wide = (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(a.m > 1 ? row : 0)) % 16 == 0;
     a.terms = a.xt == FHE_F32 ? 3 : a.xt == FHE_F16 ? 2 : 1;
-    // By the columns of pieces; k_q4_mma grows with them, k_q4_gemm hardly does.  bfloat16 rows, us by k_q4_mma and k_q4_gemm:
-    //     4,096 x 1024    8: 5.5, 9.0    16: 7.6, 9.0    24: 9.9, 9.6      16,384 x 1024   8: 7.9, 9.2    12: 9.9, 9.3
-    //     1,024 x 2048    4: 5.8, 7.2     8: 7.2, 7.2    12: 8.9, 7.2      50,304 x 1024   8: 15.4, 18.0  12: 23.1, 18.0
-    //     1,024 x 4096    4: 8.2, 9.2     6: 9.6, 9.2    12: 19.9, 9.3     16,384 x 4096   1: 18.0, 22.1   4: 20.3, 21.9   8: 24.0, 21.9
+    // By the columns of pieces, with which k_q4_mma grows and k_q4_gemm hardly does.  bfloat16 rows, us by k_q4_mma and k_q4_gemm:
+    //      4,096 x 1,024               8: 5.5,  8.9   18: 8.6,  9.6   20: 9.3,  9.6
+    //     50,304 x 1,024               8: 15.4, 17.8  10: 22.0, 18.1          32,768 x 2,048   8: 19.8, 22.2  10: 24.3, 22.1
+    //     16,384 x 4,096               5: 21.6, 21.9   8: 24.0, 22.0           1,024 x 4,096   5: 8.9,  9.3    8: 11.2, 9.3
+    //     25,000 x 4,096               8: 35.7, 36.4  10: 46.9, 36.4
+    //     32,768 x 2,048, groups of 32 14: 29.4, 29.7 16: 30.8, 29.8          20,159 x 3,008  14: 42.1, 44.5  18: 50.6, 47.2
     const int pieces = a.m * a.terms;
-    const int most = a.w.cols < 1536 ? (a.w.rows < 16384 ? 18 : 9) : a.w.rows > 9472 && a.w.cols >= 2560 ? (a.w.group % 64 ? 14 : 5) : 7;
+    const int most = a.w.rows < 16384 && a.w.cols < 1536    ? 18
+                     : a.w.rows > 16384 && a.w.group % 64 != 0 ? 14
+                     : a.w.rows <= 16384 && a.w.cols > 3584 ? 5
+                                                            : 8;
     if (pieces > most) {
         const QgArgs q{a.w, a.x, a.m, a.ldx, a.out, a.ot, a.ldo, a.wide, 0, 0, 0, 0, 0, nullptr, 0, nullptr, nullptr};
         if (a.xt == FHE_F32) q4_gemm<float>(cx, q, st);
