@@ -73,6 +73,7 @@ struct Q4Args {
     int units;       // scales that a warp holds for each row
     uint32_t group_magic;   // chunk / (chunks of a group) = chunk * magic >> 32 (both at most 2^15); 0: a group is a chunk
     int wide;        // rows of x start on 16-byte boundaries
+    int scale_vec;   // a unit is a group, and rows of scales start on 16-byte boundaries
 };
 
 // The first bf16 piece of v (its bits), and what is left of v: pieces are cut, not rounded, so none overflows; an infinity or
@@ -109,6 +110,21 @@ __device__ __forceinline__ void q4_cut(const Q4Args& a, uint4* xs, int nt, int r
         if (ch >= kb1 - kb0) continue;
         const int k = (kb0 + ch) * 32 + t * 8;
         const T* src = static_cast<const T*>(a.x) + (r0 + r) * a.ldx + k;
+        if constexpr (TERMS == 1) {   // bfloat16 is its own piece
+            const uint16_t* bits = reinterpret_cast<const uint16_t*>(src);
+            uint4 u;
+            if (a.wide && k + 8 <= a.w.cols) u = *reinterpret_cast<const uint4*>(bits);
+            else {
+                uint32_t p[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) p[j] = k + j < a.w.cols ? bits[j] : 0;
+                u = make_uint4(p[0] | p[1] << 16, p[2] | p[3] << 16, p[4] | p[5] << 16, p[6] | p[7] << 16);
+            }
+            xs[(ch * nt + (r >> 3)) * 32 + (r & 7) * 4 + t] =
+                make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
+                           __byte_perm(u.y, u.w, 0x7632));
+            continue;
+        }
         float v[8];
         if (a.wide && k + 8 <= a.w.cols) {
             T u[8];
@@ -153,16 +169,39 @@ __device__ __forceinline__ void q4_mma(float* d, const float* c, uint32_t a0, ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Scales of 16 rows (from row0) for `units` units of P chunks from chunk c0 -> sc[unit][row]; 0 past the last column
+// Scales of 16 rows for `units` units of P chunks from chunk c0 -> sc[unit][row]; 0 past the last column.  src: the lane's row.
+// Where a unit is a group and rows start on 16-byte boundaries, 16 bytes at a time: a load of single scales meets 16 rows'
+// lines, and eight such loads a warp cost 128 of the L1's steps instead of 16.  `first`: the lane's first 16 bytes, asked for
+// before x's pieces were cut, so that the two round trips are one.
 template <class S, int P>
-__device__ __forceinline__ void q4_scales(const fhe_q4& w, uint32_t magic, float* sc, int row0, int c0, int units,
-                                          int chunks) {
-    const int lane = threadIdx.x & 31;
-    const S* src = static_cast<const S*>(w.scale) + (long long)min(row0 + (lane & 15), w.rows - 1) * w.lds;
+__device__ __forceinline__ void q4_scales(const Q4Args& a, const void* row, uint4 first, float* sc, int c0, int units, int chunks) {
+    const int lane = threadIdx.x & 31, half = lane >> 4;
+    const S* src = static_cast<const S*>(row);
+    sc += lane & 15;
+    if (a.scale_vec) {
+        constexpr int V = 16 / sizeof(S);
+        const int at = c0 / P, end = (chunks + P - 1) / P;
+        uint4 q = first;
+        const int e0 = (at & ~(V - 1)) + half * V;
+        for (int e = e0; e < at + units; e += 2 * V) {
+            S v[V];
+            if (e + V <= end) {
+                if (e != e0) q = *reinterpret_cast<const uint4*>(src + e);
+                *reinterpret_cast<uint4*>(v) = q;
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j++) v[j] = e + j < end ? src[e + j] : S(0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (e + j >= at && e + j < at + units) sc[(e + j - at) * 16] = q4_float(v[j]);
+        }
+        return;
+    }
 #pragma unroll 4
-    for (int u = lane >> 4; u < units; u += 2) {
+    for (int u = half; u < units; u += 2) {
         const int ch = c0 + u * P;
-        sc[u * 16 + (lane & 15)] = ch < chunks ? q4_float(src[magic ? __umulhi(ch, magic) : ch]) : 0.f;
+        sc[u * 16] = ch < chunks ? q4_float(src[a.group_magic ? __umulhi(ch, a.group_magic) : ch]) : 0.f;
     }
 }
 
@@ -176,7 +215,7 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
     const int chunks = (a.w.cols + 31) / 32;
     const int ks = 1 << a.ks_log2, rows = 16 * kQ4Warps >> a.ks_log2;   // warps on a tile, table rows of a block
     const int row0 = blockIdx.x * rows + (warp >> a.ks_log2) * 16, kq = warp & (ks - 1);
-    const int r0 = blockIdx.y * a.per, mr = min(a.per, a.m - r0);
+    const int r0 = blockIdx.y * a.per, mr = min(a.per, a.m - r0), scale_bytes = a.w.scale_type == FHE_F32 ? 4 : 2;
     float* sc = reinterpret_cast<float*>(xs + a.kb_chunks * NT * 32) + warp * 16 * a.units;   // [unit][16 rows]
     float acc[NT][4];
 #pragma unroll
@@ -205,13 +244,19 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
         };
 #pragma unroll
         for (int s = 0; s < kQ4Stages - 1; s++) fetch(s);
-        if (a.w.scale_type == FHE_F16) q4_scales<__half, P>(a.w, a.group_magic, sc, row0, c0, (c1 - c0) / P, chunks);
-        else if (a.w.scale_type == FHE_BF16) q4_scales<__nv_bfloat16, P>(a.w, a.group_magic, sc, row0, c0, (c1 - c0) / P, chunks);
-        else q4_scales<float, P>(a.w, a.group_magic, sc, row0, c0, (c1 - c0) / P, chunks);
+        const char* srow = static_cast<const char*>(a.w.scale) + min(row0 + (lane & 15), a.w.rows - 1) * a.w.lds * scale_bytes;
+        uint4 first = make_uint4(0, 0, 0, 0);
+        if (a.scale_vec) {
+            const int v = 16 / scale_bytes, e = (c0 / P & ~(v - 1)) + (lane >> 4) * v;
+            if (e + v <= (chunks + P - 1) / P) first = *reinterpret_cast<const uint4*>(srow + (size_t)e * scale_bytes);
+        }
         __syncthreads();   // the previous block's pieces are read
         if (a.xt == FHE_F32) q4_cut<float, 3>(a, xs, NT, r0, mr, kb0, kb1);
         else if (a.xt == FHE_F16) q4_cut<__half, 2>(a, xs, NT, r0, mr, kb0, kb1);
         else q4_cut<__nv_bfloat16, 1>(a, xs, NT, r0, mr, kb0, kb1);
+        if (a.w.scale_type == FHE_F16) q4_scales<__half, P>(a, srow, first, sc, c0, (c1 - c0) / P, chunks);
+        else if (a.w.scale_type == FHE_BF16) q4_scales<__nv_bfloat16, P>(a, srow, first, sc, c0, (c1 - c0) / P, chunks);
+        else q4_scales<float, P>(a, srow, first, sc, c0, (c1 - c0) / P, chunks);
         __syncthreads();
         const uint4* xc = xs + (size_t)(c0 - kb0) * NT * 32 + lane;
         const float* su = sc + g;
@@ -288,6 +333,7 @@ static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
     const int fit = std::max(step, room / (512 * NT + 512 / P) / step * step), turns = (chunks + fit - 1) / fit;
     a.kb_chunks = ((chunks + turns - 1) / turns + step - 1) / step * step;
     a.units = (a.kb_chunks >> a.ks_log2) / P;
+    a.scale_vec = gpc == P && (reinterpret_cast<uintptr_t>(a.w.scale) | (uintptr_t)a.w.lds * (a.w.scale_type == FHE_F32 ? 4 : 2)) % 16 == 0;
     a.group_magic = gpc == 1 ? 0u : (uint32_t)(((1ull << 32) + gpc - 1) / gpc);
     const size_t smem = kQ4RingBytes + (size_t)a.kb_chunks * NT * 512 + (size_t)a.units * kQ4Warps * 64;
     if (smem > 48 * 1024) client_smem<k_q4_mma<NT, P>>(cx);
@@ -1439,7 +1485,7 @@ extern "C" int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_
         client_ptr(cx->cx, x, xb, "x");
         client_ptr(cx->cx, out, ob, "out");
         cudaStream_t st = client_stream(cx, stream);
-        fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0, 0, 0, 0, 0, 0}, st);
+        fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0, 0, 0, 0, 0, 0, 0}, st);
     });
 }
 
