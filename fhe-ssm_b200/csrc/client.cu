@@ -207,7 +207,7 @@ __device__ __forceinline__ void q4_scales(const Q4Args& a, const void* row, uint
 
 // NT: tiles of 8 columns.  P: chunks after which the scale is applied, the largest of 1, 2, 4 that divides a group's.
 template <int NT, int P>
-__global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
+__global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const Q4Args a) {
     extern __shared__ __align__(16) uint8_t qsm[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t* ring = qsm + warp * (kQ4Stages * kQ4StageBytes);
@@ -260,6 +260,7 @@ __global__ void __launch_bounds__(kQ4Threads) k_q4_mma(const Q4Args a) {
         __syncthreads();
         const uint4* xc = xs + (size_t)(c0 - kb0) * NT * 32 + lane;
         const float* su = sc + g;
+#pragma unroll 4
         for (int s = 0; s < stages; s++) {
             fetch(s + kQ4Stages - 1);
             asm volatile("cp.async.wait_group %0;" ::"n"(kQ4Stages - 1) : "memory");
