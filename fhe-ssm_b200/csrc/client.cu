@@ -328,7 +328,7 @@ static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
     a.ks_log2 = 0;
     while (a.ks_log2 < 3 && (tiles << a.ks_log2) < 148 * 8 && chunks >= (4 << a.ks_log2) * kQ4Stage) a.ks_log2++;
     // As many columns at a time as fit (512 bytes a chunk and tile of pieces, 512 a scale for 8 warps' rows), in equal blocks.  Two
-    // blocks an SM where there are as many: one row on 16,384 x 4,096 takes 17.5 us by 2,048 columns, 21.9 by all of them.
+    // blocks an SM where there are as many: one row on 16,384 x 4,096 took 18.1 us by 2,048 columns, 21.9 by all of them.
     const int each = kQ4Warps >> a.ks_log2, grid = (tiles + each - 1) / each;
     const int step = kQ4Stage << a.ks_log2, room = (grid > 148 ? 114688 : 212992) - kQ4RingBytes;
     const int fit = std::max(step, room / (512 * NT + 512 / P) / step * step), turns = (chunks + fit - 1) / fit;
@@ -422,17 +422,14 @@ static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
     const long long row = a.ldx * (a.xt == FHE_F32 ? 4 : 2);
     a.wide = (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(a.m > 1 ? row : 0)) % 16 == 0;
     a.terms = a.xt == FHE_F32 ? 3 : a.xt == FHE_F16 ? 2 : 1;
-    // By the columns of pieces, with which k_q4_mma grows and k_q4_gemm hardly does.  bfloat16 rows, us by k_q4_mma and k_q4_gemm:
-    //      4,096 x 1,024               8: 5.5,  8.9   18: 8.6,  9.6   20: 9.3,  9.6
-    //     50,304 x 1,024               8: 15.4, 17.8  10: 22.0, 18.1          32,768 x 2,048   8: 19.8, 22.2  10: 24.3, 22.1
-    //     16,384 x 4,096               5: 21.6, 21.9   8: 24.0, 22.0           1,024 x 4,096   5: 8.9,  9.3    8: 11.2, 9.3
-    //     25,000 x 4,096               8: 35.7, 36.4  10: 46.9, 36.4
-    //     32,768 x 2,048, groups of 32 14: 29.4, 29.7 16: 30.8, 29.8          20,159 x 3,008  14: 42.1, 44.5  18: 50.6, 47.2
+    // By the columns of pieces, with which k_q4_mma grows (by tiles of 8 above all) and k_q4_gemm hardly does.  bfloat16 rows, us by
+    // k_q4_mma and k_q4_gemm:
+    //     50,304 x 1,024   8: 14.4, 17.8   9: 19.2, 18.1      16,384 x 4,096    8: 21.2, 22.0  10: 33.5, 21.9
+    //     32,768 x 2,048   8: 18.5, 22.2  10: 21.6, 22.1       1,024 x 4,096    8:  9.2,  9.3  10: 13.3, 9.3
+    // a small table, where k_q4_gemm's two launches weigh more, and groups of 32, where it adds up every 32 columns, on a long one:
+    //      4,096 x 1,024  18:  8.2,  9.6      32,768 x 2,048, groups of 32  18: 30.9, 31.7  20: 32.2, 31.6
     const int pieces = a.m * a.terms;
-    const int most = a.w.rows < 16384 && a.w.cols < 1536    ? 18
-                     : a.w.rows > 16384 && a.w.group % 64 != 0 ? 14
-                     : a.w.rows <= 16384 && a.w.cols > 3584 ? 5
-                                                            : 8;
+    const int most = (a.w.rows < 16384 && a.w.cols < 1536) || (a.w.rows > 16384 && a.w.group % 64) ? 18 : 8;
     if (pieces > most) {
         const QgArgs q{a.w, a.x, a.m, a.ldx, a.out, a.ot, a.ldo, a.wide, 0, 0, 0, 0, 0, nullptr, 0, nullptr, nullptr};
         if (a.xt == FHE_F32) q4_gemm<float>(cx, q, st);
