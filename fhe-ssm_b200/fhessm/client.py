@@ -158,7 +158,7 @@ def _out(out, like, m, n, dtype, device):
 
 def q4_matvec(cx, x, table, *, dtype=torch.float32, out=None):
     """x (m, cols) times the table's transpose: (m, rows) of `dtype` (fhe_q4_matvec).  x: float32,
-    float16 or bfloat16 with contiguous rows (any row stride)."""
+    float16 or bfloat16 with contiguous rows (any row stride), 2^21 of them at most."""
     xt, m, k, ldx = _rows_of(x, "x")
     if k != table.cols:
         raise _bad(f"x has {k} columns, the table {table.cols}")

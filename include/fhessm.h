@@ -389,12 +389,13 @@ int fhe_keyswitch_noalloc(fhe_ctx* cx, uint64_t which, const uint64_t* d, int le
  * and the embedding row that is encrypted next (ml-eval/fhe_client.py:123-135).  Operands are device
  * memory of the context's GPU; rows are contiguous, ld* is the distance between rows in elements.
  * Calls are enqueued on `stream` (a cudaStream_t; NULL = the context's own stream,
- * cudaStreamLegacy / cudaStreamPerThread name those) and allocate nothing.  Operands that are
- * written must not overlap the others.  m = 0 rows is a valid call that does nothing. */
+ * cudaStreamLegacy / cudaStreamPerThread name those).  Operands that are written must not overlap the
+ * others.  m = 0 rows is a valid call that does nothing. */
 #define FHE_F32 0
 #define FHE_F16 1
 #define FHE_BF16 2
 #define FHE_Q4_MAX_COLS (1 << 20)
+#define FHE_Q4_MAX_M (1 << 21)
 /* a table of rows x cols values in 4 bits: value (i, c) = scale[i * lds + c / group] * (q - 8), q the
  * low (even c) or high (odd c) half of byte q[i * ldq + c / 2].  Rows start on 16-byte boundaries and
  * are padded to a multiple of 16 bytes (32 columns; the padding's content does not matter); ldq is
@@ -406,8 +407,11 @@ typedef struct {
     int rows, cols, group;
     long long ldq, lds;
 } fhe_q4;
-/* out[r][i] = sum_c x[r][c] W[i][c] for m rows of x (the head: W is vocabulary x d).  Sums are held in
- * 32 bits and rounded once to the output's type. */
+/* out[r][i] = sum_c x[r][c] W[i][c] for m rows of x, at most FHE_Q4_MAX_M (the head: W is vocabulary x d).
+ * Sums are held in 32 bits and rounded once to the output's type.  One row or a few take one launch.  For more, x's
+ * operand (about 4 m cols bytes) is laid out in memory that the call takes from the stream's pool and gives back to
+ * it (cudaMallocAsync); float32 values are then held to 22 bits, and values under 2^-16 of their row's largest, float16's
+ * aside, to 2^-39 of it. */
 int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_type, long long ldx, int m, void* out,
                   int out_type, long long ldo, void* stream);
 /* out[r] = row tokens[r] of the table; a token outside [0, rows) gives a row of zeros */

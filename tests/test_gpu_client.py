@@ -92,6 +92,26 @@ def test_matvec_strides(cx, m, xt):
     assert torch.equal(client.q4_matvec(cx, x, t2), out)
 
 
+@pytest.mark.parametrize("m", [1, 7, 20])
+@pytest.mark.parametrize("st", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols,group", [(40, 5000, 64), (2500, 1000, 32), (70, 1300, 128), (33, 4097, 32), (1300, 999, 96)])
+def test_matvec_scale_rows(cx, rows, cols, group, st, m):
+    """Scales whose rows start on 16-byte boundaries (contiguous or with gaps of noise) or on none: the same values."""
+    from fhessm import client
+    rng = np.random.default_rng(rows + m)
+    t, w = make_table(rng, rows, cols, group, st)
+    x = torch.from_numpy(rng.normal(0, 1, (m, cols)).astype(np.float32)).to(torch.bfloat16).cuda()
+    out = client.q4_matvec(cx, x, t)
+    check_product(out, x, w, "f32")
+    n = t.scale.shape[1]
+    for stride, at in [(-(-n // 8) * 8 + 8, 0), (-(-n // 8) * 8 + 8, 8), (n + 3 | 1, 1)]:
+        big = torch.full((rows, stride + 16), float("nan"), dtype=TYPES[st], device="cuda").flatten()
+        scale = big.as_strided((rows, n), (stride, 1), at)
+        scale.copy_(t.scale)
+        t2 = client.Q4Table(t.weight, scale, cols=cols, group=group)
+        assert torch.equal(client.q4_matvec(cx, x, t2), out)
+
+
 @pytest.mark.parametrize("m", [1, 5, 64])
 def test_matvec_large_and_small_values(cx, m):
     """float32 rows far outside the 16-bit types' range, and rows whose values span many powers of two."""
@@ -391,6 +411,11 @@ def test_refusals(cx):
         with pytest.raises(FheError):
             call()
     h = client._sigs()
+    many = torch.zeros((1 << 21) + 1, 32, dtype=torch.bfloat16, device="cuda")
+    small, _ = make_table(rng, 1, 32, 32)
+    with pytest.raises(FheError):
+        client.q4_matvec(cx, many, small)
+    assert (client.q4_matvec(cx, many[:1 << 21], small) == 0).all()
     host = np.zeros((2, 64), np.float32)
     out = torch.empty(2, 30, device="cuda")
     assert h.fhe_q4_matvec(cx.h, t.c, host.ctypes.data, 0, 64, 2, out.data_ptr(), 0, 30, None) == -1
