@@ -56,7 +56,7 @@ static void client_smem(const Context& cx) {
 // One bfloat16 row on 50,304 x 1,024 at groups of 64 takes 12.0 us (27.5 MB: 2.3 TB/s, 36% of a copy's rate), on 16,384 x 4,096
 // 15.9 us, on 4,096 x 1,024 4.1 us; 8 rows on 50,304 x 1,024 14.4 us.  About 3 us are the launch, x's pieces and the
 // scales, a round trip each; then the loop, which waits for the table's bytes 3% of its time: instructions bound it,
-// 56% of the issue slots and 51% of the integer pipe over the whole kernel (unpacking: 7 integer operations and 4 subtractions
+// 55% of the issue slots and 53% of the integer pipe over the whole kernel (unpacking: 7 integer operations and 4 subtractions
 // for 8 values), with the 24 warps an SM that the ring leaves room for.  More and smaller blocks cut x more often: 16,384 x
 // 4,096 by 4 warps a tile takes 20.5 us.
 constexpr int kQ4Warps = 8, kQ4Threads = 32 * kQ4Warps;
