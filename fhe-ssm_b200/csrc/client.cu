@@ -634,22 +634,47 @@ struct SampleRadix {
     uint64_t key[32], wt[32];
     uint64_t red[32], red2[32];
     uint64_t got, before, before2;
-    uint32_t n;
+    uint64_t mine;   // what a cluster's blocks show each other
+    uint32_t n, at_count;
     int at;
 };
 struct SampleFound {
     uint64_t key, sum;   // the last kept token's rank key, and the sum of the weights down to it
 };
 
+// f over the values of the cluster's blocks, in their order; the same in every thread.  v is the same in a block.
+template <class T, class F>
+__device__ T sample_cluster(T v, F f, SampleRadix& sh) {
+    static_assert(sizeof(T) <= sizeof(sh.mine), "");
+    auto cluster = cooperative_groups::this_cluster();
+    if (threadIdx.x == 0) *reinterpret_cast<T*>(&sh.mine) = v;
+    cluster.sync();
+    v = *reinterpret_cast<const T*>(&cluster.map_shared_rank(&sh, 0)->mine);
+    for (unsigned b = 1; b < cluster.num_blocks(); b++) v = f(v, *reinterpret_cast<const T*>(&cluster.map_shared_rank(&sh, b)->mine));
+    cluster.sync();
+    return v;
+}
+
 // The token, in rank order, at which the running count (BY_COUNT) or sum of weights reaches `want` (>= 1); key 0 and the whole
-// sum if none does.  each(f) calls f(rank key, e) for the calling thread's share of the tokens.
-template <bool BY_COUNT, class Each>
+// sum if none does.  each(f) calls f(rank key, e) for the calling thread's share of the tokens.  CLUSTER: the tokens are
+// those of all the cluster's blocks, which call it together and all get the answer.
+template <bool BY_COUNT, bool CLUSTER, class Each>
 __device__ SampleFound sample_select(SampleRadix& sh, uint64_t want, Each each) {
     const int tid = threadIdx.x;
+    const auto together = [] {
+        if constexpr (CLUSTER) cooperative_groups::this_cluster().sync();
+        else __syncthreads();
+    };
+    const auto smaller = [](uint64_t p, uint64_t q) { return min(p, q); };
+    const auto larger = [](uint64_t p, uint64_t q) { return max(p, q); };
     uint64_t lo = ~0ull, hi = 0, before = 0;
     each([&](uint64_t k, float) { lo = min(lo, k), hi = max(hi, k); });
-    lo = sample_reduce(lo, [](uint64_t p, uint64_t q) { return min(p, q); }, sh.red);
-    hi = sample_reduce(hi, [](uint64_t p, uint64_t q) { return max(p, q); }, sh.red);
+    lo = sample_reduce(lo, smaller, sh.red);
+    hi = sample_reduce(hi, larger, sh.red);
+    if constexpr (CLUSTER) {
+        lo = sample_cluster(lo, smaller, sh);
+        hi = sample_cluster(hi, larger, sh);
+    }
     if (hi == 0) return {0, 0};
     while (true) {
         // the tokens with keys in [lo, hi], in 1024 bins of equal width
@@ -664,30 +689,46 @@ __device__ SampleFound sample_select(SampleRadix& sh, uint64_t want, Each each) 
             atomicAdd(&sh.count[b], 1u);
             atomicAdd((unsigned long long*)&sh.sum[b], (unsigned long long)sample_weight(e));
         });
-        __syncthreads();
-        const uint64_t c = sh.count[tid], s = sh.sum[tid];
+        together();
+        uint64_t c = sh.count[tid], s = sh.sum[tid];
+        if constexpr (CLUSTER) {
+            auto cluster = cooperative_groups::this_cluster();
+            for (unsigned b = 0; b < cluster.num_blocks(); b++) {
+                if (b == cluster.block_rank()) continue;
+                const SampleRadix* other = cluster.map_shared_rank(&sh, b);
+                c += other->count[tid];
+                s += other->sum[tid];
+            }
+            cluster.sync();   // the bins are read
+        }
         const uint64_t sums = sample_block_scan(s, sh.red2);
         const uint64_t run = BY_COUNT ? sample_block_scan(c, sh.red) : sums, own = BY_COUNT ? c : s;
-        if (run >= want && run - own < want) sh.at = tid, sh.got = run - own, sh.before = before + sums - s;
+        if (run >= want && run - own < want) sh.at = tid, sh.at_count = c, sh.got = run - own, sh.before = before + sums - s;
         if (tid == kSampleRadix - 1) sh.before2 = before + sums;
         __syncthreads();
         const int at = sh.at;
         if (at < 0) return {0, sh.before2};
         want -= sh.got;
         before = sh.before;
-        const uint32_t n = sh.count[at];
+        const uint32_t n = sh.at_count;
         // the bin's own range of keys
         const uint64_t top = hi - ((uint64_t)at << shift), bottom = top - ((1ull << shift) - 1);
         lo = bottom > top ? lo : max(lo, bottom);
         hi = top;
         if (n <= 32) {
+            SampleRadix* list = &sh;   // the first block's
+            if constexpr (CLUSTER) list = cooperative_groups::this_cluster().map_shared_rank(&sh, 0);
             each([&](uint64_t k, float e) {
                 if (k < lo || k > hi) return;
-                const uint32_t j = atomicAdd(&sh.n, 1u);
-                sh.key[j] = k;
-                sh.wt[j] = sample_weight(e);
+                const uint32_t j = atomicAdd(&list->n, 1u);
+                list->key[j] = k;
+                list->wt[j] = sample_weight(e);
             });
-            __syncthreads();
+            together();
+            if constexpr (CLUSTER) {
+                if (list != &sh && tid < n) sh.key[tid] = list->key[tid], sh.wt[tid] = list->wt[tid];
+                together();
+            }
             if (tid < n) {
                 uint64_t c = 0, s = 0;
                 for (uint32_t l = 0; l < n; l++)
@@ -745,37 +786,44 @@ __device__ __forceinline__ float sample_logprob(const SampleRow& row, int i, uin
     return row.z(row.x(i)) - (float)log((double)total / (double)kSampleOne);
 }
 
-// Rows longer than a cluster's shared memory: one block per row, which reads the logits again for every step.
+// Rows longer than a cluster's shared memory: a cluster for each row, whose blocks read the logits again for every step.  A
+// step is a few hundred instructions a token, so one block for a row took 1.9 ms for 300,000 logits, eight take 0.28
 __global__ void __launch_bounds__(kSampleThreads) k_sample_long(const SampleArgs a) {
     __shared__ SampleRadix sh;
     __shared__ float redf[32];
-    const int r = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    auto cluster = cooperative_groups::this_cluster();
+    const int nb = cluster.num_blocks(), rank = cluster.block_rank(), r = blockIdx.x / nb;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, first = rank * kSampleThreads + tid, step = nb * kSampleThreads;
     const SampleSettings set(a, r);
     SampleRow row;
     row.set(a, r);
     float top = -INFINITY;
-    for (int i = tid; i < row.v; i += kSampleThreads) top = fmaxf(top, row.x(i));
-    top = sample_reduce(top, [](float x, float y) { return fmaxf(x, y); }, redf);
+    for (int i = first; i < row.v; i += step) top = fmaxf(top, row.x(i));
+    const auto larger = [](float x, float y) { return fmaxf(x, y); };
+    top = sample_cluster(sample_reduce(top, larger, redf), larger, sh);
     if (top == -INFINITY) {
-        if (tid == 0) a.token[r] = -1, a.logprob[r] = -INFINITY;
+        if (rank == 0 && tid == 0) a.token[r] = -1, a.logprob[r] = -INFINITY;
         return;
     }
     row.scale(top, set.t);
     auto each = [&](auto f) {
-        for (int i = tid; i < row.v; i += kSampleThreads) {
+        for (int i = first; i < row.v; i += step) {
             const float x = row.x(i);
             if (row.counts(x)) f(sample_rank_key(x, i), row.e(x));
         }
     };
     uint64_t bound = 0;
-    if (set.k) bound = sample_select<true>(sh, set.k, each).key;
+    if (set.k) bound = sample_select<true, true>(sh, set.k, each).key;
     if (set.p < 1.f) {
         uint64_t s = 0;
         each([&](uint64_t k, float e) { s += k >= bound ? sample_weight(e) : 0; });
-        s = sample_reduce(s, [](uint64_t x, uint64_t y) { return x + y; }, sh.red);
-        bound = max(bound, sample_select<false>(sh, set.limit(s), each).key);
+        const auto plus = [](uint64_t x, uint64_t y) { return x + y; };
+        s = sample_cluster(sample_reduce(s, plus, sh.red), plus, sh);
+        bound = max(bound, sample_select<false, true>(sh, set.limit(s), each).key);
     }
-    const int per = (row.v + kSampleWarps - 1) / kSampleWarps, i0 = min(row.v, warp * per), i1 = min(row.v, i0 + per);
+    // a stretch of the row for each of the cluster's warps, in order
+    const int warps = nb * kSampleWarps, per = (row.v + warps - 1) / warps;
+    const int i0 = min(row.v, (rank * kSampleWarps + warp) * per), i1 = min(row.v, i0 + per);
     auto kept = [&](int i) -> uint64_t {
         const float x = row.x(i);
         if (!row.counts(x) || sample_rank_key(x, i) < bound) return 0;
@@ -788,11 +836,19 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample_long(const SampleArgs
     __syncthreads();
     if (lane == 0) sh.red[warp] = mine;
     __syncthreads();
-    uint64_t total = 0, start = 0;
+    uint64_t own = 0, start = 0;
     for (int w = 0; w < kSampleWarps; w++) {
-        if (w == warp) start = total;
-        total += sh.red[w];
+        if (w == warp) start = own;
+        own += sh.red[w];
     }
+    if (tid == 0) sh.mine = own;
+    cluster.sync();
+    uint64_t total = 0;
+    for (int b = 0; b < nb; b++) {
+        if (b == rank) start += total;
+        total += cluster.map_shared_rank(&sh, b)->mine;
+    }
+    cluster.sync();   // a block leaves when the others have read it
     const uint64_t target = set.target(total);
     if (target < start || target >= start + mine) return;
     const int i = sample_walk(i0, i1, start, target, kept);
@@ -1326,8 +1382,8 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
                         if (row.counts(x)) f(sample_rank_key(x, i), row.e(x));
                     }
                 };
-                const SampleFound f = by_count ? sample_select<true>(sh.radix, want, each)
-                                               : sample_select<false>(sh.radix, want, each);
+                const SampleFound f = by_count ? sample_select<true, false>(sh.radix, want, each)
+                                               : sample_select<false, false>(sh.radix, want, each);
                 bound = f.key;
                 found = f.sum;
             }
@@ -1412,25 +1468,20 @@ static void sample(Context& cx, const SampleArgs& a, cudaStream_t st) {
     // blocks for every SM, each with 1024 logits at least; a row has to fit its cluster
     int nb = 1;
     while (nb < kSampleClusterMax && (nb * kSamplePart < a.vocab || (a.rows * nb * 2 <= 148 && a.vocab >= 2048 * nb))) nb *= 2;
-    if (nb * kSamplePart < a.vocab) {
-        k_sample_long<<<a.rows, kSampleThreads, 0, st>>>(a);
-        CUDA_CHECK(cudaGetLastError());
-    } else {
-        const size_t smem = sizeof(SampleShared) + (((size_t)a.vocab + nb - 1) / nb + 8 + 128) * sizeof(float);
-        client_smem<k_sample>(cx);
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)a.rows * nb);
-        cfg.blockDim = dim3(kSampleThreads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = st;
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = nb;
-        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-        CUDA_CHECK(cudaLaunchKernelEx(&cfg, k_sample, a));
-    }
+    const bool fits = a.vocab <= nb * kSamplePart;
+    if (fits) client_smem<k_sample>(cx);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.rows * nb);
+    cfg.blockDim = dim3(kSampleThreads);
+    cfg.dynamicSmemBytes = fits ? sizeof(SampleShared) + (((size_t)a.vocab + nb - 1) / nb + 8 + 128) * sizeof(float) : 0;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = nb;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    CUDA_CHECK(cudaLaunchKernelEx(&cfg, fits ? k_sample : k_sample_long, a));
     cx.launches++;
 }
 

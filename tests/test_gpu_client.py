@@ -261,6 +261,27 @@ def test_sample_long_rows(cx, xt):
             check_sample(cx, x, u, **kw)
 
 
+@pytest.mark.parametrize("vocab", [262145, 600000, 1 << 20])
+def test_sample_long_rows_of_ties_and_masks(cx, vocab):
+    """Rows longer than a cluster holds: all equal, a few values, only some allowed, one allowed, none allowed, and NaN."""
+    rng = np.random.default_rng(vocab)
+    x = np.full((6, vocab), -np.inf, np.float32)
+    x[0] = 3.0
+    x[1] = rng.integers(0, 4, vocab)
+    some = rng.choice(vocab, 700, replace=False)
+    x[2, some] = rng.normal(0, 1, 700)
+    x[3, vocab - 1] = -5.0
+    x[5] = rng.normal(0, 1, vocab)
+    x[5, ::2] = np.nan
+    x = torch.from_numpy(x).cuda()
+    u = torch.from_numpy(rng.uniform(0, 0.999, 6).astype(np.float32)).cuda()
+    for kw in (dict(), dict(k=1000), dict(k=40, p=0.5), dict(t=0.0), dict(p=0.3)):
+        token = check_sample(cx, x, u, **kw)
+        assert token[3] == vocab - 1 and token[4] == -1
+    k = torch.tensor([5, 1, 701, 7, 3, 0], dtype=torch.int32, device="cuda")
+    assert check_sample(cx, x, u, k=k)[0] < 5
+
+
 @pytest.mark.parametrize("xt", ["f32", "bf16"])
 @pytest.mark.parametrize("vocab", [6, 100, 2049, 5000, 70001])
 def test_sample_ties_by_index(cx, vocab, xt):
