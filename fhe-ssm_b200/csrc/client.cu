@@ -656,7 +656,7 @@ __device__ T sample_cluster(T v, F f, SampleRadix& sh) {
 }
 
 // The token, in rank order, at which the running count (BY_COUNT) or sum of weights reaches `want` (>= 1); key 0 and the whole
-// sum if none does.  each(f) calls f(rank key, e) for the calling thread's share of the tokens.  CLUSTER: the tokens are
+// sum if none does.  each(f) calls f(rank key, weight()) for the calling thread's share of the tokens.  CLUSTER: the tokens are
 // those of all the cluster's blocks, which call it together and all get the answer.
 template <bool BY_COUNT, bool CLUSTER, class Each>
 __device__ SampleFound sample_select(SampleRadix& sh, uint64_t want, Each each) {
@@ -668,7 +668,7 @@ __device__ SampleFound sample_select(SampleRadix& sh, uint64_t want, Each each) 
     const auto smaller = [](uint64_t p, uint64_t q) { return min(p, q); };
     const auto larger = [](uint64_t p, uint64_t q) { return max(p, q); };
     uint64_t lo = ~0ull, hi = 0, before = 0;
-    each([&](uint64_t k, float) { lo = min(lo, k), hi = max(hi, k); });
+    each([&](uint64_t k, auto) { lo = min(lo, k), hi = max(hi, k); });
     lo = sample_reduce(lo, smaller, sh.red);
     hi = sample_reduce(hi, larger, sh.red);
     if constexpr (CLUSTER) {
@@ -683,11 +683,11 @@ __device__ SampleFound sample_select(SampleRadix& sh, uint64_t want, Each each) 
         sh.count[tid] = 0;
         if (tid == 0) sh.at = -1, sh.n = 0;
         __syncthreads();
-        each([&](uint64_t k, float e) {
+        each([&](uint64_t k, auto weight) {
             if (k < lo || k > hi) return;
             const int b = (int)((hi - k) >> shift);
             atomicAdd(&sh.count[b], 1u);
-            atomicAdd((unsigned long long*)&sh.sum[b], (unsigned long long)sample_weight(e));
+            atomicAdd((unsigned long long*)&sh.sum[b], (unsigned long long)weight());
         });
         together();
         uint64_t c = sh.count[tid], s = sh.sum[tid];
@@ -718,11 +718,11 @@ __device__ SampleFound sample_select(SampleRadix& sh, uint64_t want, Each each) 
         if (n <= 32) {
             SampleRadix* list = &sh;   // the first block's
             if constexpr (CLUSTER) list = cooperative_groups::this_cluster().map_shared_rank(&sh, 0);
-            each([&](uint64_t k, float e) {
+            each([&](uint64_t k, auto weight) {
                 if (k < lo || k > hi) return;
                 const uint32_t j = atomicAdd(&list->n, 1u);
                 list->key[j] = k;
-                list->wt[j] = sample_weight(e);
+                list->wt[j] = weight();
             });
             together();
             if constexpr (CLUSTER) {
@@ -787,7 +787,7 @@ __device__ __forceinline__ float sample_logprob(const SampleRow& row, int i, uin
 }
 
 // Rows longer than a cluster's shared memory: a cluster for each row, whose blocks read the logits again for every step.  A
-// step is a few hundred instructions a token, so one block for a row took 1.9 ms for 300,000 logits, eight take 0.28
+// step is a few hundred instructions a token, so one block for a row took 1.9 ms for 300,000 logits, eight take 0.26
 __global__ void __launch_bounds__(kSampleThreads) k_sample_long(const SampleArgs a) {
     __shared__ SampleRadix sh;
     __shared__ float redf[32];
@@ -807,16 +807,20 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample_long(const SampleArgs
     }
     row.scale(top, set.t);
     auto each = [&](auto f) {
-        for (int i = first; i < row.v; i += step) {
-            const float x = row.x(i);
-            if (row.counts(x)) f(sample_rank_key(x, i), row.e(x));
+        for (int i = first; i < row.v; i += 4 * step) {   // four loads on their way
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = i + j * step < row.v ? row.x(i + j * step) : -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (row.counts(x[j])) f(sample_rank_key(x[j], i + j * step), [&] { return sample_weight(row.e(x[j])); });
         }
     };
     uint64_t bound = 0;
     if (set.k) bound = sample_select<true, true>(sh, set.k, each).key;
     if (set.p < 1.f) {
         uint64_t s = 0;
-        each([&](uint64_t k, float e) { s += k >= bound ? sample_weight(e) : 0; });
+        each([&](uint64_t k, auto weight) { s += k >= bound ? weight() : 0; });
         const auto plus = [](uint64_t x, uint64_t y) { return x + y; };
         s = sample_cluster(sample_reduce(s, plus, sh.red), plus, sh);
         bound = max(bound, sample_select<false, true>(sh, set.limit(s), each).key);
@@ -1379,7 +1383,7 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleArgs a) {
                 const auto each = [&](auto f) {
                     for (int i = tid; i < row.v; i += kSampleThreads) {
                         const float x = row.x(i);
-                        if (row.counts(x)) f(sample_rank_key(x, i), row.e(x));
+                        if (row.counts(x)) f(sample_rank_key(x, i), [&] { return sample_weight(row.e(x)); });
                     }
                 };
                 const SampleFound f = by_count ? sample_select<true, false>(sh.radix, want, each)
