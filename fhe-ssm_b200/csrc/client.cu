@@ -787,7 +787,7 @@ __device__ __forceinline__ float sample_logprob(const SampleRow& row, int i, uin
 }
 
 // Rows longer than a cluster's shared memory: a cluster for each row, whose blocks read the logits again for every step.  A
-// step is a few hundred instructions a token, so one block for a row took 1.9 ms for 300,000 logits, eight take 0.26
+// step is a few hundred instructions a token, so one block for a row of 300,000 took 1.9 ms; eight take 0.26.
 __global__ void __launch_bounds__(kSampleThreads) k_sample_long(const SampleArgs a) {
     __shared__ SampleRadix sh;
     __shared__ float redf[32];
