@@ -24,7 +24,7 @@
 // 64 float32 rows on 50,304 x 1,024 at groups of 64 take 24.2 us, bfloat16 rows 20.8 (316 TFLOP/s; 19% of cuBLAS's bfloat16
 // rate, 1.9 TB/s), on 65,536 x 1,024 25.1, 16 rows on 50,304 x 1,024 18.0.  About 8 us are the two launches, the operand's image,
 // the first tile's way through the roles and the last output; then 0.25 to 0.3 us for each 128 x 64 of the table, which is the
-// unpacking's and the drain's instructions: 60% of the issue slots over the whole kernel, with its waits between roles.
+// unpacking's and the drain's instructions: 55% of the issue slots over the whole kernel, with its waits between roles.
 //
 // Included by client.cu inside namespace fhe.
 
