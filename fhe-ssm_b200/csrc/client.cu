@@ -83,16 +83,13 @@ struct Q4Args {
     int scale_vec;   // a unit is a group, and rows of scales start on 16-byte boundaries
 };
 
-// The first bf16 piece of v (its bits), and what is left of v: pieces are cut, not rounded, so none overflows; an infinity or
-// NaN is all in the first.
+// The first bf16 piece of v (the high half of what is returned) and what is left of v: pieces are cut, not rounded, so none
+// overflows; an infinity or NaN is all in the first.
 __device__ __forceinline__ uint32_t q4_piece(float& v) {
     const uint32_t b = __float_as_uint(v);
-    if ((b & 0x7f800000u) == 0x7f800000u) {
-        v = 0.f;
-        return b & 0x007fffffu ? 0x7fffu : b >> 16;
-    }
-    v -= __uint_as_float(b & 0xffff0000u);
-    return b >> 16;
+    const bool finite = fabsf(v) < INFINITY;
+    v = finite ? v - __uint_as_float(b & 0xffff0000u) : 0.f;
+    return finite || !(b & 0x007fffffu) ? b : 0x7fff0000u;
 }
 
 template <class T>
@@ -144,14 +141,29 @@ __device__ __forceinline__ void q4_cut(const Q4Args& a, uint4* xs, int nt, int r
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = k + j < a.w.cols ? q4_float(src[j]) : 0.f;
         }
+        const auto cut = [&](auto piece) {
 #pragma unroll
-        for (int term = 0; term < TERMS; term++) {
-            uint32_t p[8];
+            for (int term = 0; term < TERMS; term++) {
+                uint32_t p[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) p[j] = q4_piece(v[j]);
-            const int col = r * TERMS + term;
-            xs[(ch * nt + (col >> 3)) * 32 + (col & 7) * 4 + t] =
-                make_uint4(p[0] | p[4] << 16, p[1] | p[5] << 16, p[2] | p[6] << 16, p[3] | p[7] << 16);
+                for (int j = 0; j < 8; j++) p[j] = piece(v[j]);
+                const int col = r * TERMS + term;
+                xs[(ch * nt + (col >> 3)) * 32 + (col & 7) * 4 + t] =
+                    make_uint4(__byte_perm(p[0], p[4], 0x7632), __byte_perm(p[1], p[5], 0x7632), __byte_perm(p[2], p[6], 0x7632),
+                               __byte_perm(p[3], p[7], 0x7632));
+            }
+        };
+        bool finite = true;
+#pragma unroll
+        for (int j = 0; j < 8; j++) finite = finite && fabsf(v[j]) < INFINITY;
+        if (finite) {   // 8 at a time: a test for each piece cost more than the cut
+            cut([](float& f) {
+                const uint32_t b = __float_as_uint(f);
+                f -= __uint_as_float(b & 0xffff0000u);
+                return b;
+            });
+        } else {
+            cut(q4_piece);
         }
     }
 }
