@@ -1530,8 +1530,9 @@ void client_ptr(const fhe::Context& c, const void* p, size_t align, const char* 
 
 void client_table(const fhe::Context& c, const fhe_q4* w) {
     REQUIRE(w, "null argument");
-    REQUIRE(w->rows >= 0 && w->cols >= 1 && w->cols <= FHE_Q4_MAX_COLS,
-            "q4 table: rows >= 0 and cols in 1..FHE_Q4_MAX_COLS");
+    // rows: the products count them, rounded up to their blocks' tiles, in 32 bits
+    REQUIRE(w->rows >= 0 && w->rows <= FHE_Q4_MAX_ROWS && w->cols >= 1 && w->cols <= FHE_Q4_MAX_COLS,
+            "q4 table: rows in 0..FHE_Q4_MAX_ROWS and cols in 1..FHE_Q4_MAX_COLS");
     REQUIRE(w->group >= 32 && w->group % 32 == 0, "q4 table: the group is a multiple of 32 columns");
     REQUIRE(w->ldq % 16 == 0 && w->ldq >= ((long long)w->cols + 31) / 32 * 16,
             "q4 table: rows are padded to a multiple of 16 bytes (32 columns)");

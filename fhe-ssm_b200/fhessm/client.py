@@ -26,6 +26,7 @@ _VP = C.c_void_p
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _LEGACY_STREAM = 1      # cudaStreamLegacy: torch calls its default stream 0, which the C-ABI takes for the context's
 MAX_VOCAB = 1 << 20
+MAX_ROWS = 1 << 30
 MAX_COLS = 1 << 20
 
 # fhe_q4 and fhe_sample_cfg as the bytes that the C-ABI reads (packed in 0.4 us; a ctypes structure takes 1.2)
@@ -98,6 +99,8 @@ class Q4Table:
         rows, nbytes = weight.shape
         if not 1 <= cols <= MAX_COLS or group < 32 or group % 32 or group >= 1 << 31:
             raise _bad(f"q4 table: 1 to {MAX_COLS} columns and a group that is a multiple of 32")
+        if rows > MAX_ROWS:
+            raise _bad(f"q4 table: {MAX_ROWS} rows at most")
         if nbytes < -(-cols // 32) * 16:
             raise _bad("q4 table: rows are padded to a multiple of 16 bytes (32 columns)")
         st, srows, groups, lds = _rows_of(scale, "q4 scales")

@@ -394,10 +394,12 @@ int fhe_keyswitch_noalloc(fhe_ctx* cx, uint64_t which, const uint64_t* d, int le
 #define FHE_F32 0
 #define FHE_F16 1
 #define FHE_BF16 2
+#define FHE_Q4_MAX_ROWS (1 << 30)
 #define FHE_Q4_MAX_COLS (1 << 20)
 #define FHE_Q4_MAX_M (1 << 21)
-/* a table of rows x cols values in 4 bits: value (i, c) = scale[i * lds + c / group] * (q - 8), q the
- * low (even c) or high (odd c) half of byte q[i * ldq + c / 2].  Rows start on 16-byte boundaries and
+/* a table of rows x cols values in 4 bits, FHE_Q4_MAX_ROWS x FHE_Q4_MAX_COLS at most:
+ * value (i, c) = scale[i * lds + c / group] * (q - 8), q the low (even c) or high (odd c) half of byte
+ * q[i * ldq + c / 2].  Rows start on 16-byte boundaries and
  * are padded to a multiple of 16 bytes (32 columns; the padding's content does not matter); ldq is
  * in bytes; group is a multiple of 32 (group >= cols: one scale a row); the last group may be short. */
 typedef struct {
