@@ -100,6 +100,7 @@ int fhe_ctx_set_option(fhe_ctx* cx, const char* name, int value) {
         if (std::strcmp(name, "matvec_tensor_cores") == 0) cx->cx.use_tc = value != 0;
         else if (std::strcmp(name, "merged_rescale") == 0) cx->cx.merged_rescale = value != 0;
         else if (std::strcmp(name, "pdl") == 0) cx->cx.use_pdl = value != 0;
+        else if (std::strcmp(name, "q4_waits") == 0) cx->cx.q4_waits = value < 0 ? -1 : value;
         else if (std::strcmp(name, "ntt_cluster") == 0) cx->cx.ntt_cluster = value != 0;
         else if (std::strcmp(name, "ntt_arith") == 0) cx->cx.ntt_arith = value == 1 ? 1 : 0;
         else if (std::strcmp(name, "baby_limbs") == 0) cx->cx.baby_limbs = value < 1 ? 1 : value > 64 ? 64 : value;

@@ -450,7 +450,8 @@ static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
     const int pieces = a.m * a.terms;
     const int most = (a.w.rows < 16384 && a.w.cols < 1536) || (a.w.rows > 16384 && a.w.group % 64) ? 18 : 8;
     if (pieces > most) {
-        const QgArgs q{a.w, a.x, a.m, a.ldx, a.out, a.ot, a.ldo, a.wide, 0, 0, 0, 0, 0, nullptr, 0, nullptr, nullptr};
+        const QgArgs q{a.w, a.x, a.m, a.ldx, a.out, a.ot, a.ldo, a.wide, 0, 0, 0, 0, 0, nullptr, 0, nullptr, nullptr,
+                       cx.q4_waits < 0 ? kQgWaits : cx.q4_waits};
         if (a.xt == FHE_F32) q4_gemm<float>(cx, q, st);
         else if (a.xt == FHE_F16) q4_gemm<__half>(cx, q, st);
         else q4_gemm<__nv_bfloat16>(cx, q, st);

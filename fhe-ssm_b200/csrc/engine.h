@@ -129,6 +129,7 @@ struct Context {
     unsigned int* d_err = nullptr;   // set by a kernel whose bounded wait ran out (checked at syncs)
     int use_tc = 1;                  // BSGS products on the tensor cores (tcgen05) where the shape allows
     int use_pdl = 1;                 // programmatic dependent launch for the hot kernels (launch_pdl)
+    int q4_waits = -1;               // tries of a wait for a free slot in k_q4_gemm; -1: its own limit
     int ntt_cluster = 0;             // N = 2^16: one cluster launch per transform (ntt.cu, k_ntt_cluster)
     int baby_limbs = 8;              // k_baby_pq: limbs walked by one thread
     int boot_compress = 1;           // bootstrap_setup: slot-periodic level plaintexts stored compressed

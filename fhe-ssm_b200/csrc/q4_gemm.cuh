@@ -38,13 +38,13 @@ constexpr int kQgXBytes = 131072;             // shared memory for them
 // A wait that has nothing to wait for costs 110 cycles, a commit 46 (measured alone), so they are few: operands change hands by
 // the job of 128 columns, and one wait of the products' warp sees to several barriers, a lane each.  (Waits with a sleep
 // time as a hint wake later: the whole kernel took 1.3 times as long with 20 us.)
-constexpr int kQgWaits = 1 << 22;             // bounded: some seconds
+constexpr int kQgWaits = 1 << 22;             // every wait is bounded: some seconds
 
 struct QgBars {
     uint64_t a_full[kQgAMax], a_empty[kQgAMax], d_full[kQgDMax], d_empty[kQgDMax], x_full[kQgSlotsMax], x_empty[kQgSlotsMax],
         s_full[2], s_empty[2], p_full, end;
     uint32_t tmem;
-    int dead;      // a wait ran out: nobody waits any more, the output is NaN
+    int dead;      // a wait ran out: the output is NaN
 };
 
 struct QgArgs {
@@ -65,6 +65,7 @@ struct QgArgs {
     int run;          // chunks that one accumulator takes before the scale is applied
     uint8_t* image;   // x's operand [tile of N rows][chunk][piece], then the rows' powers
     float* powers;    // 2^p, by which the rows' sums are multiplied
+    int waits;        // tries of the waits for a free slot (kQgWaits, or what the context's q4_waits says)
 };
 
 __device__ __forceinline__ void qg_init(uint64_t* bar, int count) {
@@ -85,14 +86,23 @@ __device__ __forceinline__ bool qg_try(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok;
 }
-// Waits until the phase of the given parity has passed; after a wait that ran out, anywhere in the block, it does not wait
-__device__ __forceinline__ void qg_wait(uint64_t* bar, uint32_t parity, QgBars* b) {
-    if (qg_try(bar, parity)) return;
-    for (int it = 0; it < kQgWaits; it++) {
-        if (qg_try(bar, parity)) return;
-        if ((it & 63) == 63 && *(volatile int*)&b->dead) return;
+// Waits until the phase of the given parity has passed.  False: this wait ran out, or another one of the block has (dead).  Whoever
+// writes operands, issues products or starts copies then stops, so that nothing is written that may still be read and no barrier
+// counts a copy twice.  The drain goes on without a test for each chunk, which cost the 64-row products 20 to 35% of their time: it
+// reads and lets go of accumulators and scales, whose sums, for all who still read them, are written out as NaN.  (A number of tries that is not a constant costs the products'
+// warp 5% at groups of 32, so only the waits for a free slot have one.)
+__device__ __forceinline__ bool qg_wait(uint64_t* bar, uint32_t parity, QgBars* b, int tries) {
+    if (qg_try(bar, parity)) return true;
+    for (int it = 0; it < tries; it++) {
+        if (qg_try(bar, parity)) return true;
+        if ((it & 63) == 63 && *(volatile int*)&b->dead) return false;
     }
     *(volatile int*)&b->dead = 1;
+    return false;
+}
+// the same by a warp, whose lanes stay together
+__device__ __forceinline__ bool qg_wait_warp(uint64_t* bar, uint32_t parity, QgBars* b, int tries) {
+    return __all_sync(0xffffffffu, qg_wait(bar, parity, b, tries));
 }
 
 // kind::f16, D float32, both operands float16 and K-major, M = 128, N = n
@@ -301,14 +311,14 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                 const int row = row0 + b * 128 + (warp & 3) * 32 + lane;
                 int left = per_group - (job0 + kr * a.slots) * kItems / a.run % per_group;
                 const float* sp = scales + (tile & 1) * a.groups * 128 + (warp & 3) * 32 + lane;
-                qg_wait(&bars->s_full[tile & 1], tile >> 1 & 1, bars);
+                qg_wait(&bars->s_full[tile & 1], tile >> 1 & 1, bars, kQgWaits);
                 uint64_t acc2[kC / 2];
 #pragma unroll
                 for (int j = 0; j < kC / 2; j++) acc2[j] = 0;
                 for (int c = 0; c < drains; c++) {
                     const float s = *sp;
                     if (--left == 0) left = per_group, sp += 128;
-                    qg_wait(&bars->d_full[slot], phase, bars);
+                    qg_wait(&bars->d_full[slot], phase, bars, kQgWaits);
                     __syncwarp();
                     asm volatile("tcgen05.fence::after_thread_sync;");
                     uint32_t v[kC];
@@ -338,12 +348,12 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     continue;
                 }
+                const int r0 = x0 + half * kC, nr = min(kC, a.m - r0);
+                qg_wait(&bars->p_full, 0, bars, kQgWaits);
                 if (*(volatile int*)&bars->dead) {
 #pragma unroll
                     for (int j = 0; j < kC; j++) acc[j] = __int_as_float(0x7fffffff);
                 }
-                const int r0 = x0 + half * kC, nr = min(kC, a.m - r0);
-                qg_wait(&bars->p_full, 0, bars);
 #pragma unroll
                 for (int j = 0; j < kC; j += 4) {
                     const float4 p = *reinterpret_cast<const float4*>(powers + half * kC + j);
@@ -407,12 +417,14 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
 #pragma unroll
         for (int s = 0; s < kQgStages - 1; s++) fetch();
         uint32_t slot = grp, phase = 1;
+        bool live = true;   // after a wait that ran out the warp still meets the others at their barrier, and only there
         for (int j = grp, s = 0; j < jobs; j += 2, s++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kQgStages - 2) : "memory");
             // all copies of the stage are there; the one before it is read
             if (grp == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
             else asm volatile("bar.sync 2, 128;" ::: "memory");
             fetch();
+            if (!live) continue;
             const uint8_t* st = my + (s % kQgStages) * kQgStageBytes + t * 64;
 #pragma unroll 1
             for (int h = 0; h < kItems; h++) {
@@ -426,12 +438,15 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                     qg_unpack(u.w, v + q * 16 + 12);
                 }
                 if (h == 0) {
-                    qg_wait(&bars->a_empty[slot], phase, bars);
-                    __syncwarp();
+                    if (!qg_wait_warp(&bars->a_empty[slot], phase, bars, a.waits)) {
+                        live = false;
+                        break;
+                    }
                     asm volatile("tcgen05.fence::after_thread_sync;");
                 }
                 qg_st<KC / 2>(tm + acol + slot * 64 + h * (KC / 2) + lanes, v);
             }
+            if (!live) continue;
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;");
             __syncwarp();
@@ -447,48 +462,52 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         const uint32_t base = __reduce_or_sync(0xffffffffu, tm);   // the same in all lanes, as the compiler now sees
         const uint64_t xdesc = tc_desc(tc_smem(xs), 128, qg_sbo<KC>());
         uint32_t i = 0, aphase = 0, slot = 0, dphase = 1;
-        for (int kr = 0; kr < ranges; kr++) {
-            const int n = range_jobs(kr);
-            for (int b = 0; b < tiles; b++)
-                for (int c = 0; c < n; c++) {
-                    const uint32_t at = base + acol + i * 64;
-                    const uint64_t xd = xdesc + (uint32_t)(c * kSlotBytes >> 4);
+        const auto issue = [&]() {
+            for (int kr = 0; kr < ranges; kr++) {
+                const int n = range_jobs(kr);
+                for (int b = 0; b < tiles; b++)
+                    for (int c = 0; c < n; c++) {
+                        const uint32_t at = base + acol + i * 64;
+                        const uint64_t xd = xdesc + (uint32_t)(c * kSlotBytes >> 4);
 #pragma unroll
-                    for (int h = 0; h < kItems; h += 2) {   // two chunks at a time, of one accumulator or two
-                        const bool wrap = slot + 1 == nd;
-                        const uint32_t slot1 = a.run == 2 ? slot : wrap ? 0 : slot + 1, phase1 = a.run == 1 && wrap ? dphase ^ 1 : dphase;
-                        uint64_t* bar = lane == 0   ? &bars->a_full[i]
-                                        : lane == 1 ? &bars->d_empty[slot]
-                                        : lane == 2 ? &bars->d_empty[slot1]
-                                                    : &bars->x_full[c];
-                        qg_wait(bar, lane == 0 ? aphase : lane == 1 ? dphase : lane == 2 ? phase1 : kr & 1, bars);
-                        __syncwarp();
-                        asm volatile("tcgen05.fence::after_thread_sync;");
-                        if (elected) {
+                        for (int h = 0; h < kItems; h += 2) {   // two chunks at a time, of one accumulator or two
+                            const bool wrap = slot + 1 == nd;
+                            const uint32_t slot1 = a.run == 2 ? slot : wrap ? 0 : slot + 1, phase1 = a.run == 1 && wrap ? dphase ^ 1 : dphase;
+                            uint64_t* bar = lane == 0   ? &bars->a_full[i]
+                                            : lane == 1 ? &bars->d_empty[slot]
+                                            : lane == 2 ? &bars->d_empty[slot1]
+                                                        : &bars->x_full[c];
+                            if (!qg_wait_warp(bar, lane == 0 ? aphase : lane == 1 ? dphase : lane == 2 ? phase1 : kr & 1, bars,
+                                              kQgWaits))
+                                return;
+                            asm volatile("tcgen05.fence::after_thread_sync;");
+                            if (elected) {
 #pragma unroll
-                            for (int g = 0; g < 2; g++) {
+                                for (int g = 0; g < 2; g++) {
 #pragma unroll
-                                for (int p = 0; p < kPieces; p++)
+                                    for (int p = 0; p < kPieces; p++)
 #pragma unroll
-                                    for (int ks = 0; ks < KC / 16; ks++)
-                                        qg_mma(base + dcol + (g ? slot1 : slot) * N, at + (h + g) * (KC / 2) + ks * 8,
-                                               xd + (((h + g) * kChunkBytes + p * kPieceBytes + ks * 256) >> 4), idesc,
-                                               p + ks > 0 || (g && a.run == 2));
-                                if (g || a.run == 1) qg_commit(&bars->d_full[g ? slot1 : slot]);
+                                        for (int ks = 0; ks < KC / 16; ks++)
+                                            qg_mma(base + dcol + (g ? slot1 : slot) * N, at + (h + g) * (KC / 2) + ks * 8,
+                                                   xd + (((h + g) * kChunkBytes + p * kPieceBytes + ks * 256) >> 4), idesc,
+                                                   p + ks > 0 || (g && a.run == 2));
+                                    if (g || a.run == 1) qg_commit(&bars->d_full[g ? slot1 : slot]);
+                                }
+                                if (h + 2 == kItems) {
+                                    qg_commit(&bars->a_empty[i]);
+                                    if (b == tiles - 1 && kr + 1 < ranges) qg_commit(&bars->x_empty[c]);
+                                }
                             }
-                            if (h + 2 == kItems) {
-                                qg_commit(&bars->a_empty[i]);
-                                if (b == tiles - 1 && kr + 1 < ranges) qg_commit(&bars->x_empty[c]);
-                            }
+                            __syncwarp();
+                            slot = slot1;
+                            dphase = phase1;
+                            if (++slot == nd) slot = 0, dphase ^= 1;
                         }
-                        __syncwarp();
-                        slot = slot1;
-                        dphase = phase1;
-                        if (++slot == nd) slot = 0, dphase ^= 1;
+                        if (++i == na) i = 0, aphase ^= 1;
                     }
-                    if (++i == na) i = 0, aphase ^= 1;
-                }
-        }
+            }
+        };
+        issue();
         if (elected) {
             qg_commit(&bars->end);   // all products, before tensor memory is given back
             for (int it = 0; it < kQgWaits && !qg_try(&bars->end, 0); it++) {}
@@ -502,17 +521,18 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         if (lane == 0) {
             qg_arrive(&bars->p_full);
             const uint8_t* src = a.image + ((size_t)blockIdx.y * a.jobs + job0) * kSlotBytes;
-            for (int ch = 0, c = 0, kr = 0; ch < all_jobs; ch++) {
-                if (kr) qg_wait(&bars->x_empty[c], (kr - 1) & 1, bars);
+            int ch = 0;
+            for (int c = 0, kr = 0; ch < all_jobs; ch++) {
+                // a slot that is handed back has had its copy: the products waited for it
+                if (kr && !qg_wait(&bars->x_empty[c], (kr - 1) & 1, bars, a.waits)) break;
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc_smem(&bars->x_full[c])), "r"(kSlotBytes)
                              : "memory");
                 tc_bulk_g2s(xs + (size_t)c * kSlotBytes, src + (size_t)ch * kSlotBytes, kSlotBytes, &bars->x_full[c]);
                 if (++c == a.slots) c = 0, kr++;
             }
-            // the last copies, if nobody else has waited for them
-            const int left = range_jobs(ranges - 1);
-            for (int c = 0; c < left; c++)
-                for (int it = 0; it < kQgWaits && !qg_try(&bars->x_full[c], (ranges - 1) & 1); it++) {}
+            // the last copy of each slot, if nobody else has waited for it
+            for (int c = 0; c < min(a.slots, ch); c++)
+                for (int it = 0; it < kQgWaits && !qg_try(&bars->x_full[c], (ch - 1 - c) / a.slots & 1); it++) {}
         }
         __syncwarp();
     } else {
@@ -530,7 +550,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
                     float* to = scales + (tile & 1) * a.groups * 128 + t;
                     const S* p0 = src + min(row0 + b * 128 + t, a.w.rows - 1) * a.w.lds + first;
                     const S* p1 = src + min(row0 + b * 128 + t + 64, a.w.rows - 1) * a.w.lds + first;
-                    if (tile > 1) qg_wait(&bars->s_empty[tile & 1], (tile >> 1 & 1) ^ 1, bars);
+                    if (tile > 1 && !qg_wait(&bars->s_empty[tile & 1], (tile >> 1 & 1) ^ 1, bars, a.waits)) return;
                     if (wide && first % kPer == 0) {
                         for (int g0 = 0; g0 < a.groups; g0 += kDeep * kPer) {
                             uint4 u[2][kDeep];

@@ -92,6 +92,8 @@ void* fhe_ctx_stream(const fhe_ctx* cx);
  * "plaintext_cache_reserve_mib" (default 24576): a plan caches only while this much device
  * memory would stay free.
  * "pdl" (default 1): programmatic dependent launch of the hot kernels.
+ * "q4_waits" (default -1): tries after which a wait for a free operand slot inside the product of several
+ * rows (fhe_q4_matvec) gives up; -1 is some seconds, 0 gives up where a slot is not free yet.
  * "ntt_cluster" (default 0): N = 2^16 transforms as one 8-CTA cluster launch per limb.
  * "ntt_arith" (default 1): NTT butterflies with the cheaper Shoup quotient; 0: exact quotient
  * (the same words either way).

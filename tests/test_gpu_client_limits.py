@@ -26,3 +26,47 @@ def test_too_many_rows_are_refused(cx, rows):
     for rc in (h.fhe_q4_matvec(cx.h, table, x.data_ptr(), 0, 32, 1, out.data_ptr(), 0, rows, None),
                h.fhe_q4_rows(cx.h, table, ids.data_ptr(), 1, out.data_ptr(), 0, 32, None)):
         assert rc == -1 and b"FHE_Q4_MAX_ROWS" in fhessm.lib().fhe_last_error()
+
+
+def random_table(rows, cols, group, seed=0, stype=torch.float16):
+    from fhessm.client import Q4Table
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = torch.randint(0, 256, (rows, -(-cols // 32) * 16), device="cuda", dtype=torch.uint8, generator=g)
+    s = torch.rand(rows, -(-cols // group), device="cuda", generator=g) * 0.01 + 0.001
+    return Q4Table(w, s.to(stype), cols=cols, group=group)
+
+
+# One tile, which needs no slot twice; several tiles in every block; several ranges of columns; columns in parts.  `lost`: a block
+# fills its slots long before the first of them is free again.
+SHAPES = [(20, 100, 256, 64, torch.bfloat16, False), (64, 50304, 1024, 64, torch.float32, True),
+          (64, 20000, 2048, 96, torch.float32, True), (17, 40000, 4096, 32, torch.float16, True),
+          (64, 300, 4096, 32, torch.bfloat16, False)]
+
+
+@pytest.mark.parametrize("m,rows,cols,group,xt,lost", SHAPES)
+def test_a_wait_that_runs_out(cx, m, rows, cols, group, xt, lost):
+    """With no tries at all, the first role that finds no free slot gives up: the call ends by itself, what is not NaN is right, a
+    NaN is reported at the next sync, and the calls after it are right again."""
+    from fhessm import FheError, client
+    t = random_table(rows, cols, group)
+    x = torch.randn(m, cols, device="cuda").to(xt)
+    want = client.q4_matvec(cx, x, t)
+    torch.cuda.synchronize()
+    cx.sync()
+    cx.set_option("q4_waits", 0)
+    try:
+        for _ in range(4):
+            got = client.q4_matvec(cx, x, t)
+            torch.cuda.synchronize()
+            nan = torch.isnan(got)
+            assert ((got == want) | nan).all()
+            assert nan.any() or not lost
+            if nan.any():
+                with pytest.raises(FheError, match="wait"):
+                    cx.sync()
+            cx.sync()
+    finally:
+        cx.set_option("q4_waits", -1)
+    assert torch.equal(client.q4_matvec(cx, x, t), want)
+    torch.cuda.synchronize()
+    cx.sync()
