@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(kQgThreads, 1) k_q4_gemm(const QgArgs a, unsig
         __syncwarp();
     } else {
         // ---- scales: 0 past the last column's group
-        const int t = tid - 18 * 32, groups = (a.w.cols + a.w.group - 1) / a.w.group;
+        const int t = tid - 18 * 32, groups = (a.w.cols - 1) / a.w.group + 1;   // (a group may be near 2^31)
         uint32_t tile = 0;
         const auto fill = [&](auto* src) {
             using S = typename std::remove_cv<typename std::remove_pointer<decltype(src)>::type>::type;

@@ -70,3 +70,19 @@ def test_a_wait_that_runs_out(cx, m, rows, cols, group, xt, lost):
     assert torch.equal(client.q4_matvec(cx, x, t), want)
     torch.cuda.synchronize()
     cx.sync()
+
+
+@pytest.mark.parametrize("m", [1, 20, 64])
+@pytest.mark.parametrize("group", [1 << 20, (1 << 31) - 1024, (1 << 31) - 32])
+def test_a_group_far_above_the_columns(cx, group, m):
+    """One scale a row, whatever the group's size: the same product as with the next group above the columns."""
+    from fhessm import client
+    t = random_table(200, 1000, 1024)
+    x = torch.randn(m, 1000, device="cuda")
+    wide = client.Q4Table(t.weight, t.scale, cols=1000, group=group)
+    want = client.q4_matvec(cx, x, t)
+    # sums of the same products, rounded in another order: 1,000 roundings of 2^-24 on either side
+    mag = x.abs().double() @ t.dequantise().abs().double().T
+    assert ((client.q4_matvec(cx, x, wide).double() - want.double()).abs() <= 2 * 1000 * 2.0 ** -24 * mag).all()
+    ids = torch.arange(200, device="cuda")
+    assert torch.equal(client.q4_rows(cx, ids, wide), t.dequantise())
