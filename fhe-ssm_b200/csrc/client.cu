@@ -396,34 +396,27 @@ static void q4_gemm_launch(Context& cx, QgArgs a, cudaStream_t st) {
     const size_t smem = 2 * kQgStages * kQgStageBytes + (size_t)a.slots * kSlot + (size_t)a.groups * 1024 + N * sizeof(float) +
                         sizeof(QgBars);
     const size_t image = (size_t)xt * a.jobs * kSlot, powers = (size_t)xt * N * sizeof(float);
-    uint8_t* work = nullptr;
-    CUDA_CHECK(cudaMallocAsync((void**)&work, image + powers + (parts > 1 ? (size_t)parts * a.m * a.w.rows * sizeof(float) : 0), st));
-    a.image = work;
-    a.powers = reinterpret_cast<float*>(work + image);
-    a.parts = parts > 1 ? reinterpret_cast<float*>(work + image + powers) : nullptr;
-    try {
-        client_smem<k_q4_gemm<N, KC, kPieces>>(cx);
-        k_q4_pack<N, KC, XT><<<xt * N, 128, 0, st>>>(a);
-        CUDA_CHECK(cudaGetLastError());
-        launch_pdl(cx, k_q4_gemm<N, KC, kPieces>, dim3((a.w.rows + a.block_rows - 1) / a.block_rows, xt, parts), dim3(kQgThreads),
-                   smem, st, a, cx.d_err);
-        cx.launches += 2;
-        if (parts > 1) {
-            const dim3 grid((unsigned)std::min<long long>(592, ((long long)a.m * a.w.rows + 255) / 256));
-            const auto sum = [&](auto* out) {
-                using T = typename std::remove_pointer<decltype(out)>::type;
-                launch_pdl(cx, k_q4_sum<T>, grid, dim3(256), 0, st, a.parts, parts, a.m, a.w.rows, out, a.ldo);
-            };
-            if (a.ot == FHE_F32) sum(static_cast<float*>(a.out));
-            else if (a.ot == FHE_F16) sum(static_cast<__half*>(a.out));
-            else sum(static_cast<__nv_bfloat16*>(a.out));
-            cx.launches++;
-        }
-    } catch (...) {
-        cudaFreeAsync(work, st);
-        throw;
+    const DevBuf work((image + powers + (parts > 1 ? (size_t)parts * a.m * a.w.rows * sizeof(float) : 0) + 7) / 8, st);
+    a.image = reinterpret_cast<uint8_t*>(work.p);
+    a.powers = reinterpret_cast<float*>(a.image + image);
+    a.parts = parts > 1 ? reinterpret_cast<float*>(a.image + image + powers) : nullptr;
+    client_smem<k_q4_gemm<N, KC, kPieces>>(cx);
+    k_q4_pack<N, KC, XT><<<xt * N, 128, 0, st>>>(a);
+    CUDA_CHECK(cudaGetLastError());
+    launch_pdl(cx, k_q4_gemm<N, KC, kPieces>, dim3((a.w.rows + a.block_rows - 1) / a.block_rows, xt, parts), dim3(kQgThreads),
+               smem, st, a, cx.d_err);
+    cx.launches += 2;
+    if (parts > 1) {
+        const dim3 grid((unsigned)std::min<long long>(592, ((long long)a.m * a.w.rows + 255) / 256));
+        const auto sum = [&](auto* out) {
+            using T = typename std::remove_pointer<decltype(out)>::type;
+            launch_pdl(cx, k_q4_sum<T>, grid, dim3(256), 0, st, a.parts, parts, a.m, a.w.rows, out, a.ldo);
+        };
+        if (a.ot == FHE_F32) sum(static_cast<float*>(a.out));
+        else if (a.ot == FHE_F16) sum(static_cast<__half*>(a.out));
+        else sum(static_cast<__nv_bfloat16*>(a.out));
+        cx.launches++;
     }
-    CUDA_CHECK(cudaFreeAsync(work, st));
 }
 template <int N, class XT>
 static void q4_gemm_group(Context& cx, const QgArgs& a, cudaStream_t st) {

@@ -55,11 +55,13 @@ DevBuf::DevBuf(size_t w, cudaStream_t s) : words(w), st(s) {
     cudaError_t e = cudaMallocAsync((void**)&p, w * sizeof(uint64_t), s);
     if (e == cudaErrorMemoryAllocation) {
         // the pool keeps freed buffers (the context sets no release threshold): hand the unused
-        // ones back to the driver and try once more before failing
+        // ones back to the driver and try once more before failing (a stream that is being captured
+        // cannot be waited for)
         (void)cudaGetLastError();
         int dev = 0;
         cudaMemPool_t pool;
-        if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetDefaultMemPool(&pool, dev) == cudaSuccess &&
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(s, &cap) == cudaSuccess && cap == cudaStreamCaptureStatusNone && cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetDefaultMemPool(&pool, dev) == cudaSuccess &&
             cudaStreamSynchronize(s) == cudaSuccess && cudaMemPoolTrimTo(pool, 0) == cudaSuccess)
             e = cudaMallocAsync((void**)&p, w * sizeof(uint64_t), s);
     }

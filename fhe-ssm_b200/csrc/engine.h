@@ -27,13 +27,16 @@ struct Error : std::runtime_error {
     explicit Error(const std::string& s, int c = -1) : std::runtime_error(s), code(c) {}
 };
 
+// The error is reported here and taken out of the runtime, where the next launch check, this library's or torch's, would find it again.
 #define CUDA_CHECK(x)                                                                            \
     do {                                                                                         \
         cudaError_t err__ = (x);                                                                 \
-        if (err__ != cudaSuccess)                                                                \
+        if (err__ != cudaSuccess) {                                                              \
+            (void)cudaGetLastError();                                                            \
             throw ::fhe::Error(std::string("CUDA error: ") + cudaGetErrorString(err__) + " at " + \
                                    __FILE__ + ":" + std::to_string(__LINE__),                    \
                                -3);                                                              \
+        }                                                                                        \
     } while (0)
 
 constexpr int kMaxMod = 64;

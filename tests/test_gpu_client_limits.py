@@ -86,3 +86,33 @@ def test_a_group_far_above_the_columns(cx, group, m):
     assert ((client.q4_matvec(cx, x, wide).double() - want.double()).abs() <= 2 * 1000 * 2.0 ** -24 * mag).all()
     ids = torch.arange(200, device="cuda")
     assert torch.equal(client.q4_rows(cx, ids, wide), t.dequantise())
+
+
+def trim_pool():
+    """Gives the driver what its stream-ordered pool holds and nobody uses, as after earlier tests."""
+    import ctypes
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    rt, pool = ctypes.CDLL("libcudart.so.12"), ctypes.c_void_p()
+    assert rt.cudaDeviceGetDefaultMemPool(ctypes.byref(pool), 0) == 0
+    assert rt.cudaMemPoolTrimTo(pool, ctypes.c_size_t(0)) == 0
+
+
+def test_a_product_refused_for_memory(cx):
+    """A workspace as large as x, of which the GPU holds one only: the call is refused, and the calls after it, torch's too, are
+    served."""
+    from fhessm import FheError, client
+    trim_pool()
+    mem = cx.memory()
+    cols = 12288
+    x = torch.empty(min(1 << 21, int(0.6 * mem["total"]) // (4 * cols)), cols, device="cuda")
+    t = random_table(1, cols, 64)
+    with pytest.raises(FheError, match="memory"):
+        client.q4_matvec(cx, x, t)
+    ids = torch.zeros(3, dtype=torch.int64, device="cuda")
+    assert torch.equal(client.q4_rows(cx, ids, t), t.dequantise().expand(3, cols))
+    assert torch.ones(5, device="cuda").sum() == 5
+    few = torch.zeros(20, cols, device="cuda")
+    assert (client.q4_matvec(cx, few, t) == 0).all()
+    del x
+    trim_pool()
