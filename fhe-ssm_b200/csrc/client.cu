@@ -74,11 +74,10 @@ struct Q4Args {
     void* out;
     int ot;
     long long ldo;
-    int per;         // rows of x that a block takes
     int ks_log2;     // 2^ks_log2 warps share a row tile's columns
     int kb_chunks;   // chunks of columns held at a time, in whole stages for each of these warps
     int units;       // scales that a warp holds for each row
-    uint32_t group_magic;   // chunk / (chunks of a group) = chunk * magic >> 32 (both at most 2^15); 0: a group is a chunk
+    uint32_t group_magic;   // q4_group_magic
     int wide;        // rows of x start on 16-byte boundaries
     int scale_vec;   // a unit is a group, and rows of scales start on 16-byte boundaries
 };
@@ -101,19 +100,19 @@ __device__ __forceinline__ float q4_float(__half v) { return __half2float(v); }
 template <>
 __device__ __forceinline__ float q4_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Pieces of rows r0..r0+mr of x, chunks kb0..kb1 -> the product's operand [chunk][tile of 8 columns][lane], 16 bytes each:
+// Pieces of x's rows, chunks kb0..kb1 -> the product's operand [chunk][tile of 8 columns][lane], 16 bytes each:
 // the lane's column (r TERMS + piece) and its 8 values, paired as q4_unpack pairs the table's.
 template <class T, int TERMS>
-__device__ __forceinline__ void q4_cut(const Q4Args& a, uint4* xs, int nt, int r0, int mr, int kb0, int kb1) {
+__device__ __forceinline__ void q4_cut(const Q4Args& a, uint4* xs, int nt, int kb0, int kb1) {
     // a warp takes 8 chunks of a row at a time
     const int lane = threadIdx.x & 31, t = lane & 3;
     int r = threadIdx.x >> 5, ch = lane >> 2;
     for (;; r += kQ4Warps) {
-        while (r >= mr) r -= mr, ch += 8;
+        while (r >= a.m) r -= a.m, ch += 8;
         if (ch - (lane >> 2) >= kb1 - kb0) break;
         if (ch >= kb1 - kb0) continue;
         const int k = (kb0 + ch) * 32 + t * 8;
-        const T* src = static_cast<const T*>(a.x) + (r0 + r) * a.ldx + k;
+        const T* src = static_cast<const T*>(a.x) + r * a.ldx + k;
         if constexpr (TERMS == 1) {   // bfloat16 is its own piece
             const uint16_t* bits = reinterpret_cast<const uint16_t*>(src);
             uint4 u;
@@ -224,7 +223,7 @@ __device__ __forceinline__ void q4_scales(const Q4Args& a, const void* row, uint
     }
 }
 
-// NT: tiles of 8 columns.  P: chunks after which the scale is applied, the largest of 1, 2, 4 that divides a group's.
+// NT: tiles of 8 columns, which hold the pieces of all rows of x.  P: chunks after which the scale is applied, the largest of 1, 2, 4 that divides a group's.
 template <int NT, int P>
 __global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const Q4Args a) {
     extern __shared__ __align__(16) uint8_t qsm[];
@@ -234,7 +233,7 @@ __global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const Q4Args a) {
     const int chunks = (a.w.cols + 31) / 32;
     const int ks = 1 << a.ks_log2, rows = 16 * kQ4Warps >> a.ks_log2;   // warps on a tile, table rows of a block
     const int row0 = blockIdx.x * rows + (warp >> a.ks_log2) * 16, kq = warp & (ks - 1);
-    const int r0 = blockIdx.y * a.per, mr = min(a.per, a.m - r0), scale_bytes = a.w.scale_type == FHE_F32 ? 4 : 2;
+    const int scale_bytes = a.w.scale_type == FHE_F32 ? 4 : 2;
     float* sc = reinterpret_cast<float*>(xs + a.kb_chunks * NT * 32) + warp * 16 * a.units;   // [unit][16 rows]
     float acc[NT][4];
 #pragma unroll
@@ -270,9 +269,9 @@ __global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const Q4Args a) {
             if (e + v <= (chunks + P - 1) / P) first = *reinterpret_cast<const uint4*>(srow + (size_t)e * scale_bytes);
         }
         __syncthreads();   // the previous block's pieces are read
-        if (a.xt == FHE_F32) q4_cut<float, 3>(a, xs, NT, r0, mr, kb0, kb1);
-        else if (a.xt == FHE_F16) q4_cut<__half, 2>(a, xs, NT, r0, mr, kb0, kb1);
-        else q4_cut<__nv_bfloat16, 1>(a, xs, NT, r0, mr, kb0, kb1);
+        if (a.xt == FHE_F32) q4_cut<float, 3>(a, xs, NT, kb0, kb1);
+        else if (a.xt == FHE_F16) q4_cut<__half, 2>(a, xs, NT, kb0, kb1);
+        else q4_cut<__nv_bfloat16, 1>(a, xs, NT, kb0, kb1);
         if (a.w.scale_type == FHE_F16) q4_scales<__half, P>(a, srow, first, sc, c0, (c1 - c0) / P, chunks);
         else if (a.w.scale_type == FHE_BF16) q4_scales<__nv_bfloat16, P>(a, srow, first, sc, c0, (c1 - c0) / P, chunks);
         else q4_scales<float, P>(a, srow, first, sc, c0, (c1 - c0) / P, chunks);
@@ -327,15 +326,21 @@ __global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const Q4Args a) {
     }
     __syncthreads();
     const int rows_log2 = 7 - a.ks_log2;
-    for (int i = tid; i < mr << rows_log2; i += kQ4Threads) {
+    for (int i = tid; i < a.m << rows_log2; i += kQ4Threads) {
         const int r = i >> rows_log2, row = i & (rows - 1), at = blockIdx.x * rows + row;
         if (at >= a.w.rows) continue;
         const float* sp = reinterpret_cast<const float*>(qsm) + ((row >> 4) << a.ks_log2) * (NT * 8 * 16) + (row & 15);
         float v = 0.f;
         for (int k = 0; k < ks; k++)
             for (int j = a.terms - 1; j >= 0; j--) v += sp[k * (NT * 8 * 16) + (r * a.terms + j) * 16];
-        st_any(a.out, a.ot, (long long)(r0 + r) * a.ldo + at, v);
+        st_any(a.out, a.ot, (long long)r * a.ldo + at, v);
     }
+}
+
+// chunk / (chunks of a group) = chunk * magic >> 32 (both at most 2^15); 0: a group is a chunk
+static uint32_t q4_group_magic(const fhe_q4& w) {
+    const int gpc = std::min(w.group, FHE_Q4_MAX_COLS) / 32;
+    return gpc == 1 ? 0u : (uint32_t)(((1ull << 32) + gpc - 1) / gpc);
 }
 
 template <int NT, int P>
@@ -343,7 +348,6 @@ static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
     const int tiles = (a.w.rows + 15) / 16, gpc = std::min(a.w.group, FHE_Q4_MAX_COLS) / 32;
     // warps enough to keep the loads in flight (8 an SM), but two stages of columns at least for each
     const int chunks = (a.w.cols + 31) / 32;
-    a.per = NT * 8 / a.terms;
     a.ks_log2 = 0;
     while (a.ks_log2 < 3 && (tiles << a.ks_log2) < 148 * 8 && chunks >= (4 << a.ks_log2) * kQ4Stage) a.ks_log2++;
     // As many columns at a time as fit (512 bytes a chunk and tile of pieces, 512 a scale for 8 warps' rows), in equal blocks.  Two
@@ -354,10 +358,10 @@ static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
     a.kb_chunks = ((chunks + turns - 1) / turns + step - 1) / step * step;
     a.units = (a.kb_chunks >> a.ks_log2) / P;
     a.scale_vec = gpc == P && (reinterpret_cast<uintptr_t>(a.w.scale) | (uintptr_t)a.w.lds * (a.w.scale_type == FHE_F32 ? 4 : 2)) % 16 == 0;
-    a.group_magic = gpc == 1 ? 0u : (uint32_t)(((1ull << 32) + gpc - 1) / gpc);
+    a.group_magic = q4_group_magic(a.w);
     const size_t smem = kQ4RingBytes + (size_t)a.kb_chunks * NT * 512 + (size_t)a.units * kQ4Warps * 64;
     if (smem > 48 * 1024) client_smem<k_q4_mma<NT, P>>(cx);
-    k_q4_mma<NT, P><<<dim3(grid, (a.m + a.per - 1) / a.per), kQ4Threads, smem, st>>>(a);
+    k_q4_mma<NT, P><<<grid, kQ4Threads, smem, st>>>(a);
     CUDA_CHECK(cudaGetLastError());
     cx.launches++;
 }
@@ -488,11 +492,6 @@ __global__ void __launch_bounds__(128) k_q4_rows(const fhe_q4 w, const int64_t* 
         for (int j = 0; j < 8; j++)
             if (c + j < w.cols) o[j] = u[j];
     }
-}
-
-static uint32_t q4_group_magic(const fhe_q4& w) {
-    const int gpc = std::min(w.group, FHE_Q4_MAX_COLS) / 32;
-    return gpc == 1 ? 0u : (uint32_t)(((1ull << 32) + gpc - 1) / gpc);
 }
 
 template <class T>
@@ -1557,7 +1556,7 @@ extern "C" int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_
         client_ptr(cx->cx, x, xb, "x");
         client_ptr(cx->cx, out, ob, "out");
         cudaStream_t st = client_stream(cx, stream);
-        fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0, 0, 0, 0, 0, 0, 0}, st);
+        fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0, 0, 0, 0, 0, 0}, st);
     });
 }
 
