@@ -44,7 +44,8 @@ static void client_smem(const Context& cx) {
 // Within a group the sum is a product of whole numbers -8..7, which every 16-bit float holds exactly, with x; the
 // scale is applied to the group's sum in float32.  x is cut into bf16 pieces that add up to it exactly (float32: 3 of 8
 // bits, float16: 2, bf16: itself), each piece a column of the matrix product, so nothing is rounded before the
-// float32 sums.
+// float32 sums.  The group's sum is up to 2^10 times the largest value of x, which the scale would bring back into range but float32
+// does not hold for values of 2^117 and more: a row that has one is cut 2^-16 times as large, and its output multiplied again.
 //
 // k_q4_mma: few columns (one row of x, or some).  What it must read is the table, so a warp streams 16 table rows through a
 // shared-memory ring of its own (cp.async, no block barrier) and multiplies them on the tensor cores (m16n8k16: 16 table
@@ -64,7 +65,7 @@ constexpr int kQ4Stage = 4;             // 32-column chunks of a stage
 constexpr int kQ4Stages = 4;
 constexpr int kQ4Pitch = kQ4Stage * 16 + 16;   // bytes of a row in a stage: 20 banks apart, 8 rows x 4 words meet all 32
 constexpr int kQ4StageBytes = 16 * kQ4Pitch;
-constexpr int kQ4RingBytes = kQ4Warps * kQ4Stages * kQ4StageBytes;
+constexpr int kQ4RingBytes = 16 + kQ4Warps * kQ4Stages * kQ4StageBytes;   // before it a word: the rows that are large
 
 struct Q4Args {
     fhe_q4 w;
@@ -100,13 +101,18 @@ __device__ __forceinline__ float q4_float(__half v) { return __half2float(v); }
 template <>
 __device__ __forceinline__ float q4_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+constexpr float kQ4Big = 1.661534994731145e35f;   // 2^117
+constexpr float kQ4Down = 1.f / 65536.f;
+
 // Pieces of x's rows, chunks kb0..kb1 -> the product's operand [chunk][tile of 8 columns][lane], 16 bytes each:
-// the lane's column (r TERMS + piece) and its 8 values, paired as q4_unpack pairs the table's.
-template <class T, int TERMS>
-__device__ __forceinline__ void q4_cut(const Q4Args& a, uint4* xs, int nt, int kb0, int kb1) {
+// the lane's column (r TERMS + piece) and its 8 values, paired as q4_unpack pairs the table's.  DOWN: rows in the mask `down`
+// are cut times kQ4Down.  True: the thread has met a value of kQ4Big or more, or one that is not finite.
+template <class T, int TERMS, bool DOWN = false>
+__device__ __forceinline__ bool q4_cut(const Q4Args& a, uint4* xs, int nt, int kb0, int kb1, uint32_t down = 0) {
     // a warp takes 8 chunks of a row at a time
     const int lane = threadIdx.x & 31, t = lane & 3;
     int r = threadIdx.x >> 5, ch = lane >> 2;
+    bool large = false;
     for (;; r += kQ4Warps) {
         while (r >= a.m) r -= a.m, ch += 8;
         if (ch - (lane >> 2) >= kb1 - kb0) break;
@@ -122,6 +128,18 @@ __device__ __forceinline__ void q4_cut(const Q4Args& a, uint4* xs, int nt, int k
 #pragma unroll
                 for (int j = 0; j < 8; j++) p[j] = k + j < a.w.cols ? bits[j] : 0;
                 u = make_uint4(p[0] | p[1] << 16, p[2] | p[3] << 16, p[4] | p[5] << 16, p[6] | p[7] << 16);
+            }
+            const auto larger = [](__nv_bfloat162 p, __nv_bfloat162 q) { return __hmax2(__habs2(p), __habs2(q)); };
+            const auto two = [](const uint32_t& w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+            const __nv_bfloat162 most = larger(larger(two(u.x), two(u.y)), larger(two(u.z), two(u.w)));
+            // bit 15 of a half: 0x7a00, kQ4Big's bits, or more
+            if (*reinterpret_cast<const uint32_t*>(&most) + 0x06000600u & 0x80008000u) large = true;
+            if (DOWN && (down >> r & 1)) {
+                const auto times = [](uint32_t w) {
+                    return __byte_perm(__float_as_uint(__uint_as_float(w << 16) * kQ4Down),
+                                       __float_as_uint(__uint_as_float(w & 0xffff0000u) * kQ4Down), 0x7632);
+                };
+                u = make_uint4(times(u.x), times(u.y), times(u.z), times(u.w));
             }
             xs[(ch * nt + (r >> 3)) * 32 + (r & 7) * 4 + t] =
                 make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632), __byte_perm(u.y, u.w, 0x5410),
@@ -152,19 +170,47 @@ __device__ __forceinline__ void q4_cut(const Q4Args& a, uint4* xs, int nt, int k
                                __byte_perm(p[3], p[7], 0x7632));
             }
         };
-        bool finite = true;
+        if (DOWN && (down >> r & 1)) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) finite = finite && fabsf(v[j]) < INFINITY;
-        if (finite) {   // 8 at a time: a test for each piece cost more than the cut
+            for (int j = 0; j < 8; j++) v[j] *= kQ4Down;
+        }
+        bool plain = true;
+#pragma unroll
+        for (int j = 0; j < 8; j++) plain = plain && fabsf(v[j]) < kQ4Big;
+        if (plain) {   // 8 at a time: a test for each piece cost more than the cut
             cut([](float& f) {
                 const uint32_t b = __float_as_uint(f);
                 f -= __uint_as_float(b & 0xffff0000u);
                 return b;
             });
         } else {
+            large = true;
             cut(q4_piece);
         }
     }
+    return large;
+}
+
+// The rows that have finite values of kQ4Big and more, in these chunks or before: into *big, and cut again times kQ4Down.  Returns
+// those that are new.  By the whole block, and seldom: out of line, so that the way past it costs nothing.
+template <class T, int TERMS>
+__device__ __forceinline__ uint32_t q4_cut_large(const Q4Args& a, uint4* xs, int nt, int kb0, int kb1, uint32_t* big) {
+    const uint32_t was = *big;
+    __syncthreads();
+    const int k0 = kb0 * 32, n = min(kb1 * 32, a.w.cols) - k0;
+    for (int r = 0; r < a.m; r++) {
+        bool found = false;
+        for (int k = threadIdx.x; k < n; k += kQ4Threads) {
+            const float v = fabsf(q4_float(static_cast<const T*>(a.x)[r * a.ldx + k0 + k]));
+            found = found || (v >= kQ4Big && v < INFINITY);
+        }
+        if (found) atomicOr(big, 1u << r);
+    }
+    __syncthreads();
+    const uint32_t now = *big;
+    if (now) q4_cut<T, TERMS, true>(a, xs, nt, kb0, kb1, now);
+    __syncthreads();
+    return now ^ was;
 }
 
 // 8 values of 4 bits -> bf16 pairs (0,4), (1,5), (2,6), (3,7) of q - 8: 0x4300 is 128, its last bits count in ones
@@ -225,16 +271,18 @@ __device__ __forceinline__ void q4_scales(const Q4Args& a, const void* row, uint
 
 // NT: tiles of 8 columns, which hold the pieces of all rows of x.  P: chunks after which the scale is applied, the largest of 1, 2, 4 that divides a group's.
 template <int NT, int P>
-__global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const Q4Args a) {
+__global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const __grid_constant__ Q4Args a) {
     extern __shared__ __align__(16) uint8_t qsm[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    uint8_t* ring = qsm + warp * (kQ4Stages * kQ4StageBytes);
+    uint32_t* big = reinterpret_cast<uint32_t*>(qsm);
+    uint8_t* ring = qsm + 16 + warp * (kQ4Stages * kQ4StageBytes);
     uint4* xs = reinterpret_cast<uint4*>(qsm + kQ4RingBytes);
     const int chunks = (a.w.cols + 31) / 32;
     const int ks = 1 << a.ks_log2, rows = 16 * kQ4Warps >> a.ks_log2;   // warps on a tile, table rows of a block
     const int row0 = blockIdx.x * rows + (warp >> a.ks_log2) * 16, kq = warp & (ks - 1);
     const int scale_bytes = a.w.scale_type == FHE_F32 ? 4 : 2;
     float* sc = reinterpret_cast<float*>(xs + a.kb_chunks * NT * 32) + warp * 16 * a.units;   // [unit][16 rows]
+    if (tid == 0) *big = 0;
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -269,13 +317,23 @@ __global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const Q4Args a) {
             if (e + v <= (chunks + P - 1) / P) first = *reinterpret_cast<const uint4*>(srow + (size_t)e * scale_bytes);
         }
         __syncthreads();   // the previous block's pieces are read
-        if (a.xt == FHE_F32) q4_cut<float, 3>(a, xs, NT, kb0, kb1);
+        bool large = *big != 0;
+        if (a.xt == FHE_F32) large |= q4_cut<float, 3>(a, xs, NT, kb0, kb1);
         else if (a.xt == FHE_F16) q4_cut<__half, 2>(a, xs, NT, kb0, kb1);
-        else q4_cut<__nv_bfloat16, 1>(a, xs, NT, kb0, kb1);
+        else large |= q4_cut<__nv_bfloat16, 1>(a, xs, NT, kb0, kb1);
         if (a.w.scale_type == FHE_F16) q4_scales<__half, P>(a, srow, first, sc, c0, (c1 - c0) / P, chunks);
         else if (a.w.scale_type == FHE_BF16) q4_scales<__nv_bfloat16, P>(a, srow, first, sc, c0, (c1 - c0) / P, chunks);
         else q4_scales<float, P>(a, srow, first, sc, c0, (c1 - c0) / P, chunks);
-        __syncthreads();
+        if (__syncthreads_or(large)) {
+            const uint32_t more = a.xt == FHE_F32 ? q4_cut_large<float, 3>(a, xs, NT, kb0, kb1, big)
+                                                  : q4_cut_large<__nv_bfloat16, 1>(a, xs, NT, kb0, kb1, big);
+            // what was summed of the rows that are large from here on
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (more >> ((n * 8 + 2 * t + (j & 1)) / a.terms) & 1) acc[n][j] *= kQ4Down;
+        }
         const uint4* xc = xs + (size_t)(c0 - kb0) * NT * 32 + lane;
         const float* su = sc + g;
 #pragma unroll 4
@@ -316,7 +374,7 @@ __global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const Q4Args a) {
     }
     // [warp][column][16 rows], then the pieces and the ks warps' parts are added up
     __syncthreads();
-    float* so = reinterpret_cast<float*>(qsm) + warp * (NT * 8 * 16);
+    float* so = reinterpret_cast<float*>(qsm + 16) + warp * (NT * 8 * 16);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         so[(n * 8 + 2 * t) * 16 + g] = acc[n][0];
@@ -329,10 +387,11 @@ __global__ void __launch_bounds__(kQ4Threads, 3) k_q4_mma(const Q4Args a) {
     for (int i = tid; i < a.m << rows_log2; i += kQ4Threads) {
         const int r = i >> rows_log2, row = i & (rows - 1), at = blockIdx.x * rows + row;
         if (at >= a.w.rows) continue;
-        const float* sp = reinterpret_cast<const float*>(qsm) + ((row >> 4) << a.ks_log2) * (NT * 8 * 16) + (row & 15);
+        const float* sp = reinterpret_cast<const float*>(qsm + 16) + ((row >> 4) << a.ks_log2) * (NT * 8 * 16) + (row & 15);
         float v = 0.f;
         for (int k = 0; k < ks; k++)
             for (int j = a.terms - 1; j >= 0; j--) v += sp[k * (NT * 8 * 16) + (r * a.terms + j) * 16];
+        if (*big >> r & 1) v *= 1.f / kQ4Down;
         st_any(a.out, a.ot, (long long)r * a.ldo + at, v);
     }
 }

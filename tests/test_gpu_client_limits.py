@@ -1,7 +1,10 @@
 """The client's token step on the GPU at its limits: sizes that are refused, values at the ends of their types, memory that runs out,
 waits that run out."""
+import numpy as np
 import pytest
 import torch
+
+from test_gpu_client import check_product
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +119,76 @@ def test_a_product_refused_for_memory(cx):
     assert (client.q4_matvec(cx, few, t) == 0).all()
     del x
     trim_pool()
+
+
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m", [1, 2, 6, 8, 18, 40])
+@pytest.mark.parametrize("group", [32, 64, 128, 1024])
+def test_rows_near_the_end_of_float32(cx, group, m, xt):
+    """Rows of 10^37 with scales that bring the products back, beside ordinary rows: whole numbers times x alone would pass
+    float32's range.  The tolerance is the products' usual one."""
+    from fhessm import client
+    t = random_table(200, 500, group, seed=m, stype=torch.float32)
+    x = torch.randn(m, 500, device="cuda", dtype=torch.float64)
+    x[::2] *= 1e37
+    if m > 3:
+        x[3] = 0
+        x[3, 77] = torch.finfo(torch.float32).max if xt == torch.float32 else torch.finfo(xt).max
+    x = x.to(xt)
+    w = t.dequantise().double().cpu().numpy()
+    assert np.abs(x.double().cpu().numpy()).max() * 8 > 3.4e38 / 4
+    check_product(client.q4_matvec(cx, x, t), x, w, "f32")
+
+
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16])
+def test_large_values_in_some_columns_only(cx, xt):
+    """Rows long enough to be taken in several blocks of columns, with their large values in the first, the last or a middle
+    one, or in none."""
+    from fhessm import client
+    cols = 40000
+    t = random_table(40, cols, 64, stype=torch.float32)
+    x = torch.randn(2, 4, cols, device="cuda", dtype=torch.float64)
+    x[0, 0, :50] *= 1e37
+    x[0, 1, -50:] *= 1e37
+    x[1, 0, 20000:20050] *= 1e37
+    x[1, 2, 3::5000] *= 1e37
+    w = t.dequantise().double().cpu().numpy()
+    for rows in (x[0, :2], x[0, :1], x[1, :2], x[1, 2:]):
+        rows = rows.to(xt).contiguous()
+        check_product(client.q4_matvec(cx, rows, t), rows, w, "f32")
+
+
+@pytest.mark.parametrize("xt", [torch.float32, torch.bfloat16])
+def test_an_infinity_beside_large_values(cx, xt):
+    from fhessm import client
+    t = random_table(150, 100, 32, stype=torch.float32)
+    x = torch.randn(2, 100, device="cuda")
+    x[0] *= 1e37
+    x[0, 40] = float("inf")
+    x = x.to(xt)
+    w = t.dequantise().cpu().numpy()[:, 40]
+    got = client.q4_matvec(cx, x, t).cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want = np.where(w == 0, np.nan, np.sign(w) * np.inf)
+    assert np.array_equal(got[0], want, equal_nan=True)
+    check_product(torch.from_numpy(got[1:]), x[1:], t.dequantise().double().cpu().numpy(), "f32")
+
+
+@pytest.mark.parametrize("m", [1, 12, 64])
+def test_not_finite_in_float16(cx, m):
+    """An infinity or NaN in one row stays in that row, and gives there what the sum of the products is."""
+    from fhessm import client
+    t = random_table(150, 100, 32)
+    x = torch.randn(m, 100, device="cuda").half()
+    r = m // 2
+    x[r, 40] = -float("inf")
+    w = t.dequantise().double().cpu().numpy()
+    got = client.q4_matvec(cx, x, t).cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want = np.where(w[:, 40] == 0, np.nan, -np.sign(w[:, 40]) * np.inf)
+    assert np.array_equal(got[r], want, equal_nan=True)
+    rest = np.arange(m) != r
+    if rest.any():
+        check_product(torch.from_numpy(got[rest]), x[torch.from_numpy(rest).cuda()], w, "f32")
+    x[r, 41] = float("nan")
+    assert torch.isnan(client.q4_matvec(cx, x, t)[r]).all()
