@@ -1595,10 +1595,26 @@ void client_table(const fhe::Context& c, const fhe_q4* w) {
     client_ptr(c, w->scale, sb, "q4 scales");
 }
 
-cudaStream_t client_stream(fhe_ctx* cx, void* stream) {
-    CUDA_CHECK(cudaSetDevice(cx->cx.device));
+cudaStream_t client_stream(const fhe_ctx* cx, void* stream) {
     return stream ? static_cast<cudaStream_t>(stream) : cx->cx.stream;
 }
+
+// The context's GPU is the thread's current one for the length of a call, and the caller's again after it: these calls stand among
+// torch's, which put theirs back.
+struct ClientDevice {
+    int was = -1;
+    explicit ClientDevice(int device) {
+        int now = -1;
+        CUDA_CHECK(cudaGetDevice(&now));
+        if (now == device) return;
+        CUDA_CHECK(cudaSetDevice(device));
+        was = now;
+    }
+    ~ClientDevice() {
+        if (was >= 0) cudaSetDevice(was);
+    }
+    ClientDevice(const ClientDevice&) = delete;
+};
 
 }  // namespace
 
@@ -1614,6 +1630,7 @@ extern "C" int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_
         if (m == 0 || w->rows == 0) return;
         client_ptr(cx->cx, x, xb, "x");
         client_ptr(cx->cx, out, ob, "out");
+        const ClientDevice on(cx->cx.device);
         cudaStream_t st = client_stream(cx, stream);
         fhe::q4_matvec(cx->cx, fhe::Q4Args{*w, x, x_type, 0, m, ldx, out, out_type, ldo, 0, 0, 0, 0, 0, 0}, st);
     });
@@ -1630,6 +1647,7 @@ extern "C" int fhe_q4_rows(fhe_ctx* cx, const fhe_q4* w, const int64_t* tokens, 
         if (m == 0) return;
         client_ptr(cx->cx, tokens, 8, "tokens");
         client_ptr(cx->cx, out, ob, "out");
+        const ClientDevice on(cx->cx.device);
         cudaStream_t st = client_stream(cx, stream);
         if (out_type == FHE_F32) fhe::q4_rows<float>(cx->cx, *w, tokens, m, out, ldo, st);
         else if (out_type == FHE_F16) fhe::q4_rows<__half>(cx->cx, *w, tokens, m, out, ldo, st);
@@ -1659,6 +1677,7 @@ extern "C" int fhe_sample(fhe_ctx* cx, const fhe_sample_cfg* cfg, const void* lo
         if (cfg->top_k) client_ptr(cx->cx, cfg->top_k, 4, "top_k");
         if (cfg->top_p) client_ptr(cx->cx, cfg->top_p, 4, "top_p");
         if (cfg->min_p) client_ptr(cx->cx, cfg->min_p, 4, "min_p");
+        const ClientDevice on(cx->cx.device);
         cudaStream_t st = client_stream(cx, stream);
         fhe::SampleArgs a{logits, ld, type, rows, vocab, u, cfg->temperature, cfg->top_p, cfg->min_p, cfg->top_k,
                           cfg->temperature_all, cfg->top_p_all, cfg->min_p_all, cfg->top_k_all, token, logprob};

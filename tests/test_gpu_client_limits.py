@@ -192,3 +192,30 @@ def test_not_finite_in_float16(cx, m):
         check_product(torch.from_numpy(got[rest]), x[torch.from_numpy(rest).cuda()], w, "f32")
     x[r, 41] = float("nan")
     assert torch.isnan(client.q4_matvec(cx, x, t)[r]).all()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_the_current_device_stays():
+    """A context on a GPU other than the current one: each call leaves the current one current, refused calls too."""
+    import fhessm
+    from fhessm import FheError, client
+    from fhessm.client import Q4Table
+    c = fhessm.CryptoContext(logN=12, L=2, K=1, alpha=1, hw=64, device=1)
+    torch.cuda.set_device(0)
+    t = random_table(64, 100, 32)
+    t = Q4Table(t.weight.to("cuda:1"), t.scale.to("cuda:1"), cols=100, group=32)
+    x, u = torch.randn(20, 100, device="cuda:1"), torch.rand(20, device="cuda:1")
+    assert torch.cuda.current_device() == 0
+    for rows in (x[:1], x):
+        logits = client.q4_matvec(c, rows, t)
+        assert torch.cuda.current_device() == 0
+        check_product(logits, rows, t.dequantise().double().cpu().numpy(), "f32")
+    token, _ = client.sample(c, logits, u, top_k=5)
+    assert torch.cuda.current_device() == 0
+    assert torch.equal(client.q4_rows(c, token, t), t.dequantise()[token])
+    assert torch.cuda.current_device() == 0
+    with pytest.raises(FheError):
+        client.sample(c, logits, u, temperature=-1.0)
+    assert torch.cuda.current_device() == 0
+    c.close()
+    torch.cuda.set_device(0)
