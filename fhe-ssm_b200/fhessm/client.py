@@ -12,7 +12,8 @@ a scale for each group of columns, and the three steps are kernels:
 
 Tensors are torch tensors on the context's GPU; calls are enqueued on torch's current stream of that
 GPU, like any torch operation, and do not synchronise.  A call that cannot be served raises
-``FheError``; nothing is converted or copied silently.
+``FheError``; nothing is converted or copied silently, and no gradient is dropped: an operand that
+requires one is refused unless gradients are off.
 """
 import ctypes as C
 import struct
@@ -64,6 +65,14 @@ def _stream(device):
 def _on_gpu(device, t, what):
     if not t.is_cuda or t.get_device() != device:
         raise _bad(f"{what} is not on the context's GPU (cuda:{device})")
+
+
+def _no_gradient(*named):
+    # nothing here is differentiable: a gradient that somebody waits for is refused, not dropped
+    if torch.is_grad_enabled():
+        for t, what in named:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise _bad(f"{what} requires a gradient, which this call does not have: detach it, or call under torch.no_grad()")
 
 
 def _rows_of(t, what):
@@ -123,7 +132,8 @@ class Q4Table:
     def quantise(cls, w, *, group=64, scale_dtype=torch.float16, device="cpu"):
         """The 4-bit table nearest to w (rows x cols, a float array or tensor): a group's scale is its largest
         magnitude over 7, rounded to scale_dtype."""
-        w = torch.as_tensor(np.asarray(w) if not torch.is_tensor(w) else w).to(device=device, dtype=torch.float32)
+        w = w.detach() if torch.is_tensor(w) else torch.as_tensor(np.asarray(w))
+        w = w.to(device=device, dtype=torch.float32)
         if w.dim() != 2 or group < 32 or group % 32:
             raise _bad("quantise: rows x cols and a group that is a multiple of 32")
         rows, cols = w.shape
@@ -163,6 +173,7 @@ def q4_matvec(cx, x, table, *, dtype=torch.float32, out=None):
     """x (m, cols) times the table's transpose: (m, rows) of `dtype` (fhe_q4_matvec).  x: float32,
     float16 or bfloat16 with contiguous rows (any row stride), 2^21 of them at most."""
     xt, m, k, ldx = _rows_of(x, "x")
+    _no_gradient((x, "x"), (table.scale, "the table's scale"), (out, "out"))
     if k != table.cols:
         raise _bad(f"x has {k} columns, the table {table.cols}")
     device = cx.p.device
@@ -180,6 +191,7 @@ def q4_rows(cx, tokens, table, *, dtype=torch.float32, out=None):
     outside the table (the -1 of an empty row) gives zeros."""
     if tokens.dim() != 1 or tokens.dtype != torch.int64 or not tokens.is_contiguous():
         raise _bad("tokens: a contiguous int64 vector")
+    _no_gradient((table.scale, "the table's scale"), (out, "out"))
     device = cx.p.device
     _on_gpu(device, tokens, "tokens")
     if table.device != device:
@@ -207,6 +219,7 @@ def sample(cx, logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     one number or a vector with a value for each row (float32; top_k int32).  temperature 0: the
     largest logit.  top_k 0, top_p 1 and min_p 0 are off.  The token of a row that allows none is -1."""
     lt, rows, vocab, ld = _rows_of(logits, "logits")
+    _no_gradient((logits, "logits"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (u, "u"))
     device = cx.p.device
     _on_gpu(device, logits, "logits")
     if not 1 <= vocab <= MAX_VOCAB:

@@ -1,6 +1,10 @@
 """Limits of the client's token step that need no GPU: what a table may be, and what its values become."""
+from types import SimpleNamespace
+
 import pytest
 import torch
+
+ON_GPU_0 = SimpleNamespace(p=SimpleNamespace(device=0), h=None)    # a context as far as the checks of arguments look
 
 
 @pytest.mark.parametrize("rows,ok", [(1 << 30, True), ((1 << 30) + 1, False), ((1 << 31) - 1, False), ((1 << 31) + 5, False)])
@@ -14,3 +18,33 @@ def test_rows_of_a_table(rows, ok):
     else:
         with pytest.raises(FheError, match="rows at most"):
             Q4Table(w, s, cols=32, group=32)
+
+
+def test_gradients_are_refused():
+    """An operand, an output or a setting that requires a gradient: refused before anything else is looked at, served where
+    gradients are off (then these host tensors are refused for what they are)."""
+    from fhessm import FheError, client
+    w = torch.zeros(4, 32, dtype=torch.uint8)
+    table = client.Q4Table(w, torch.ones(4, 2), cols=64, group=32)
+    learnt = client.Q4Table(w, torch.ones(4, 2, requires_grad=True), cols=64, group=32)
+    x, u, ids = torch.ones(2, 64), torch.zeros(2), torch.zeros(2, dtype=torch.int64)
+    f = lambda *shape: torch.ones(*shape, requires_grad=True)
+    for call in [lambda: client.q4_matvec(ON_GPU_0, f(2, 64), table), lambda: client.q4_matvec(ON_GPU_0, x, learnt),
+                 lambda: client.q4_matvec(ON_GPU_0, x, table, out=f(2, 4)), lambda: client.q4_rows(ON_GPU_0, ids, learnt),
+                 lambda: client.q4_rows(ON_GPU_0, ids, table, out=f(2, 64)), lambda: client.sample(ON_GPU_0, f(2, 9), u),
+                 lambda: client.sample(ON_GPU_0, torch.ones(2, 9), u, temperature=f(2)),
+                 lambda: client.sample(ON_GPU_0, torch.ones(2, 9), u, top_p=f(2)),
+                 lambda: client.sample(ON_GPU_0, torch.ones(2, 9), u, min_p=f(2)),
+                 lambda: client.sample(ON_GPU_0, torch.ones(2, 9), f(2))]:
+        with pytest.raises(FheError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(FheError, match="not on the context's GPU"):
+            call()
+
+
+def test_quantise_takes_a_parameter():
+    """The nearest table is no differentiable function of the weights: it holds none of their graph."""
+    from fhessm.client import Q4Table
+    w = torch.nn.Parameter(torch.randn(3, 64))
+    t = Q4Table.quantise(w, group=32)
+    assert not t.scale.requires_grad and torch.equal(t.weight, Q4Table.quantise(w.detach(), group=32).weight)
