@@ -142,6 +142,8 @@ class Q4Table:
         wide[:, :cols] = w
         wide = wide.view(rows, groups, group)
         scale = (wide.abs().amax(2) / 7).to(scale_dtype)
+        if not torch.isfinite(scale).all():
+            raise _bad(f"quantise: values that are not finite, or too large for a scale in {scale_dtype}")
         s = scale.float().unsqueeze(2)
         q = torch.where(s > 0, torch.round(wide / torch.where(s > 0, s, torch.ones_like(s))), torch.zeros_like(wide))
         q = (q.clamp(-8, 7) + 8).to(torch.uint8).view(rows, -1)[:, :-(-cols // 32) * 32]

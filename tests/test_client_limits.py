@@ -48,3 +48,17 @@ def test_quantise_takes_a_parameter():
     w = torch.nn.Parameter(torch.randn(3, 64))
     t = Q4Table.quantise(w, group=32)
     assert not t.scale.requires_grad and torch.equal(t.weight, Q4Table.quantise(w.detach(), group=32).weight)
+
+
+@pytest.mark.parametrize("value,dtype", [(float("inf"), torch.float32), (float("nan"), torch.bfloat16), (-5e5, torch.float16)])
+def test_quantise_refuses_what_no_scale_holds(value, dtype):
+    """A group's scale is its largest magnitude over 7: 65,504 x 7 = 458,528 is the end of float16's."""
+    from fhessm import FheError
+    from fhessm.client import Q4Table
+    w = torch.ones(3, 100)
+    w[1, 70] = value
+    with pytest.raises(FheError, match="scale"):
+        Q4Table.quantise(w, group=32, scale_dtype=dtype)
+    w[1, 70] = 4.5e5
+    t = Q4Table.quantise(w, group=32, scale_dtype=dtype)
+    assert torch.isfinite(t.dequantise()).all()
