@@ -16,6 +16,7 @@ GPU, like any torch operation, and do not synchronise.  A call that cannot be se
 requires one is refused unless gradients are off.
 """
 import ctypes as C
+import operator
 import struct
 
 import numpy as np
@@ -94,6 +95,13 @@ def _rows_of(t, what):
     return kind, m, n, ld if m > 1 else n
 
 
+def _whole(what, *values):
+    try:
+        return [operator.index(v) for v in values]
+    except TypeError:
+        raise _bad(f"{what}: columns and group are whole numbers") from None
+
+
 class Q4Table:
     """A table of rows x cols values in 4 bits with a scale for each `group` columns of a row:
     value (i, c) = scale[i, c // group] * (q - 8), q the low (even c) or high (odd c) half of byte
@@ -106,6 +114,7 @@ class Q4Table:
         if weight.dtype != torch.uint8 or weight.dim() != 2:
             raise _bad("q4 table: weight is a uint8 tensor, rows x bytes")
         rows, nbytes = weight.shape
+        cols, group = _whole("q4 table", cols, group)
         if not 1 <= cols <= MAX_COLS or group < 32 or group % 32 or group >= 1 << 31:
             raise _bad(f"q4 table: 1 to {MAX_COLS} columns and a group that is a multiple of 32")
         if rows > MAX_ROWS:
@@ -134,8 +143,11 @@ class Q4Table:
         magnitude over 7, rounded to scale_dtype."""
         w = w.detach() if torch.is_tensor(w) else torch.as_tensor(np.asarray(w))
         w = w.to(device=device, dtype=torch.float32)
+        group, = _whole("quantise", group)
         if w.dim() != 2 or group < 32 or group % 32:
             raise _bad("quantise: rows x cols and a group that is a multiple of 32")
+        if scale_dtype not in _TYPES:
+            raise _bad(f"quantise: scales in float32, float16 or bfloat16, not {scale_dtype}")
         rows, cols = w.shape
         groups = -(-cols // group)
         wide = torch.zeros(rows, groups * group, dtype=torch.float32, device=w.device)
@@ -146,7 +158,7 @@ class Q4Table:
             raise _bad(f"quantise: values that are not finite, or too large for a scale in {scale_dtype}")
         s = scale.float().unsqueeze(2)
         q = torch.where(s > 0, torch.round(wide / torch.where(s > 0, s, torch.ones_like(s))), torch.zeros_like(wide))
-        q = (q.clamp(-8, 7) + 8).to(torch.uint8).view(rows, -1)[:, :-(-cols // 32) * 32]
+        q = (q.clamp(-8, 7) + 8).to(torch.uint8).view(rows, groups * group)[:, :-(-cols // 32) * 32]
         return cls((q[:, 0::2] | q[:, 1::2] << 4).contiguous(), scale.contiguous(), cols=cols, group=group)
 
     def to(self, device):

@@ -62,3 +62,19 @@ def test_quantise_refuses_what_no_scale_holds(value, dtype):
     w[1, 70] = 4.5e5
     t = Q4Table.quantise(w, group=32, scale_dtype=dtype)
     assert torch.isfinite(t.dequantise()).all()
+
+
+def test_a_table_of_no_rows_and_sizes_that_are_no_whole_numbers():
+    import numpy as np
+    from fhessm import FheError
+    from fhessm.client import Q4Table
+    w, s = torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 2)
+    assert Q4Table(w, s, cols=np.int64(64), group=np.int32(32)).cols == 64
+    for kw in (dict(cols=64.0, group=32), dict(cols=64, group=32.0), dict(cols="64", group=32), dict(cols=64, group=None)):
+        with pytest.raises(FheError):
+            Q4Table(w, s, **kw)
+    empty = Q4Table.quantise(torch.zeros(0, 70), group=32)
+    assert empty.rows == 0 and empty.dequantise().shape == (0, 70)
+    for kw in (dict(group=32.0), dict(group=48), dict(group=32, scale_dtype=torch.float64), dict(group=32, scale_dtype=torch.int8)):
+        with pytest.raises(FheError):
+            Q4Table.quantise(torch.ones(2, 64), **kw)
