@@ -50,6 +50,8 @@ def main():
         normed = unpack_lanes(cx.Decrypt(model.step(ct)), cfg.D, lanes, cfg.d)
         u = torch.rand(lanes, generator=rng, device=rng.device)
         tokens, logprob, rows = head.step(normed, u, temperature=a.temperature, top_k=a.top_k, top_p=a.top_p)
+        torch.cuda.current_stream().synchronize()
+        cx.sync()                                            # raises if the tick lost anything to a wait that ran out
         print(f"tick {tick}: {lanes} conversations, mean log-probability {logprob.mean().item():.3f}, "
               f"first tokens {tokens[:8].tolist()}")
     cx.close()

@@ -185,7 +185,8 @@ def _out(out, like, m, n, dtype, device):
 
 def q4_matvec(cx, x, table, *, dtype=torch.float32, out=None):
     """x (m, cols) times the table's transpose: (m, rows) of `dtype` (fhe_q4_matvec).  x: float32,
-    float16 or bfloat16 with contiguous rows (any row stride), 2^21 of them at most."""
+    float16 or bfloat16 with contiguous rows (any row stride), 2^21 of them at most.  A kernel whose bounded wait
+    runs out leaves NaN, and ``cx.sync()`` raises once the stream is synchronised."""
     xt, m, k, ldx = _rows_of(x, "x")
     _no_gradient((x, "x"), (table.scale, "the table's scale"), (out, "out"))
     if k != table.cols:
@@ -274,6 +275,8 @@ class TokenHead:
         return q4_rows(self.cx, tokens, self.table)
 
     def step(self, hidden, u, **settings):
-        """(tokens, log-probabilities, embedded rows) of the next tick; `settings` as in sample()."""
+        """(tokens, log-probabilities, embedded rows) of the next tick; `settings` as in sample().  Logits that were lost
+        (q4_matvec's NaN) come out as token -1 and a row of zeros: call ``cx.sync()`` once a tick, when the stream is
+        synchronised, which raises for them."""
         tokens, logprob = sample(self.cx, self.logits(hidden), u, **settings)
         return tokens, logprob, self.embed(tokens)

@@ -415,7 +415,10 @@ typedef struct {
  * Sums are held in 32 bits and rounded once to the output's type.  One row or a few take one launch.  For more, x's
  * operand (about 4 m cols bytes) is laid out in memory that the call takes from the stream's pool and gives back to
  * it (cudaMallocAsync); float32 values are then held to 22 bits, and values under 2^-16 of their row's largest, float16's
- * aside, to 2^-39 of it. */
+ * aside, to 2^-39 of it.  That kernel's waits are bounded: where one runs out (a fault, or a GPU that is shared with work
+ * that starves it) the call still returns FHE_OK, as its work is enqueued, the outputs that it did not reach are NaN, and the
+ * next fhe_ctx_sync after the stream has been synchronised returns the error.  fhe_sample reads NaN as "not allowed", so a
+ * caller who feeds one call's output to the next asks once a step. */
 int fhe_q4_matvec(fhe_ctx* cx, const fhe_q4* w, const void* x, int x_type, long long ldx, int m, void* out,
                   int out_type, long long ldo, void* stream);
 /* out[r] = row tokens[r] of the table; a token outside [0, rows) gives a row of zeros */

@@ -219,3 +219,37 @@ def test_the_current_device_stays():
     assert torch.cuda.current_device() == 0
     c.close()
     torch.cuda.set_device(0)
+
+
+def test_a_lost_step_is_reported(cx):
+    """Lost logits pass the choice and the look-up as "nothing allowed"; the sync after the step tells."""
+    from fhessm import FheError, client
+    head = client.TokenHead(cx, random_table(50304, 1024, 64))
+    hidden, u = torch.randn(64, 1024, device="cuda"), torch.rand(64, device="cuda")
+    want, _, _ = head.step(hidden, u, top_k=50)
+    torch.cuda.synchronize()
+    cx.sync()
+    cx.set_option("q4_waits", 0)
+    try:
+        tokens, _, rows = head.step(hidden, u, top_k=50)
+    finally:
+        cx.set_option("q4_waits", -1)
+    torch.cuda.synchronize()
+    assert (tokens == -1).any() and (rows[tokens == -1] == 0).all()
+    with pytest.raises(FheError, match="wait"):
+        cx.sync()
+    tokens, _, _ = head.step(hidden, u, top_k=50)
+    torch.cuda.synchronize()
+    cx.sync()
+    assert torch.equal(tokens, want)
+
+
+def test_the_example_runs():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, os.path.join(root, "examples", "decode_loop.py"), "--ticks", "2"], timeout=300,
+                         capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr[-2000:]
+    assert out.stdout.count("mean log-probability -") == 2
