@@ -185,8 +185,9 @@ def _out(out, like, m, n, dtype, device):
 
 def q4_matvec(cx, x, table, *, dtype=torch.float32, out=None):
     """x (m, cols) times the table's transpose: (m, rows) of `dtype` (fhe_q4_matvec).  x: float32,
-    float16 or bfloat16 with contiguous rows (any row stride), 2^21 of them at most.  A kernel whose bounded wait
-    runs out leaves NaN, and ``cx.sync()`` raises once the stream is synchronised."""
+    float16 or bfloat16 with contiguous rows (any row stride), 2^21 of them at most.  Two float32 rows at a time are
+    held whole; of more, on most tables, a value is held to 22 bits and to 2^-39 of its row's largest.  A kernel whose
+    bounded wait runs out leaves NaN, and ``cx.sync()`` raises once the stream is synchronised."""
     xt, m, k, ldx = _rows_of(x, "x")
     _no_gradient((x, "x"), (table.scale, "the table's scale"), (out, "out"))
     if k != table.cols:

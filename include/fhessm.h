@@ -412,10 +412,15 @@ typedef struct {
     long long ldq, lds;
 } fhe_q4;
 /* out[r][i] = sum_c x[r][c] W[i][c] for m rows of x, at most FHE_Q4_MAX_M (the head: W is vocabulary x d).
- * Sums are held in 32 bits and rounded once to the output's type.  One row or a few take one launch.  For more, x's
- * operand (about 4 m cols bytes) is laid out in memory that the call takes from the stream's pool and gives back to
- * it (cudaMallocAsync); float32 values are then held to 22 bits, and values under 2^-16 of their row's largest, float16's
- * aside, to 2^-39 of it.  That kernel's waits are bounded: where one runs out (a fault, or a GPU that is shared with work
+ * Sums are held in 32 bits and rounded once to the output's type.
+ * Two kernels share the calls, by m times the pieces of x's type (3 for float32, 2 for float16, 1 for bfloat16).  Up to 8 of them
+ * (18 for tables of less than 16,384 rows and 1,536 columns, and for those of more than 16,384 rows whose group is no multiple
+ * of 64) take one launch that holds x whole.  For more, x's operand (2 bytes a value, 4 for float32, of whole 16, 32 or 64 rows
+ * and 128 columns) is laid out in memory that the call takes from the stream's pool and gives back to it
+ * (cudaMallocAsync), in units of each row's largest finite value: float32 is then held to 22 bits, and float32 and bfloat16 to no
+ * less than 2^-39 of that value.  So the last bits of a row's output depend on how many rows share the call; who needs
+ * float32 rows whole passes two at a time.  Sums in these units stay in float32's range for scales up to 2^90.  The
+ * second kernel's waits are bounded: where one runs out (a fault, or a GPU that is shared with work
  * that starves it) the call still returns FHE_OK, as its work is enqueued, the outputs that it did not reach are NaN, and the
  * next fhe_ctx_sync after the stream has been synchronised returns the error.  fhe_sample reads NaN as "not allowed", so a
  * caller who feeds one call's output to the next asks once a step. */

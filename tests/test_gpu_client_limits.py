@@ -253,3 +253,30 @@ def test_the_example_runs():
                          capture_output=True, text=True)
     assert out.returncode == 0, out.stderr[-2000:]
     assert out.stdout.count("mean log-probability -") == 2
+
+
+@pytest.mark.parametrize("rows,whole", [(16384, 8), (1000, 18)])
+@pytest.mark.parametrize("xt,pieces", [(torch.float32, 3), (torch.float16, 2), (torch.bfloat16, 1)])
+def test_how_x_is_held(cx, rows, whole, xt, pieces):
+    """Table rows with a single one among zeros read x out: whole while rows of x times the pieces of its type are at most `whole`,
+    to 22 bits (float32) and to 2^-39 of the row's largest value above, which stands where a table row may hold zero."""
+    from fhessm import client
+    cols = 128
+    q = torch.full((rows, cols), 8, dtype=torch.uint8, device="cuda")
+    at = torch.arange(rows, device="cuda")
+    q[at, at % cols] = 9
+    t = client.Q4Table(q[:, 0::2] | q[:, 1::2] << 4, torch.ones(rows, 2, device="cuda"), cols=cols, group=64)
+    for m in (1, whole // pieces, whole // pieces + 1, 20, 64):
+        x = torch.randn(m, cols, device="cuda") * torch.exp2(torch.randint(-12, 13, (m, cols), device="cuda").float())
+        if xt != torch.float16:
+            x[:, 5] *= 2.0 ** 24
+            x[:, 9] = 2.0 ** -30
+        x = x.to(xt)
+        got = client.q4_matvec(cx, x, t)[:, :cols].double()
+        x = x.double()
+        if m * pieces <= whole or xt == torch.float16:
+            assert torch.equal(got, x)
+        else:
+            held = 2.0 ** -22 * x.abs() if xt == torch.float32 else 0
+            assert ((got - x).abs() <= held + 2.0 ** -39 * x.abs().amax(1, keepdim=True)).all()
+            assert not torch.equal(got, x)
