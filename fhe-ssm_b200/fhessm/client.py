@@ -259,7 +259,9 @@ def sample(cx, logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
 class TokenHead:
     """The client's side of a decode tick with a tied 4-bit table: decrypted normed rows in, tokens and the
-    next tick's input rows out."""
+    next tick's input rows out.  Only for a tied table: a model with an embedding of its own (RWKV-7) takes
+    q4_matvec with its head's table, after its output norm, and q4_rows with its embedding's, into which its
+    input norm is folded."""
 
     def __init__(self, cx, table):
         self.cx = cx
