@@ -257,7 +257,10 @@ struct ProfScope {
 // A kernel launched by launch_pdl may be scheduled while the previous kernel on the stream is
 // still running: its CTAs start, run pdl_wait() -- which returns once the previous grid has
 // completed and its writes are visible -- and only then touch memory.  Every kernel launched this
-// way calls pdl_wait() before its first global load or store; pdl_trigger() lets the next grid be
+// way calls pdl_wait() before its first global load or store of what an earlier kernel may still
+// write or read.  k_q4_gemm alone reads something before: its table and scales, which no kernel of
+// its own call writes, and whatever wrote them ended before k_q4_pack began, since that one is
+// launched the ordinary way (and has to stay so).  pdl_trigger() lets the next grid be
 // scheduled as soon as all of this grid's CTAs have started.  For a kernel launched the ordinary
 // way both are no-ops.  What is gained is the gap between dependent kernels (scheduling the next
 // grid, its CTAs' start-up), which dominates the short launches of small batches.
