@@ -54,10 +54,10 @@ static void client_smem(const Context& cx) {
 // 8 values is a lane's share of two steps: the pairs (0,4), (1,5), (2,6), (3,7) come out of the word by one
 // mask each.  Several warps share 16 rows where the table is short, each a part of the columns.
 //
-// One bfloat16 row on 50,304 x 1,024 at groups of 64 takes 12.0 us (27.5 MB: 2.3 TB/s, 36% of a copy's rate), on 16,384 x 4,096
-// 15.9 us, on 4,096 x 1,024 4.1 us; 8 rows on 50,304 x 1,024 14.4 us.  About 3 us are the launch, x's pieces and the
+// One bfloat16 row on 50,304 x 1,024 at groups of 64 takes 11.6 us (27.5 MB: 2.4 TB/s, 37% of a copy's rate), on 16,384 x 4,096
+// 16.2 us, on 4,096 x 1,024 4.1 us; 8 rows on 50,304 x 1,024 14.1 us.  About 3 us are the launch, x's pieces and the
 // scales, a round trip each; then the loop, which waits for the table's bytes 3% of its time: instructions bound it,
-// 55% of the issue slots and 53% of the integer pipe over the whole kernel (unpacking: 7 integer operations and 4 subtractions
+// 54% of the issue slots and 51% of the integer pipe over the whole kernel (unpacking: 7 integer operations and 4 subtractions
 // for 8 values), with the 24 warps an SM that the ring leaves room for.  More and smaller blocks cut x more often: 16,384 x
 // 4,096 by 4 warps a tile takes 20.5 us.
 constexpr int kQ4Warps = 8, kQ4Threads = 32 * kQ4Warps;
@@ -521,7 +521,7 @@ static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
 
 // ---- rows of a 4-bit table by token id --------------------------------------------------------
 // A thread takes 8 columns: one 32-bit load, one scale, 16 or 32 bytes out.  What it costs is one round trip for the token, one
-// for its row and scale, and the output's bytes: 64 rows of 1,024 columns take 2.6 us, 2,048 rows 4.7 us (9.5 MB: 2.0 TB/s).
+// for its row and scale, and the output's bytes: 64 rows of 1,024 columns take 2.0 us, 2,048 rows 4.1 us (9.5 MB: 2.3 TB/s).
 // A token outside the table gives zeros.
 template <class T>
 __global__ void __launch_bounds__(128) k_q4_rows(const fhe_q4 w, const int64_t* __restrict__ tokens, T* __restrict__ out,
