@@ -412,7 +412,7 @@ static void q4_mma_launch(Context& cx, Q4Args a, cudaStream_t st) {
     // As many columns at a time as fit (512 bytes a chunk and tile of pieces, 512 a scale for 8 warps' rows), in equal blocks.  Two
     // blocks an SM where there are as many: one row on 16,384 x 4,096 took 18.1 us by 2,048 columns, 21.9 by all of them.
     const int each = kQ4Warps >> a.ks_log2, grid = (tiles + each - 1) / each;
-    const int step = kQ4Stage << a.ks_log2, room = (grid > 148 ? 114688 : 212992) - kQ4RingBytes;
+    const int step = kQ4Stage << a.ks_log2, room = (grid > 148 ? 114704 : 213008) - kQ4RingBytes;
     const int fit = std::max(step, room / (512 * NT + 512 / P) / step * step), turns = (chunks + fit - 1) / fit;
     a.kb_chunks = ((chunks + turns - 1) / turns + step - 1) / step * step;
     a.units = (a.kb_chunks >> a.ks_log2) / P;
@@ -503,7 +503,7 @@ static void q4_matvec(Context& cx, Q4Args a, cudaStream_t st) {
     //     50,304 x 1,024   8: 14.4, 17.8   9: 19.2, 18.1      16,384 x 4,096    8: 21.2, 22.0  10: 33.5, 21.9
     //     32,768 x 2,048   8: 18.5, 22.2  10: 21.6, 22.1       1,024 x 4,096    8:  9.2,  9.3  10: 13.3, 9.3
     // a small table, where k_q4_gemm's two launches weigh more, and groups of 32, where it adds up every 32 columns, on a long one:
-    //      4,096 x 1,024  18:  8.2,  9.6      32,768 x 2,048, groups of 32  18: 30.9, 31.7  20: 32.2, 31.6
+    //      4,096 x 1,024  18:  8.2,  9.6      32,768 x 2,048, groups of 32  18: 31.8, 31.7  20: 32.2, 31.6
     const int pieces = a.m * a.terms;
     const int most = (a.w.rows < 16384 && a.w.cols < 1536) || (a.w.rows > 16384 && a.w.group % 64) ? 18 : 8;
     if (pieces > most) {
